@@ -1,0 +1,979 @@
+// The whole MoE layer for up to 32 tokens in two launches: x [T, H] and the router's weights in, out [T, H] out.
+//
+//   route    logits = x Wr^T in fp32 (clusters of eight blocks, a slice of H each), x laid out as the tensor core's second operand
+//   experts  top-k of every token (each block for itself), the experts that are hit, fc1 + SwiGLU, fc2, sum over the experts
+//
+// What bounds it: the weights of the experts hit, once from HBM. Everything else is arranged around that stream:
+//   - The weights are the tensor core's first operand (M = 128 weight rows), all T tokens the second (N), for every expert that any
+//     token chose; columns of tokens that did not choose it are computed and dropped. So there is no sort, no gather and no
+//     dependence of the weight stream on who chose what. The MMAs take a fraction of the time that the weights take to arrive.
+//   - FP8 weights meet activations that are not quantised: a value x of a group of 128 is split into hi + lo / 16, both e4m3, times a
+//     power of two s with 128 <= amax / s < 256. e4m3 has four significant bits and the rest of a bf16 value after its first four has
+//     four more, so the split is exact down to 2^-13 of the group's largest value and off by at most 2^-21 of that below it. hi and lo
+//     are separate columns of the same MMA: N = 2 T, no conversion of weights, which go from memory to the tensor core untouched. The
+//     intermediate (fp32) is split the same way, within 2^-9 of each value (bf16's half step is 2^-8); with bf16 weights into two bf16.
+//   - Each phase is a list of 32 KiB units (fc1: 128 gate and 128 value rows x 128 bytes; fc2: 128 rows x 256 bytes), cut into one
+//     equal share per SM, whatever the tiles (streamk.cuh).
+//   - fc2's weights are fetched into the ring while the last parts of fc1 are still being summed; only the second operand waits.
+// Shares are claimed from a counter, fc1's before fc2's: a block waits for parts of fc1 only when each of them belongs to a block that
+// is running, so the wait ends also where not all blocks fit the GPU at once (another stream's kernels, several of these among them).
+//
+// No counterpart in the reference, whose runner (csrc/moe_kernels.h:770-892) takes routed rows and five launches.
+#include <mutex>
+
+#include "common.cuh"
+#include "gemm_tile.cuh"
+#include "ptx_sm100.cuh"
+#include "route_topk.cuh"
+#include "streamk.cuh"
+
+namespace dq {
+namespace moe_decode {
+
+constexpr int kMaxTokens = 32;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopk = 32;
+constexpr int kThreads = 256;                 // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue; all of them choose the experts
+constexpr int kRows = 128;                    // weight rows of an MMA
+constexpr int kKBytes = 128;                  // bytes of a K block: one swizzle row
+constexpr int kTileBytes = kRows * kKBytes;   // 16 KiB
+constexpr int kABytes = 2 * kTileBytes;       // a unit's weights
+constexpr int kRingBytes = 205 * 1024;
+constexpr int kMaxStages = 6;
+constexpr int kScaleBytes = 1024;             // room behind a stage's second operand for its scales
+constexpr int kClaims = 4;
+constexpr long long kWaitLimit = 1000000000LL;  // clock cycles before a wait gives up (~0.5 s)
+constexpr int kStatusRing = 301, kStatusPhase = 302;
+constexpr int kSplit = 8;                     // blocks of a route cluster: slices of H
+constexpr int kRouteThreads = 256;
+
+__host__ __device__ constexpr int token_rows(int T) { return T <= 8 ? 8 : T <= 16 ? 16 : 32; }
+// columns of the second operand: hi and lo (FP8; the intermediate also with bf16 weights), M = 128 wants a multiple of 16
+__host__ __device__ constexpr int fc1_cols(bool fp8, int tp) { return fp8 ? 2 * tp : (tp < 16 ? 16 : tp); }
+__host__ __device__ constexpr int fc2_cols(int tp) { return 2 * tp; }
+__host__ __device__ constexpr int stage_bytes(int tp) { return kABytes + 2 * fc2_cols(tp) * kKBytes + kScaleBytes; }
+__host__ __device__ constexpr int stages(int tp) { return kRingBytes / stage_bytes(tp) < kMaxStages ? kRingBytes / stage_bytes(tp) : kMaxStages; }
+
+struct Params {
+    const __nv_bfloat16* x;
+    const void* w_router;
+    const float* b_scale;
+    const float* b1_scale;
+    __nv_bfloat16* out;
+    int T, H, I, E, k, n_shared;
+    int scoring, mode;
+    int kb1, pairs2;          // K blocks of fc1; pairs of K blocks of fc2
+    int tiles1, tiles2;       // tiles of 128 rows of I and H
+    int shares;
+    int n_counters;
+    size_t rec1, rec2;        // bytes of a unit's second operand with its scales
+    int* counters;            // claims of fc1, of fc2, finished tiles of fc1, unused, then the parts seen of each tile
+    float* logits;            // [T, E]
+    uint8_t* xq;              // [kb1] records: [fc1_cols][128 B] swizzled, scales [token_rows]
+    uint8_t* aq;              // [experts hit][pairs2] records: two of [fc2_cols][128 B] swizzled, scales [2][token_rows]
+    float* part1;             // [shares][2][gate, value][token][128]
+    float* part2;             // [shares][2][token][128]
+    int* status;
+};
+
+// byte `byte` of row `row` of an operand tile with 128-byte rows, as the 128-byte swizzle places it
+__device__ __forceinline__ int swizzled(int row, int byte) { return row * kKBytes + (byte ^ ((row & 7) << 4)); }
+
+// 2^(exponent(amax) - 7) for the largest of a group's magnitudes, given as bits, so that amax / s lies in [128, 256); not below 2^-100, and
+// NaN where the group holds an infinity or a NaN (its token's results are NaN then)
+__device__ __forceinline__ float split_scale(uint32_t amax_bits, float* inv) {
+    if (amax_bits >= 0x7f800000u) {
+        *inv = 0.0f;
+        return __uint_as_float(0x7fffffffu);
+    }
+    const int e = max(int(amax_bits >> 23) - 127 - 7, -100);
+    *inv = __uint_as_float(uint32_t(127 - e) << 23);
+    return __uint_as_float(uint32_t(127 + e) << 23);
+}
+// two scaled values -> e4m3 pairs hi and lo with x = hi + lo / 16
+__device__ __forceinline__ void split_e4m3x2(float x0, float x1, uint32_t* hi, uint32_t* lo) {
+    *hi = f2e4m3x2(x0, x1);
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(*hi), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    *lo = f2e4m3x2((x0 - f.x) * 16.0f, (x1 - f.y) * 16.0f);
+}
+
+// ---------------------------------------------------------------- route
+
+template <bool kF32>
+__device__ __forceinline__ void load_router8(const void* w, size_t at, float (&f)[8]) {
+    if constexpr (kF32) {
+        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
+        const float4 a = p[0], b = p[1];
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at);
+        f[0] = bf16_lo(v.x), f[1] = bf16_hi(v.x), f[2] = bf16_lo(v.y), f[3] = bf16_hi(v.y);
+        f[4] = bf16_lo(v.z), f[5] = bf16_hi(v.z), f[6] = bf16_lo(v.w), f[7] = bf16_hi(v.w);
+    }
+}
+
+// One warp per expert and slice; the eight slices of a cluster are added in their order through distributed shared memory.
+template <bool kF32, int kTp>
+__device__ __forceinline__ void partial_logits(const Params& p, int e, int rank, float* part /*[T]*/, int lane) {
+    const int slice = (p.H + kSplit * 8 - 1) / (kSplit * 8) * 8;
+    const int k0 = rank * slice, k1 = min(p.H, k0 + slice);
+    float acc[kTp];
+#pragma unroll
+    for (int t = 0; t < kTp; ++t) acc[t] = 0.0f;
+    for (int k = k0 + lane * 8; k < k1; k += 256) {
+        float w[8];
+        load_router8<kF32>(p.w_router, size_t(e) * p.H + k, w);
+#pragma unroll
+        for (int t = 0; t < kTp; ++t)
+            if (t < p.T) {
+                const uint4 v = *reinterpret_cast<const uint4*>(p.x + size_t(t) * p.H + k);
+                float a = acc[t];
+                a = fmaf(bf16_lo(v.x), w[0], a), a = fmaf(bf16_hi(v.x), w[1], a);
+                a = fmaf(bf16_lo(v.y), w[2], a), a = fmaf(bf16_hi(v.y), w[3], a);
+                a = fmaf(bf16_lo(v.z), w[4], a), a = fmaf(bf16_hi(v.z), w[5], a);
+                a = fmaf(bf16_lo(v.w), w[6], a), a = fmaf(bf16_hi(v.w), w[7], a);
+                acc[t] = a;
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < kTp; ++t)
+        if (t < p.T) {
+            const float s = warp_sum(acc[t]);
+            if (lane == 0) part[t] = s;
+        }
+}
+
+// A K block of a token's x into its record.
+template <bool kFp8>
+__device__ __forceinline__ void lay_out_x(const Params& p, int kb, int t, int tp, int lane) {
+    uint8_t* rec = p.xq + size_t(kb) * p.rec1;
+    if constexpr (kFp8) {
+        const int k = kb * kKBytes + lane * 4;
+        uint2 v = make_uint2(0, 0);
+        if (k < p.H) v = *reinterpret_cast<const uint2*>(p.x + size_t(t) * p.H + k);
+        const uint32_t most = max(max((v.x & 0x7fffu) << 16, v.x & 0x7fff0000u), max((v.y & 0x7fffu) << 16, v.y & 0x7fff0000u));
+        float inv;
+        const float s = split_scale(__reduce_max_sync(0xffffffffu, most), &inv);
+        uint32_t h0, l0, h1, l1;
+        split_e4m3x2(bf16_lo(v.x) * inv, bf16_hi(v.x) * inv, &h0, &l0);
+        split_e4m3x2(bf16_lo(v.y) * inv, bf16_hi(v.y) * inv, &h1, &l1);
+        *reinterpret_cast<uint32_t*>(rec + swizzled(t, lane * 4)) = h0 | (h1 << 16);
+        *reinterpret_cast<uint32_t*>(rec + swizzled(tp + t, lane * 4)) = l0 | (l1 << 16);
+        if (lane == 0) reinterpret_cast<float*>(rec + fc1_cols(true, tp) * kKBytes)[t] = s;
+    } else {
+        const int k = kb * (kKBytes / 2) + lane * 2;
+        const uint32_t v = k < p.H ? *reinterpret_cast<const uint32_t*>(p.x + size_t(t) * p.H + k) : 0u;
+        *reinterpret_cast<uint32_t*>(rec + swizzled(t, lane * 4)) = v;
+    }
+}
+
+template <bool kF32, bool kFp8>
+__global__ void __launch_bounds__(kRouteThreads) moe_decode_route_kernel(const __grid_constant__ Params p) {
+    pdl_enter();
+    __shared__ float s_part[kRouteThreads / 32][kMaxTokens];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = int(ptx::cluster_ctarank());
+    const int chunk = blockIdx.x / kSplit, e = chunk * 8 + warp;
+    const int tp = token_rows(p.T);
+    const bool working = chunk * 8 < p.E;
+    if (e < p.E) {
+        if (tp == 8) partial_logits<kF32, 8>(p, e, rank, s_part[warp], lane);
+        else if (tp == 16) partial_logits<kF32, 16>(p, e, rank, s_part[warp], lane);
+        else partial_logits<kF32, 32>(p, e, rank, s_part[warp], lane);
+    }
+    for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kRouteThreads) p.counters[i] = 0;
+    const int warps = gridDim.x * (kRouteThreads / 32);
+    for (int u = blockIdx.x * (kRouteThreads / 32) + warp; u < p.kb1 * p.T; u += warps) lay_out_x<kFp8>(p, u / p.T, u % p.T, tp, lane);
+    if (!working) return;  // whole clusters
+    ptx::cluster_sync();
+    const int mine = chunk * 8 + rank;  // the expert whose slices this block adds
+    if (mine < p.E && threadIdx.x < p.T) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kSplit; ++r) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(&s_part[rank][threadIdx.x], r)) : "memory");
+            sum += v;
+        }
+        p.logits[size_t(threadIdx.x) * p.E + mine] = sum;
+    }
+    ptx::cluster_sync();  // the other blocks read this one's shared memory
+}
+
+// ---------------------------------------------------------------- experts
+
+struct alignas(16) Tail {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t tmem_full[4], tmem_empty[4];
+    uint64_t claim_full[kClaims], claim_empty[kClaims];
+    uint64_t meet;                             // the four epilogue warps
+    int claim[kClaims];
+    uint32_t tmem_base;
+    int abort_flag;
+    int n_hit;
+    uint32_t bad_tokens;                       // tokens without a number among their weights
+    int last_part;
+    uint32_t amax[4][kMaxTokens];
+    int topk_index[kMaxTokens][kMaxTopk];
+    float topk_weight[kMaxTokens][kMaxTopk];
+    uint32_t mask[kMaxExperts];                // tokens of an expert
+    uint32_t hit_mask[kMaxExperts];            // the same by place in the list of experts hit
+    uint16_t hit[kMaxExperts];
+};
+constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
+
+struct Share {
+    int phase, lo, hi, index;  // units [lo, hi) of phase 0 (fc1) or 1 (fc2); phase 2 = no more
+};
+__device__ __forceinline__ int phase_units(const Params& p, const Tail& st, int phase) {
+    return st.n_hit * (phase == 0 ? p.tiles1 * p.kb1 : p.tiles2 * p.pairs2);
+}
+// none of them empty: the parts of a tile are those of all shares between its first unit's and its last one's
+__device__ __forceinline__ int phase_shares(const Params& p, int units) { return min(p.shares, units); }
+__device__ __forceinline__ Share share_at(const Params& p, const Tail& st, int code) {
+    Share s;
+    s.phase = code >> 28;
+    s.index = code & 0xfffffff;
+    const int units = phase_units(p, st, s.phase & 1);
+    s.lo = streamk::first_unit(s.index, phase_shares(p, units), units);
+    s.hi = streamk::first_unit(s.index + 1, phase_shares(p, units), units);
+    return s;
+}
+constexpr int kEnd = 2 << 28;
+
+// The next share, as the producer announces it to the other roles.
+template <bool kWarp>
+__device__ __forceinline__ int next_claim(Tail& st, int it, int lane) {
+    const int slot = it % kClaims, parity = (it / kClaims) & 1;
+    const bool ok = kWarp ? ptx::mbar_wait_warp(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit)
+                          : ptx::mbar_wait(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit);
+    if (!ok) return kEnd;
+    const int code = *const_cast<volatile int*>(&st.claim[slot]);
+    if constexpr (kWarp) __syncwarp();
+    if (!kWarp || lane == 0) ptx::mbar_arrive(&st.claim_empty[slot]);
+    return code;
+}
+
+template <bool kFp8, int kTp>
+struct Shape {
+    static constexpr int kN1 = fc1_cols(kFp8, kTp), kN2 = fc2_cols(kTp);
+    static constexpr int kKElems = kFp8 ? kKBytes : kKBytes / 2;
+    static constexpr int kStages = stages(kTp);
+    static constexpr int kStage = stage_bytes(kTp);
+    // FP8: the accumulators of one unit per buffer, handed over unit by unit; bf16: those of one tile and expert
+    static constexpr int kBufCols = kFp8 ? 2 * kN1 : (2 * kN1 > kN2 ? 2 * kN1 : kN2);
+    static constexpr int kBufs = kFp8 ? 4 : 2;
+    static constexpr int kTmemCols = kBufs * kBufCols;  // 128 / 256 / 512 and 64 / 64 / 128
+    static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM allocation");
+};
+
+template <bool kFp8, int kTp>
+__device__ __forceinline__ void produce(const Params& p, const CUtensorMap& map_b, const CUtensorMap& map_b1, Tail& st, uint8_t* ring, int claim) {
+    using S = Shape<kFp8, kTp>;
+    int it = 0;        // units whose weights were asked for
+    int pushed = 0;
+    bool ready = false;
+    bool ok = true;
+    auto stage_at = [&](int i) { return ring + (i % S::kStages) * S::kStage; };
+    auto load_weights = [&](const Share& s, int u, int i) {
+        const int slot = i % S::kStages;
+        if (!ptx::mbar_wait(&st.empty[slot], ((i / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
+        uint8_t* a = stage_at(i);
+        if (s.phase == 0) {
+            const int tile = u / p.kb1, kb = u - tile * p.kb1;
+            const int j = tile / p.tiles1, row = st.hit[j] * 2 * p.I + (tile - j * p.tiles1) * kRows;
+            ptx::mbar_arrive_expect_tx(&st.full[slot], kABytes + uint32_t(p.rec1));
+            ptx::tma_load_2d(a, &map_b, kb * S::kKElems, row, &st.full[slot]);
+            ptx::tma_load_2d(a + kTileBytes, &map_b, kb * S::kKElems, row + p.I, &st.full[slot]);
+        } else {
+            const int per_tile = st.n_hit * p.pairs2;
+            const int tile = u / per_tile, rest = u - tile * per_tile, j = rest / p.pairs2, pair = rest - j * p.pairs2;
+            const int row = st.hit[j] * p.H + tile * kRows;
+            // a last pair's second block may lie past I, where the copy writes zeros
+            ptx::mbar_arrive_expect_tx(&st.full[slot], kABytes + uint32_t(p.rec2));
+            ptx::tma_load_2d(a, &map_b1, pair * 2 * S::kKElems, row, &st.full[slot]);
+            ptx::tma_load_2d(a + kTileBytes, &map_b1, (pair * 2 + 1) * S::kKElems, row, &st.full[slot]);
+        }
+        return true;
+    };
+    auto load_tokens = [&](const Share& s, int u, int i) {
+        const int slot = i % S::kStages;
+        if (s.phase == 0) {
+            ptx::bulk_load(stage_at(i) + kABytes, p.xq + size_t(u % p.kb1) * p.rec1, uint32_t(p.rec1), &st.full[slot]);
+        } else {
+            const int rest = u % (st.n_hit * p.pairs2);  // [expert][pair]
+            ptx::bulk_load(stage_at(i) + kABytes, p.aq + size_t(rest) * p.rec2, uint32_t(p.rec2), &st.full[slot]);
+        }
+    };
+    auto push = [&](int code) {
+        const int slot = pushed % kClaims;
+        if (!ptx::mbar_wait(&st.claim_empty[slot], ((pushed / kClaims) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
+        *const_cast<volatile int*>(&st.claim[slot]) = code;
+        ptx::mbar_arrive(&st.claim_full[slot]);
+        ++pushed;
+        return true;
+    };
+    for (int phase = 0; phase < 2 && ok; ++phase) {
+        if (phase == 1) claim = atomicAdd(&p.counters[1], 1);
+        const int shares = phase_shares(p, phase_units(p, st, phase));
+        for (; ok && claim < shares; claim = atomicAdd(&p.counters[phase], 1)) {
+            const int code = (phase << 28) | claim;
+            const Share s = share_at(p, st, code);
+            if (!push(code)) {
+                ok = false;
+                break;
+            }
+            int u = s.lo;
+            if (phase == 1 && !ready) {
+                // weights into every free stage first, then wait for fc1
+                const int first = it;
+                while (u < s.hi && it - first < S::kStages && (ok = load_weights(s, u, it))) ++u, ++it;
+                const int tiles = st.n_hit * p.tiles1;
+                const long long t0 = clock64();
+                while (ok && streamk::ld_acquire_gpu(&p.counters[2]) < tiles) {
+                    if (*const_cast<volatile int*>(&st.abort_flag) != 0) ok = false;
+                    else if (clock64() - t0 > kWaitLimit) {
+                        *const_cast<volatile int*>(&st.abort_flag) = 1;
+                        *p.status = kStatusPhase;
+                        ok = false;
+                    }
+                }
+                // also where the wait gave up: the copies complete the stages that were announced, so that the block can be left
+                asm volatile("fence.proxy.async;" ::: "memory");
+                for (int i = first; i < it; ++i) load_tokens(s, s.lo + i - first, i);
+                ready = true;
+            }
+            for (; ok && u < s.hi; ++u, ++it) {
+                if (!(ok = load_weights(s, u, it))) break;
+                load_tokens(s, u, it);
+            }
+        }
+    }
+    if (ok) push(kEnd);
+    // Nobody may leave with copies in flight. Where all went well the other roles have waited for each of them.
+    if (*const_cast<volatile int*>(&st.abort_flag) != 0) {
+        const long long t0 = clock64();
+        for (int i = max(0, it - S::kStages); i < it; ++i)
+            while (!ptx::mbar_try_wait(&st.full[i % S::kStages], (i / S::kStages) & 1) && clock64() - t0 < kWaitLimit) {}
+    }
+}
+
+template <bool kFp8, int kTp>
+__device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* ring, uint32_t tmem) {
+    using S = Shape<kFp8, kTp>;
+    constexpr int kKind = kFp8 ? 0 : 1;
+    constexpr uint32_t kFormat = kFp8 ? 0 : 1;
+    constexpr uint32_t kId1 = ptx::make_idesc(kFormat, kRows, S::kN1), kId2 = ptx::make_idesc(kFormat, kRows, S::kN2);
+    int it = 0, buf_it = 0;
+    for (int n = 0;; ++n) {
+        const int code = next_claim<false>(st, n, 0);
+        if (code == kEnd) return;
+        const Share s = share_at(p, st, code);
+        const int group = s.phase == 0 ? p.kb1 : p.pairs2;  // units of a tile and expert
+        bool fresh = true;                                  // the next unit begins an accumulator buffer
+        for (int u = s.lo; u < s.hi; ++u, ++it) {
+            const int slot = it % S::kStages, buf = buf_it % S::kBufs;
+            if (fresh && !ptx::mbar_wait(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
+            if (!ptx::mbar_wait(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit)) return;
+            ptx::tc_fence_after();
+            const uint32_t a = ptx::smem_u32(ring + slot * S::kStage);
+            const uint64_t da = ptx::smem_desc_sw128(a), db = ptx::smem_desc_sw128(a + kABytes);
+            const uint32_t d = tmem + buf * S::kBufCols;
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t ak = ptx::smem_desc_advance(da, half * kTileBytes + k * 32);
+                    if (s.phase == 0)  // gate rows, value rows
+                        ptx::umma<kKind>(d + half * S::kN1, ak, ptx::smem_desc_advance(db, k * 32), kId1, (!kFp8 && !fresh) || k > 0);
+                    else               // two K blocks: with their own scales in FP8, one sum in bf16
+                        ptx::umma<kKind>(d + (kFp8 ? half * S::kN2 : 0), ak, ptx::smem_desc_advance(db, half * S::kN2 * kKBytes + k * 32), kId2,
+                                         (!kFp8 && (!fresh || half > 0)) || k > 0);
+                }
+            ptx::umma_commit(&st.empty[slot]);
+            const bool done = kFp8 || u + 1 == s.hi || (u + 1) % group == 0;
+            if (done) {
+                ptx::umma_commit(&st.tmem_full[buf]);
+                ++buf_it;
+            }
+            fresh = done;
+        }
+    }
+}
+
+// columns [c, c + kCount) of this warp's lanes
+template <int kCount>
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
+    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    if constexpr (kCount == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(taddr) : "memory");
+    } else if constexpr (kCount == 16) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+                       "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]) : "r"(taddr) : "memory");
+    } else {
+        ptx::tmem_ld32(taddr, *reinterpret_cast<uint32_t (*)[32]>(&r));
+    }
+}
+// Wait for the loads; the registers pass through statements behind the wait.
+template <int kCount>
+__device__ __forceinline__ void tmem_landed(float (&a)[kCount], float (&b)[kCount]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i])::"memory");
+}
+
+// Scale of a weight row in a unit: constant over the weights (bf16: 1), an expert, a row, or a 128x128 block.
+__device__ __forceinline__ float weight_scale(const float* scale, int mode, int e, int rows, int row, int blocks_k, int kb) {
+    if (mode == DQMOE_QUANT_FP8_BLOCK) return scale[(size_t(e) * ((rows + 127) / 128) + row / 128) * blocks_k + kb];
+    if (mode == DQMOE_QUANT_FP8_CHANNEL) return scale[size_t(e) * rows + row];
+    return mode == DQMOE_QUANT_FP8_TENSOR ? scale[e] : 1.0f;
+}
+
+template <bool kFp8, int kTp>
+struct Epilogue {
+    using S = Shape<kFp8, kTp>;
+    const Params& p;
+    Tail& st;
+    uint8_t* ring;
+    uint32_t tmem;
+    int warp, lane, row;  // warp 0..3 of the epilogue, row = TMEM lane = weight row of the tile
+    int it = 0, buf_it = 0;
+    uint32_t meetings = 0;
+
+    // The epilogue warps wait for one another at an mbarrier, whose wait ends also where one of them has given up.
+    __device__ __forceinline__ bool meet() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&st.meet);
+        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
+    }
+    __device__ __forceinline__ bool acquire() {
+        const int buf = buf_it % S::kBufs;
+        if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (buf_it / S::kBufs) & 1, &st.abort_flag, kWaitLimit)) return false;
+        ptx::tc_fence_after();
+        return true;
+    }
+    // scales of a unit's tokens: they came with the stage, whose barrier this warp has to see for itself
+    __device__ __forceinline__ bool stage_full() {
+        return ptx::mbar_wait_warp(&st.full[it % S::kStages], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit);
+    }
+    __device__ __forceinline__ void release_stage() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&st.empty[it % S::kStages]);
+    }
+    __device__ __forceinline__ void release_buffer() {
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
+        ++buf_it;
+    }
+    __device__ __forceinline__ uint32_t buffer() const { return tmem + (uint32_t(warp * 32) << 16) + (buf_it % S::kBufs) * S::kBufCols; }
+
+    // sum += (hi + lo / 16) * scale of every token of `mask`
+    __device__ __forceinline__ void add_scaled(uint32_t taddr, const float* token_scale, float row_scale, uint32_t mask, float (&sum)[kTp]) {
+        float hi[kTp], lo[kTp];
+        tmem_read<kTp>(taddr, hi);
+        tmem_read<kTp>(taddr + kTp, lo);
+        tmem_landed<kTp>(hi, lo);
+#pragma unroll
+        for (int t = 0; t < kTp; t += 4) {
+            const float4 sc = *reinterpret_cast<const float4*>(token_scale + t);
+            const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if ((mask >> (t + i)) & 1u) sum[t + i] = fmaf(fmaf(lo[t + i], 0.0625f, hi[t + i]), s4[i] * row_scale, sum[t + i]);
+        }
+    }
+
+    // Counts this block's part of a tile in: 1 for the block whose part is the last, 0 for another, -1 where a warp has given up.
+    __device__ __forceinline__ int last_part(int* counter, int parts) {
+        __threadfence();
+        if (!meet()) return -1;
+        if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(counter, 1) == parts - 1;
+        if (!meet()) return -1;
+        const int last = *const_cast<volatile int*>(&st.last_part);
+        __threadfence();
+        return last;
+    }
+
+    // Weight of token t for the expert e (routed ids only), by all lanes together.
+    __device__ __forceinline__ float weight_of(int t, int e) const {
+        const bool mine = lane < p.k && st.topk_index[t][lane] == e;
+        const uint32_t who = __ballot_sync(0xffffffffu, mine);
+        return who == 0 ? 1.0f : st.topk_weight[t][__ffs(who) - 1];  // shared experts are not in the list
+    }
+
+    __device__ __forceinline__ bool finish_fc1(int tile, float (&g)[kTp], float (&v)[kTp]) {
+        const int j = tile / p.tiles1, it_tile = tile - j * p.tiles1, e = st.hit[j];
+        const uint32_t mask = st.hit_mask[j];
+        const bool inside = it_tile * kRows + row < p.I;
+        uint8_t* rec = p.aq + (size_t(j) * p.pairs2 + (kFp8 ? it_tile >> 1 : it_tile)) * p.rec2;
+        if constexpr (kFp8) {
+            const int half = it_tile & 1;
+#pragma unroll
+            for (int t = 0; t < kTp; ++t)
+                if ((mask >> t) & 1u) {  // the same for all threads
+                    const float w = weight_of(t, e);  // all lanes, also those of rows past I
+                    g[t] = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
+                    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(g[t]) & 0x7fffffffu);
+                    if (lane == 0) st.amax[warp][t] = most;
+                }
+            if (!meet()) return false;
+            uint8_t* data = rec + half * S::kN2 * kKBytes;
+            float* scales = reinterpret_cast<float*>(rec + 2 * S::kN2 * kKBytes) + half * kTp;
+#pragma unroll
+            for (int t = 0; t < kTp; ++t)
+                if ((mask >> t) & 1u) {
+                    float inv;
+                    const float s = split_scale(max(max(st.amax[0][t], st.amax[1][t]), max(st.amax[2][t], st.amax[3][t])), &inv);
+                    uint32_t hi, lo;
+                    split_e4m3x2(g[t] * inv, 0.0f, &hi, &lo);
+                    data[swizzled(t, row)] = uint8_t(hi);
+                    data[swizzled(kTp + t, row)] = uint8_t(lo);
+                    if (row == 0) scales[t] = s;
+                }
+        } else {
+            uint8_t* data = rec + (row >> 6) * S::kN2 * kKBytes;
+            const int byte = (row & 63) * 2;
+#pragma unroll
+            for (int t = 0; t < kTp; ++t)
+                if ((mask >> t) & 1u) {
+                    const float w = weight_of(t, e);  // all lanes, also those of rows past I
+                    const float a = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
+                    const uint32_t hi = f2bf_bits(a);
+                    const float rest = a - __uint_as_float(hi << 16);
+                    // an infinite value has no rest
+                    const uint32_t lo = (hi & 0x7fffu) < 0x7f80u ? f2bf_bits(rest) : 0u;
+                    *reinterpret_cast<uint16_t*>(data + swizzled(t, byte)) = uint16_t(hi);
+                    *reinterpret_cast<uint16_t*>(data + swizzled(kTp + t, byte)) = uint16_t(lo);
+                }
+        }
+        // to the bulk copies of other blocks
+        asm volatile("fence.proxy.async;" ::: "memory");
+        __threadfence();
+        if (!meet()) return false;
+        if (warp == 0 && lane == 0) streamk::atomic_add_acq_rel_gpu(&p.counters[2], 1);
+        return true;
+    }
+
+    __device__ __forceinline__ bool fc1(const Share& s, int units) {
+        const int shares = phase_shares(p, units);
+        for (int u = s.lo; u < s.hi;) {
+            const int tile = u / p.kb1, end = min(s.hi, (tile + 1) * p.kb1);
+            const int j = tile / p.tiles1, e = st.hit[j], i = min((tile - j * p.tiles1) * kRows + row, p.I - 1);
+            float g[kTp], v[kTp];
+            if constexpr (kFp8) {
+#pragma unroll
+                for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
+                const uint32_t mask = st.hit_mask[j];
+                const int kb0 = u - tile * p.kb1;
+                float sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb0);
+                float sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb0);
+                for (; u < end; ++u, ++it) {
+                    const int kb = u - tile * p.kb1;
+                    const float gs = sg, vs = sv;
+                    if (kb + 1 < p.kb1) {  // the next unit's, while this one's MMAs are on their way
+                        sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb + 1);
+                        sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb + 1);
+                    }
+                    if (!stage_full() || !acquire()) return false;
+                    const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + S::kN1 * kKBytes);
+                    add_scaled(buffer(), token_scale, gs, mask, g);
+                    add_scaled(buffer() + S::kN1, token_scale, vs, mask, v);
+                    release_buffer();
+                    release_stage();
+                }
+            } else {
+                it += end - u;
+                u = end;
+                if (!acquire()) return false;
+                tmem_read<kTp>(buffer(), g);
+                tmem_read<kTp>(buffer() + S::kN1, v);
+                tmem_landed<kTp>(g, v);
+                release_buffer();
+            }
+            const int first = streamk::share_of(tile * p.kb1, shares, units), last = streamk::share_of((tile + 1) * p.kb1 - 1, shares, units);
+            if (first < last) {
+                // a share's first tile has slot 0, a later one slot 1: only the first and the last can be shared with others
+                const size_t block = size_t(2) * kTp * kRows;
+                float* mine = p.part1 + (size_t(s.index) * 2 + (tile == s.lo / p.kb1 ? 0 : 1)) * block + row;
+#pragma unroll
+                for (int t = 0; t < kTp; ++t)
+                    if (t < p.T) {
+                        mine[t * kRows] = g[t];
+                        mine[(kTp + t) * kRows] = v[t];
+                    }
+                const int now = last_part(&p.counters[4 + tile], last - first + 1);
+                if (now < 0) return false;
+                if (now == 0) continue;
+#pragma unroll
+                for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
+                for (int o = first; o <= last; ++o) {
+                    const int o_lo = streamk::first_unit(o, shares, units);
+                    const float* part = p.part1 + (size_t(o) * 2 + (tile == o_lo / p.kb1 ? 0 : 1)) * block + row;
+#pragma unroll
+                    for (int t = 0; t < kTp; ++t)
+                        if (t < p.T) {
+                            g[t] += streamk::ld_partial(part + t * kRows);
+                            v[t] += streamk::ld_partial(part + (kTp + t) * kRows);
+                        }
+                }
+            }
+            if (!finish_fc1(tile, g, v)) return false;
+        }
+        return true;
+    }
+
+    __device__ __forceinline__ bool fc2(const Share& s, int units) {
+        const int shares = phase_shares(p, units);
+        const int per_tile = st.n_hit * p.pairs2;
+        const int kb2 = (p.I + S::kKElems - 1) / S::kKElems;
+        for (int u = s.lo; u < s.hi;) {
+            const int tile = u / per_tile, end = min(s.hi, (tile + 1) * per_tile);
+            const int h = min(tile * kRows + row, p.H - 1);
+            float sum[kTp];
+#pragma unroll
+            for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
+            if constexpr (kFp8) {
+                float scale[2];
+                auto scales_of = [&](int unit) {
+                    const int rest = unit - tile * per_tile, j = rest / p.pairs2, kb = (rest - j * p.pairs2) * 2;
+                    scale[0] = weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb);
+                    scale[1] = kb + 1 < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb + 1) : 0.0f;
+                };
+                scales_of(u);
+                for (; u < end; ++u, ++it) {
+                    const int rest = u - tile * per_tile, j = rest / p.pairs2, kb = (rest - j * p.pairs2) * 2;
+                    const float s0 = scale[0], s1 = scale[1];
+                    if (u + 1 < end) scales_of(u + 1);
+                    const uint32_t mask = st.hit_mask[j];
+                    if (!stage_full() || !acquire()) return false;
+                    const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + 2 * S::kN2 * kKBytes);
+                    add_scaled(buffer(), token_scale, s0, mask, sum);
+                    if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale + kTp, s1, mask, sum);  // nothing was laid out for a block past I
+                    release_buffer();
+                    release_stage();
+                }
+            } else {
+                while (u < end) {  // expert by expert: only the tokens that chose it take part
+                    const int j = (u - tile * per_tile) / p.pairs2, stop = min(end, tile * per_tile + (j + 1) * p.pairs2);
+                    it += stop - u;
+                    u = stop;
+                    if (!acquire()) return false;
+                    float hi[kTp], lo[kTp];
+                    tmem_read<kTp>(buffer(), hi);
+                    tmem_read<kTp>(buffer() + kTp, lo);
+                    tmem_landed<kTp>(hi, lo);
+                    release_buffer();
+                    const uint32_t mask = st.hit_mask[j];
+#pragma unroll
+                    for (int t = 0; t < kTp; ++t)
+                        if ((mask >> t) & 1u) sum[t] += hi[t] + lo[t];
+                }
+            }
+            const int first = streamk::share_of(tile * per_tile, shares, units), last = streamk::share_of((tile + 1) * per_tile - 1, shares, units);
+            if (first < last) {
+                const size_t block = size_t(kTp) * kRows;
+                float* mine = p.part2 + (size_t(s.index) * 2 + (tile == s.lo / per_tile ? 0 : 1)) * block + row;
+#pragma unroll
+                for (int t = 0; t < kTp; ++t)
+                    if (t < p.T) mine[t * kRows] = sum[t];
+                const int now = last_part(&p.counters[4 + st.n_hit * p.tiles1 + tile], last - first + 1);
+                if (now < 0) return false;
+                if (now == 0) continue;
+#pragma unroll
+                for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
+                for (int o = first; o <= last; ++o) {
+                    const int o_lo = streamk::first_unit(o, shares, units);
+                    const float* part = p.part2 + (size_t(o) * 2 + (tile == o_lo / per_tile ? 0 : 1)) * block + row;
+#pragma unroll
+                    for (int t = 0; t < kTp; ++t)
+                        if (t < p.T) sum[t] += streamk::ld_partial(part + t * kRows);
+                }
+            }
+            if (tile * kRows + row < p.H) {
+                const uint32_t bad = st.bad_tokens;
+#pragma unroll
+                for (int t = 0; t < kTp; ++t)
+                    if (t < p.T) p.out[size_t(t) * p.H + h] = __float2bfloat16_rn((bad >> t) & 1u ? __uint_as_float(0x7fffffffu) : sum[t]);
+            }
+        }
+        return true;
+    }
+
+    __device__ __forceinline__ void run() {
+        for (int n = 0;; ++n) {
+            const int code = next_claim<true>(st, n, lane);
+            if (code == kEnd) return;
+            const Share s = share_at(p, st, code);
+            const int units = phase_units(p, st, s.phase);
+            if (!(s.phase == 0 ? fc1(s, units) : fc2(s, units))) return;
+        }
+    }
+};
+
+// Chosen experts of every token into shared memory, and the list of experts that any token chose, shared ones at its end.
+__device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int lane) {
+    for (int i = threadIdx.x; i < p.E; i += kThreads) st.mask[i] = 0;
+    if (threadIdx.x == 0) st.bad_tokens = 0;
+    __syncthreads();
+    for (int t = warp; t < p.T; t += kThreads / 32) {
+        const float* row = p.logits + size_t(t) * p.E;
+        int* index = st.topk_index[t];
+        float* weight = st.topk_weight[t];
+        if (p.E <= 32) route::topk_of_token<1>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
+        else if (p.E <= 128) route::topk_of_token<4>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
+        else if (p.E <= 256) route::topk_of_token<8>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
+        else route::topk_of_token<32>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
+        __syncwarp();
+        if (lane < p.k) {
+            if (index[lane] < p.E) atomicOr(&st.mask[index[lane]], 1u << t);
+            if (isnan(weight[lane])) atomicOr(&st.bad_tokens, 1u << t);
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int count = 0;
+        for (int e0 = 0; e0 < p.E; e0 += 32) {
+            const uint32_t m = e0 + lane < p.E ? st.mask[e0 + lane] : 0u;
+            const uint32_t hits = __ballot_sync(0xffffffffu, m != 0);
+            const int at = count + __popc(hits & ((1u << lane) - 1u));
+            if (m != 0) {
+                st.hit[at] = uint16_t(e0 + lane);
+                st.hit_mask[at] = m;
+            }
+            count += __popc(hits);
+        }
+        for (int i = lane; i < p.n_shared; i += 32) {
+            st.hit[count + i] = uint16_t(p.E + i);
+            st.hit_mask[count + i] = p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u;
+        }
+        if (lane == 0) st.n_hit = count + p.n_shared;
+    }
+}
+
+template <bool kFp8, int kTp>
+__global__ void __launch_bounds__(kThreads, 1)
+moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ Params p) {
+    using S = Shape<kFp8, kTp>;
+    pdl_launch();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Tail& st = *reinterpret_cast<Tail*>(ring + kRingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            ptx::mbar_init(&st.full[i], 1);
+            ptx::mbar_init(&st.empty[i], kFp8 ? 5 : 1);  // the tensor core's reads, and the epilogue warps' of the scales
+        }
+        for (int i = 0; i < 4; ++i) {
+            ptx::mbar_init(&st.tmem_full[i], 1);
+            ptx::mbar_init(&st.tmem_empty[i], 4);
+        }
+        for (int i = 0; i < kClaims; ++i) {
+            ptx::mbar_init(&st.claim_full[i], 1);
+            ptx::mbar_init(&st.claim_empty[i], 5);
+        }
+        ptx::mbar_init(&st.meet, 4);
+        st.abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&st.tmem_base, S::kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    if (threadIdx.x == 32 * 2) ptx::prefetch_tensormap(&map_b);
+    if (threadIdx.x == 32 * 3) ptx::prefetch_tensormap(&map_b1);
+    pdl_wait();
+    int claim = 0;
+    if (threadIdx.x == 0) claim = atomicAdd(&p.counters[0], 1);
+    claim = __shfl_sync(0xffffffffu, claim, 0);
+    choose(p, st, warp, lane);
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
+
+    if (st.n_hit == 0) {  // no token has an expert
+        for (int i = blockIdx.x * kThreads + threadIdx.x; i < p.T * p.H; i += gridDim.x * kThreads)
+            p.out[i] = __float2bfloat16_rn((st.bad_tokens >> (i / p.H)) & 1u ? __uint_as_float(0x7fffffffu) : 0.0f);
+    } else if (warp == 0) {
+        if (ptx::elect_one()) produce<kFp8, kTp>(p, map_b, map_b1, st, ring, claim);
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ptx::elect_one()) multiply<kFp8, kTp>(p, st, ring, tmem);
+        __syncwarp();
+    } else if (warp >= 4) {
+        Epilogue<kFp8, kTp> ep{p, st, ring, tmem, warp - 4, lane, (warp - 4) * 32 + lane};
+        ep.run();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && st.abort_flag != 0 && *const_cast<volatile int*>(p.status) == 0) *p.status = kStatusRing;
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, S::kTmemCols);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+struct Layout {
+    size_t counters, logits, xq, aq, part1, part2, total;
+};
+static Layout plan(Params* p, bool fp8) {
+    const int tp = token_rows(p->T);
+    const int ke = fp8 ? 128 : 64;
+    const int hit = (p->T * p->k < p->E ? p->T * p->k : p->E) + p->n_shared;
+    p->kb1 = ceil_div(p->H, ke);
+    p->pairs2 = ceil_div(ceil_div(p->I, ke), 2);
+    p->tiles1 = ceil_div(p->I, kRows);
+    p->tiles2 = ceil_div(p->H, kRows);
+    p->rec1 = size_t(fc1_cols(fp8, tp)) * kKBytes + (fp8 ? size_t(tp) * sizeof(float) : 0);
+    p->rec2 = size_t(2) * fc2_cols(tp) * kKBytes + (fp8 ? size_t(2) * tp * sizeof(float) : 0);
+    p->shares = sm_count();
+    p->n_counters = 4 + hit * p->tiles1 + p->tiles2;
+    Layout L{};
+    size_t off = 0;
+    auto add = [&](size_t bytes) {
+        const size_t at = off;
+        off += align_up(bytes, 256);
+        return at;
+    };
+    L.counters = add(size_t(p->n_counters) * sizeof(int));
+    L.logits = add(size_t(p->T) * p->E * sizeof(float));
+    L.xq = add(size_t(p->kb1) * p->rec1);
+    L.aq = add(size_t(hit) * p->pairs2 * p->rec2);
+    L.part1 = add(size_t(p->shares) * 4 * tp * kRows * sizeof(float));
+    L.part2 = add(size_t(p->shares) * 2 * tp * kRows * sizeof(float));
+    L.total = off;
+    return L;
+}
+
+static int check_sizes(int T, int H, int I, int E, int k, int n_shared, int quant_mode) {
+    DQ_CHECK_FMT(quant_mode == DQMOE_QUANT_NONE || quant_mode == DQMOE_QUANT_FP8_TENSOR || quant_mode == DQMOE_QUANT_FP8_CHANNEL ||
+                     quant_mode == DQMOE_QUANT_FP8_BLOCK,
+                 "quant_mode=%d: bf16 weights, or FP8 with scales per tensor, channel or block", quant_mode);
+    DQ_CHECK_FMT(T >= 0 && T <= kMaxTokens, "T=%d: at most %d tokens (dqmoe_moe_block takes any number)", T, kMaxTokens);
+    DQ_CHECK(H > 0 && I > 0 && E > 0 && k > 0 && k <= E && k <= kMaxTopk && n_shared >= 0);
+    DQ_CHECK_FMT(int64_t(E) + n_shared <= kMaxExperts, "E=%d and n_shared=%d: at most %d experts", E, n_shared, kMaxExperts);
+    DQ_CHECK_FMT(H % 16 == 0 && I % 16 == 0, "hidden_size=%d and inter_size=%d must be multiples of 16", H, I);
+    // row numbers of the tensor maps, unit numbers and offsets in a tile are 32-bit
+    DQ_CHECK_FMT(H <= (1 << 17) && I <= (1 << 17) && int64_t(E + n_shared) * (int64_t(2) * I + H) < (int64_t(1) << 31) &&
+                     int64_t(E + n_shared) * ceil_div(I, 64) * ceil_div(H, 64) < (int64_t(1) << 30),
+                 "H=%d I=%d E=%d: too large", H, I, E);
+    return DQMOE_OK;
+}
+
+template <class K>
+static int opt_in(K kern, int which) {
+    static std::mutex mu;
+    static bool configured[6][64] = {};
+    int dev = 0;
+    DQ_CUDA(cudaGetDevice(&dev));
+    DQ_CHECK(dev >= 0 && dev < 64);
+    std::lock_guard<std::mutex> lk(mu);
+    if (!configured[which][dev]) {
+        DQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes)));
+        configured[which][dev] = true;
+    }
+    return DQMOE_OK;
+}
+
+template <bool kFp8, int kTp>
+static int launch_experts(const CUtensorMap& b, const CUtensorMap& b1, const Params& p, cudaStream_t stream) {
+    DQ_RC(opt_in(moe_decode_experts_kernel<kFp8, kTp>, (kFp8 ? 3 : 0) + (kTp == 8 ? 0 : kTp == 16 ? 1 : 2)));
+    return launch_pdl(moe_decode_experts_kernel<kFp8, kTp>, dim3(p.shares), kThreads, kSmemBytes, stream, b, b1, p);
+}
+
+template <bool kF32, bool kFp8>
+static int launch_route(const Params& p, cudaStream_t stream) {
+    // a cluster for eight experts; more of them only lay x out, a K block of a token per warp and turn
+    const int clusters = ceil_div(p.E, 8), wanted = ceil_div(p.kb1 * p.T, kSplit * 2 * (kRouteThreads / 32));
+    const int most = sm_count() / kSplit;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(kSplit * (clusters > wanted ? clusters : wanted < most ? wanted : (clusters > most ? clusters : most))), 1, 1);
+    cfg.blockDim = dim3(kRouteThreads, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kSplit;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    DQ_CUDA(cudaLaunchKernelEx(&cfg, moe_decode_route_kernel<kF32, kFp8>, p));
+    return DQMOE_OK;
+}
+
+}  // namespace moe_decode
+}  // namespace dq
+
+using namespace dq;
+
+extern "C" {
+
+size_t dqmoe_moe_decode_workspace_bytes(int T, int H, int I, int E, int k, int n_shared, int quant_mode) {
+    if (moe_decode::check_sizes(T, H, I, E, k, n_shared, quant_mode) != DQMOE_OK) return 0;
+    moe_decode::Params p{};
+    p.T = T, p.H = H, p.I = I, p.E = E, p.k = k, p.n_shared = n_shared;
+    return moe_decode::plan(&p, quant_mode != DQMOE_QUANT_NONE).total;
+}
+
+int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, const void* b, const float* b_scale, const void* b1,
+                     const float* b1_scale, void* out_bf16, void* workspace, size_t workspace_bytes, int T, int H, int I, int E, int k,
+                     int n_shared, int scoring, int quant_mode, dqmoe_stream_t stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    DQ_RC(moe_decode::check_sizes(T, H, I, E, k, n_shared, quant_mode));
+    DQ_CHECK(scoring == DQMOE_SCORE_SOFTMAX || scoring == DQMOE_SCORE_SIGMOID);
+    DQ_CHECK_FMT(router_type == DQMOE_DT_BF16 || router_type == DQMOE_DT_FLOAT, "router_type=%d: BF16 or FLOAT", router_type);
+    if (T == 0) return DQMOE_OK;
+    const bool fp8 = quant_mode != DQMOE_QUANT_NONE;
+    DQ_CHECK(x_bf16 != nullptr && w_router != nullptr && b != nullptr && b1 != nullptr && out_bf16 != nullptr);
+    if (fp8) DQ_CHECK(b_scale != nullptr && b1_scale != nullptr);
+    DQ_CHECK(is_aligned(x_bf16, 16) && is_aligned(w_router, 16) && is_aligned(b, 16) && is_aligned(b1, 16) && is_aligned(out_bf16, 2));
+    if (fp8) DQ_CHECK(is_aligned(b_scale, 4) && is_aligned(b1_scale, 4));
+    DQ_CHECK_FMT(workspace != nullptr && is_aligned(workspace, 256), "workspace pointer %p is not aligned!", workspace);
+    moe_decode::Params p{};
+    p.T = T, p.H = H, p.I = I, p.E = E, p.k = k, p.n_shared = n_shared;
+    const moe_decode::Layout L = moe_decode::plan(&p, fp8);
+    if (workspace_bytes != 0 && workspace_bytes < L.total)
+        return fail(DQMOE_ERR_WORKSPACE, __FILE__, __LINE__, "workspace_bytes >= dqmoe_moe_decode_workspace_bytes(...)",
+                    "workspace has %zu bytes, the layer needs %zu", workspace_bytes, L.total);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.x = static_cast<const __nv_bfloat16*>(x_bf16);
+    p.w_router = w_router;
+    p.b_scale = b_scale;
+    p.b1_scale = b1_scale;
+    p.out = static_cast<__nv_bfloat16*>(out_bf16);
+    p.scoring = scoring;
+    p.mode = quant_mode;
+    p.counters = reinterpret_cast<int*>(ws + L.counters);
+    p.logits = reinterpret_cast<float*>(ws + L.logits);
+    p.xq = ws + L.xq;
+    p.aq = ws + L.aq;
+    p.part1 = reinterpret_cast<float*>(ws + L.part1);
+    p.part2 = reinterpret_cast<float*>(ws + L.part2);
+    p.status = device_status_word();
+    if (p.status == nullptr) return DQMOE_ERR_CUDA;
+    const int esz = fp8 ? 1 : 2;
+    CUtensorMap map_b, map_b1;
+    DQ_RC(gemm::make_map(&map_b, b, esz, uint64_t(E + n_shared) * 2 * I, uint64_t(H), moe_decode::kRows));
+    DQ_RC(gemm::make_map(&map_b1, b1, esz, uint64_t(E + n_shared) * H, uint64_t(I), moe_decode::kRows));
+    const bool f32 = router_type == DQMOE_DT_FLOAT;
+    DQ_RC(f32 ? (fp8 ? moe_decode::launch_route<true, true>(p, stream) : moe_decode::launch_route<true, false>(p, stream))
+              : (fp8 ? moe_decode::launch_route<false, true>(p, stream) : moe_decode::launch_route<false, false>(p, stream)));
+    switch (moe_decode::token_rows(T)) {
+        case 8: return fp8 ? moe_decode::launch_experts<true, 8>(map_b, map_b1, p, stream) : moe_decode::launch_experts<false, 8>(map_b, map_b1, p, stream);
+        case 16: return fp8 ? moe_decode::launch_experts<true, 16>(map_b, map_b1, p, stream) : moe_decode::launch_experts<false, 16>(map_b, map_b1, p, stream);
+        default: return fp8 ? moe_decode::launch_experts<true, 32>(map_b, map_b1, p, stream) : moe_decode::launch_experts<false, 32>(map_b, map_b1, p, stream);
+    }
+}
+
+}  // extern "C"

@@ -22,6 +22,9 @@ QUANT_FP8_BLOCK = 1024
 QUANT_FP8_MX = 2048
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
+DT_FLOAT = 0
+DT_HALF = 1
+DT_BF16 = 7
 
 FP8 = torch.float8_e4m3fn
 
@@ -173,6 +176,66 @@ def moe_block(x: torch.Tensor, logits: torch.Tensor, b, b_scale, b1, b1_scale, k
         _lib.check(lib.dqmoe_moe_block_shared(_p(x), _p(logits), _p(b), _p(b_scale), _p(b1), _p(b1_scale), _p(out),
                                               _p(workspace), workspace.numel(), T, H, I, E, k, n_shared, mode,
                                               int(quant_mode), _stream(x.device)))
+    return out
+
+
+def moe_decode_workspace_bytes(T: int, H: int, I: int, E: int, k: int, n_shared: int = 0, quant_mode: int = QUANT_FP8_BLOCK) -> int:
+    """Bytes of workspace for moe_decode; 0 where the sizes are not ones it takes."""
+    return int(_lib.load().dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, int(quant_mode)))
+
+
+def moe_decode(x: torch.Tensor, w_router: torch.Tensor, b: torch.Tensor, b_scale, b1: torch.Tensor, b1_scale, k: int,
+               scoring: str = "softmax", quant_mode: int = QUANT_FP8_BLOCK, n_shared: int = 0,
+               workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The whole MoE layer for at most 32 tokens in two launches, router included; see dqmoe_moe_decode.
+
+    x [T, H] bf16, w_router [E, H] bf16 or fp32, experts' weights bf16 (quant_mode 0) or e4m3 with that mode's scales
+    (256 / 512 / 1024). The activations are not quantised. The last n_shared experts of b / b1 are shared ones that every token
+    passes through with weight 1. Returns out [T, H] bf16."""
+    for name, t in (("x", x), ("w_router", w_router), ("b", b), ("b1", b1)):
+        _cuda(t, name)
+        if t.device != x.device:
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
+    quant_mode = int(quant_mode)
+    weights = torch.bfloat16 if quant_mode == QUANT_NONE else FP8
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: x is bf16 [T, H]")
+    T, H = x.shape
+    if b.dim() != 3 or b1.dim() != 3 or b.dtype != weights or b1.dtype != weights:
+        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: b and b1 are {weights} [E, 2I, H] and [E, H, I]")
+    E_all, I = b.shape[0], b1.shape[2]
+    E = E_all - n_shared
+    if tuple(b.shape) != (E_all, 2 * I, H) or tuple(b1.shape) != (E_all, H, I):
+        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: b is [E, 2I, H] and b1 [E, H, I]  Info: got {tuple(b.shape)}, {tuple(b1.shape)}")
+    if n_shared < 0 or E <= 0 or tuple(w_router.shape) != (E, H) or w_router.dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: w_router is bf16 or fp32 [num_experts - n_shared, H]")
+    if quant_mode in (QUANT_FP8_TENSOR, QUANT_FP8_CHANNEL, QUANT_FP8_BLOCK):
+        g = lambda n: (n + 127) // 128
+        want = {QUANT_FP8_TENSOR: (E_all, E_all), QUANT_FP8_CHANNEL: (E_all * 2 * I, E_all * H),
+                QUANT_FP8_BLOCK: (E_all * g(2 * I) * g(H), E_all * g(H) * g(I))}[quant_mode]
+        for name, t, n in (("b_scale", b_scale, want[0]), ("b1_scale", b1_scale, want[1])):
+            if t is None or t.device != x.device or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
+                raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor of {n} elements on x's device "
+                                   f"for quant mode {quant_mode}")
+    lib = _lib.load()
+    if workspace is None:
+        need = int(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode))
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+    else:
+        _cuda(workspace, "workspace")
+        if workspace.device != x.device:
+            raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is on x's device")
+    if out is None:
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
+    else:
+        _cuda(out, "out")
+        if tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device:
+            raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is bf16 [T, H] on x's device")
+    mode = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}[scoring]
+    with torch.cuda.device(x.device):
+        _lib.check(lib.dqmoe_moe_decode(_p(x), _p(w_router), DT_FLOAT if w_router.dtype == torch.float32 else DT_BF16, _p(b), _p(b_scale),
+                                        _p(b1), _p(b1_scale), _p(out), _p(workspace), workspace.numel() * workspace.element_size(), T, H, I,
+                                        E, k, n_shared, mode, quant_mode, _stream(x.device)))
     return out
 
 

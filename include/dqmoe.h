@@ -206,6 +206,23 @@ int dqmoe_moe_block_shared(const void* x_bf16, const float* logits, const void* 
                            size_t workspace_bytes, int T, int H, int I, int E, int k, int n_shared,
                            int scoring, int quant_mode, dqmoe_stream_t stream);
 
+/*
+ * The whole MoE layer for a few tokens (T <= 32), from the activations and the router's weights to its output, in two launches:
+ *   logits = x Wr^T (fp32); the k experts of the largest logits with weights as dqmoe_route_topk gives them; out[t] = sum over them of
+ *   weight * W2 (silu(G x) * (V x)); then n_shared shared experts, which stand behind the E routed ones in b / b1, with weight 1.
+ * x [T, H] bf16, w_router [E, H] of router_type DQMOE_DT_BF16 or DQMOE_DT_FLOAT, b [E + n_shared, 2I, H], b1 [E + n_shared, H, I],
+ * out [T, H] bf16. quant_mode NONE (bf16 weights) or FP8_TENSOR / _CHANNEL / _BLOCK (e4m3 weights with scales as listed at the top of
+ * this file). The activations are not quantised in any mode, sums are fp32, and only the result is rounded to bf16: against
+ * dqmoe_moe_block, which quantises both operands, the results differ by that quantisation. T <= 32, E + n_shared <= 1024, k <= 32, H and I
+ * multiples of 16, operands aligned to 16 bytes. A token whose weights are not numbers (no logit above -inf) gets NaN, and so does
+ * one whose x holds an infinity or a NaN in the FP8 modes; it changes no other token's result. The status codes of
+ * dqmoe_device_status are 301 and 302. A call has its workspace for itself until it is over. No counterpart in the reference.
+ */
+size_t dqmoe_moe_decode_workspace_bytes(int T, int H, int I, int E, int k, int n_shared, int quant_mode);
+int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, const void* b, const float* b_scale,
+                     const void* b1, const float* b1_scale, void* out_bf16, void* workspace, size_t workspace_bytes, int T,
+                     int H, int I, int E, int k, int n_shared, int scoring, int quant_mode, dqmoe_stream_t stream);
+
 /* ------------------------------------------------------------------ plugin-shaped front end */
 
 /*
