@@ -61,6 +61,8 @@ SIGNATURES = {
     "dqmoe_moe_forward_nvfp4": (_c_int, [_ptr] * 15 + [_c_size] + [_c_int] * 5 + [_ptr]),
     "dqmoe_grouped_gemm": (_c_int, [_ptr] * 6 + [_c_int] * 6 + [_ptr] * 5),
     "dqmoe_grouped_gemm_rows": (_c_int, [_ptr] * 6 + [_c_int] * 5 + [_ptr, _ptr]),
+    "dqmoe_lora_linear_workspace_bytes": (_c_size, [_c_int] * 5),
+    "dqmoe_lora_linear": (_c_int, [_ptr, _c_i64] + [_ptr] * 7 + [_c_i64, _ptr, _c_size] + [_c_int] * 6 + [_ptr]),
     "dqmoe_ep_publish_counts": (_c_int, [_ptr, _c_int, _c_int, _c_int, _ptr, _ptr, _c_int, _ptr]),
     "dqmoe_ep_plan": (_c_int, [_ptr, _ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _ptr, _ptr, _ptr, _ptr]),
     "dqmoe_ep_set_wait_limit": (_c_int, [_c_i64]),

@@ -1,0 +1,737 @@
+// A projection that many requests share, each row with its request's low-rank adapter beside it, in two launches:
+//   y[t] = x[t] W^T + bias + scale_a (x[t] A_a^T) B_a^T,   a = ids[t]; rows whose id is outside [0, L) have no adapter.
+//
+//   shrink    z[t] = scale_a x[t] A_a^T, fp32 [T, R] and once more in the operands' type
+//   project   y = x W^T, with z B_a^T added to the same fp32 sums
+//
+// What bounds it: few rows the weights W and the adapters in use from HBM, many rows the tensor cores. project runs with W on the
+// tensor core's first operand (M = 128 rows of W) and up to 256 rows of x on the second, so that a decode batch computes few columns too
+// many. Tiles that do not fill the chip are cut along K into equal shares per SM (streamk.cuh).
+//
+// Where a row tile of project belongs to one adapter - prefill, where a request's rows stand together - z B_a^T is further K blocks of the
+// same product. Elsewhere (decode batches, the tiles where requests meet) it is added by the threads of the epilogue, row by row with
+// its own B: masks on a mixed product would let one adapter's infinities reach the rows of another, and z keeps its 32 bits.
+// shrink takes 64 rows of x at a time against all adapters among them, several adapters' A stacked on M = 128, and keeps from the product
+// what belongs together.
+//
+// project starts while shrink runs: it reads only x, W and ids until a tile is summed up. That is sound because shrink lets it start
+// behind its own wait for the kernels before, which wrote those. No counterpart in the reference.
+#include <mutex>
+
+#include "common.cuh"
+#include "gemm_tile.cuh"
+#include "ptx_sm100.cuh"
+#include "streamk.cuh"
+
+namespace dq {
+namespace lora {
+
+constexpr int kKBytes = 128;                    // bytes of a K block: one swizzle row, 64 values
+constexpr int kKElems = 64;
+constexpr int kRows = 128;                      // rows of W, or of stacked A, of an MMA
+constexpr int kABytes = kRows * kKBytes;        // 16 KiB
+constexpr int kMaxRank = 128;
+constexpr long long kWaitLimit = 1000000000LL;  // clock cycles before a wait gives up (~0.5 s)
+constexpr int kStatusShrink = 311, kStatusProject = 312;
+
+// ---------------------------------------------------------------- shrink
+
+constexpr int kShrinkTok = 64;                  // rows of x per tile
+constexpr int kShrinkThreads = 256;             // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
+constexpr int kShrinkStage = kABytes + kShrinkTok * kKBytes;
+constexpr int kShrinkStages = 4;
+constexpr int kMaxSplit = 8;                    // blocks of a cluster: slices of K
+constexpr int kNone = -1, kMixed = -2;          // a tile's adapter where it has not one
+
+struct ShrinkParams {
+    const int* ids;
+    const float* scale;     // [L] or null
+    float* z;               // [T, R]
+    uint16_t* z16;          // [T, R] in the operands' type
+    int* info;              // [ceil(T / 64)] adapter of a tile: id, kNone or kMixed
+    int* counters;          // project's, cleared here
+    int n_counters;
+    int T, K, L, R;
+    int half;               // operands fp16, else bf16
+    int slots;              // clusters that share a tile's groups of adapters
+    int* status;
+};
+struct alignas(16) ShrinkTail {
+    uint64_t full[kShrinkStages], empty[kShrinkStages], tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+    int distinct;                               // adapters of the tile
+    int overflow;                               // some z does not fit the operands' type
+    int id[kShrinkTok];                         // -1 where there is none
+    int place[kShrinkTok];                      // place of a row's adapter among the tile's
+    int adapter[kShrinkTok];                    // the tile's adapters in the order of their first rows
+    uint32_t firsts[2];
+};
+static size_t shrink_smem(int R) { return 1024 + size_t(kShrinkStages) * kShrinkStage + size_t(kShrinkTok) * R * sizeof(float) + sizeof(ShrinkTail); }
+
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t n;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+
+__device__ __forceinline__ uint16_t to_bits(float f, bool half) {
+    return half ? __half_as_ushort(__float2half_rn(f)) : uint16_t(f2bf_bits(f));
+}
+
+__global__ void __launch_bounds__(kShrinkThreads)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ShrinkParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* part = reinterpret_cast<float*>(ring + kShrinkStages * kShrinkStage);  // [64][R] of this block's slice of K
+    ShrinkTail& st = *reinterpret_cast<ShrinkTail*>(part + kShrinkTok * p.R);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kShrinkStages; ++i) {
+            ptx::mbar_init(&st.full[i], 1);
+            ptx::mbar_init(&st.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&st.tmem_full[i], 1);
+            ptx::mbar_init(&st.tmem_empty[i], 4);
+        }
+        st.abort_flag = 0;
+        st.overflow = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&st.tmem_base, 2 * kShrinkTok);
+        ptx::tmem_relinquish();
+    }
+    pdl_wait();    // x, ids and the workspace
+    pdl_launch();
+    const int rank = int(ptx::cluster_ctarank()), split = int(cluster_nctarank());
+    const int cluster = blockIdx.x / split, tile = cluster / p.slots, slot = cluster - tile * p.slots;
+    for (int i = blockIdx.x * kShrinkThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kShrinkThreads) p.counters[i] = 0;
+    if (threadIdx.x < kShrinkTok) {
+        const int t = tile * kShrinkTok + threadIdx.x;
+        const int id = t < p.T ? p.ids[t] : -1;
+        st.id[threadIdx.x] = id >= 0 && id < p.L ? id : -1;
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
+    // the distinct adapters, in the order of their first rows
+    int first = kShrinkTok;  // this row's adapter appears first in row `first`
+    if (threadIdx.x < kShrinkTok) {
+        const int mine = st.id[threadIdx.x];
+        for (int t = kShrinkTok - 1; t >= 0; --t)
+            if (st.id[t] == mine) first = t;
+        const uint32_t firsts = __ballot_sync(0xffffffffu, mine >= 0 && first == int(threadIdx.x));
+        if (lane == 0) st.firsts[warp] = firsts;
+    }
+    __syncthreads();
+    if (threadIdx.x < kShrinkTok) {
+        const uint32_t lo = st.firsts[0], hi = st.firsts[1];
+        const int mine = st.id[threadIdx.x];
+        const int at = first < 32 ? __popc(lo & ((1u << first) - 1u)) : __popc(lo) + __popc(hi & ((1u << (first - 32)) - 1u));
+        st.place[threadIdx.x] = mine >= 0 ? at : -1;
+        if (mine >= 0 && first == int(threadIdx.x)) st.adapter[at] = mine;
+        if (threadIdx.x == 0) st.distinct = __popc(lo) + __popc(hi);
+    }
+    __syncthreads();
+
+    const int cap = kRows / p.R, groups = (st.distinct + cap - 1) / cap;  // adapters of a product, products of the tile
+    const int kbs = (p.K + kKElems - 1) / kKElems;
+    const int kb0 = rank * kbs / split, kb1 = (rank + 1) * kbs / split;
+    if (kb0 == kb1)
+        for (int i = threadIdx.x; i < kShrinkTok * p.R; i += kShrinkThreads) part[i] = 0.0f;
+    if (warp == 0 && kb0 < kb1) {
+        if (ptx::elect_one()) {
+            int it = 0;
+            bool ok = true;
+            for (int g = slot; ok && g < groups; g += p.slots) {
+                const int n = min(cap, st.distinct - g * cap);
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = it % kShrinkStages;
+                    if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / kShrinkStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+                    uint8_t* a = ring + s * kShrinkStage;
+                    ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(n * p.R + kShrinkTok) * kKBytes);
+                    ptx::tma_load_2d(a + kABytes, &map_x, kb * kKElems, tile * kShrinkTok, &st.full[s]);
+                    for (int i = 0; i < n; ++i)
+                        ptx::tma_load_2d(a + i * p.R * kKBytes, &map_a, kb * kKElems, st.adapter[g * cap + i] * p.R, &st.full[s]);
+                }
+            }
+            if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
+                const long long t0 = clock64();
+                for (int i = max(0, it - kShrinkStages); i < it; ++i)
+                    while (!ptx::mbar_try_wait(&st.full[i % kShrinkStages], (i / kShrinkStages) & 1) && clock64() - t0 < kWaitLimit) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1 && kb0 < kb1) {
+        if (ptx::elect_one()) {
+            const uint32_t idesc = ptx::make_idesc(p.half ? 0 : 1, kRows, kShrinkTok);
+            int it = 0, acc = 0;
+            bool ok = true;
+            for (int g = slot; ok && g < groups; g += p.slots, ++acc) {
+                if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = it % kShrinkStages;
+                    if (!(ok = ptx::mbar_wait(&st.full[s], (it / kShrinkStages) & 1, &st.abort_flag, kWaitLimit))) break;
+                    ptx::tc_fence_after();
+                    const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * kShrinkStage));
+                    const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * kShrinkStage + kABytes));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        ptx::umma<1>(tmem + (acc & 1) * kShrinkTok, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc,
+                                     kb > kb0 || k > 0);
+                    ptx::umma_commit(&st.empty[s]);
+                }
+                ptx::umma_commit(&st.tmem_full[acc & 1]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4 && kb0 < kb1) {
+        const int row = (warp - 4) * 32 + lane, mine = row / p.R, r = row - mine * p.R;
+        int acc = 0;
+        for (int g = slot; g < groups; g += p.slots, ++acc) {
+            if (!ptx::mbar_wait_warp(&st.tmem_full[acc & 1], (acc >> 1) & 1, &st.abort_flag, kWaitLimit)) break;
+            ptx::tc_fence_after();
+            for (int c = 0; c < kShrinkTok; c += 32) {
+                float v[32];
+                ptx::tmem_read<32>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
+                ptx::tmem_landed<32>(v);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (mine < cap && st.place[c + i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[acc & 1]);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && st.abort_flag != 0) *p.status = kStatusShrink;
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 2 * kShrinkTok);
+    }
+    __syncwarp();
+    // the slices of K in their order; each block of the cluster adds its share of the values
+    ptx::cluster_sync();
+    bool over = false;
+    for (int i = rank * kShrinkThreads + threadIdx.x; i < kShrinkTok * p.R; i += split * kShrinkThreads) {
+        const int t = i / p.R, r = i - t * p.R;
+        const int place = st.place[t];
+        if (place < 0 || (place / cap) % p.slots != slot) continue;
+        float sum = 0.0f;
+        for (int c = 0; c < split; ++c) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(part + i, c)) : "memory");
+            sum += v;
+        }
+        if (p.scale != nullptr) sum *= p.scale[st.id[t]];
+        const size_t at = size_t(tile * kShrinkTok + t) * p.R + r;
+        p.z[at] = sum;
+        p.z16[at] = to_bits(sum, p.half);
+        over |= p.half && !(fabsf(sum) <= 65504.0f);
+    }
+    if (over) st.overflow = 1;
+    __syncthreads();
+    ptx::cluster_sync();  // orders the flags, too, and the others read this block's shared memory until here
+    if (slot == 0 && rank == 0 && threadIdx.x == 0) {
+        const int rows = min(kShrinkTok, p.T - tile * kShrinkTok);
+        bool all = true;
+        for (int t = 0; t < rows; ++t) all = all && st.id[t] == st.id[0];
+        int over_any = 0;
+        for (int c = 0; c < split; ++c) {
+            int v;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_cta(&st.overflow, c)) : "memory");
+            over_any |= v;
+        }
+        p.info[tile] = !all || over_any ? kMixed : st.id[0] >= 0 ? st.id[0] : kNone;
+    }
+    __syncthreads();
+    ptx::cluster_sync();
+}
+
+// ---------------------------------------------------------------- project
+
+constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
+constexpr int kMaxTok = 256;
+constexpr int kRingBytes = 200 * 1024;
+constexpr int kMaxStages = 10;
+constexpr int kChunk = 16;                      // columns that an epilogue warp takes at a time
+
+struct Params {
+    const int* ids;
+    const float* z;
+    const int* info;
+    const uint16_t* lora_b;   // [L, N, R]
+    const float* bias;        // [N] or null
+    uint16_t* y;
+    int64_t ldy;
+    int T, N, K, L, R;
+    int tok;                  // rows of x per tile: 16, 32, 64, 128 or 256
+    int stages;
+    int n_tiles, tiles;       // tiles along N, and in all
+    int kbs;
+    int whole;                // tiles that are not split: block b takes b, b + grid, ...; the others are cut into equal shares
+    int shares;               // of the others
+    int by_mma;               // z B^T by MMA where a tile has one adapter
+    int* counters;            // parts seen of each split tile
+    float* part;              // [shares][2][tok][128]
+    int* status;
+};
+struct alignas(16) Tail {
+    uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2];
+    uint64_t meet;            // the epilogue warps
+    uint32_t tmem_base;
+    int abort_flag;
+    int last_part;
+    alignas(16) float z[8][kChunk * 8];  // per epilogue warp: 16 rows' z at eight ranks
+};
+constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
+
+struct Piece {
+    int tile, kb0, kb1;
+    int part;                 // slot of its partial sums, -1 for a whole tile
+};
+// The pieces of a block, in order: its whole tiles, then those of its share of the others.
+struct Pieces {
+    const Params& p;
+    int whole, u, hi, lo;
+    __device__ __forceinline__ explicit Pieces(const Params& p_) : p(p_), whole(blockIdx.x), u(0), hi(0), lo(0) {
+        if (int(blockIdx.x) < p.shares) {
+            const int units = (p.tiles - p.whole) * p.kbs;
+            lo = u = streamk::first_unit(blockIdx.x, p.shares, units);
+            hi = streamk::first_unit(blockIdx.x + 1, p.shares, units);
+        }
+    }
+    __device__ __forceinline__ bool next(Piece* q) {
+        if (whole < p.whole) {
+            *q = Piece{whole, 0, p.kbs, -1};
+            whole += gridDim.x;
+            return true;
+        }
+        if (u >= hi) return false;
+        const int tile = u / p.kbs, end = min(hi, (tile + 1) * p.kbs);
+        *q = Piece{p.whole + tile, u - tile * p.kbs, end - tile * p.kbs, 2 * int(blockIdx.x) + (tile == lo / p.kbs ? 0 : 1)};
+        if (q->kb0 == 0 && q->kb1 == p.kbs) q->part = -1;
+        u = end;
+        return true;
+    }
+};
+
+// The adapter of a row tile: id, kNone or kMixed.
+__device__ __forceinline__ int tile_adapter(const Params& p, int tt) {
+    const int i0 = tt * (p.tok / kShrinkTok), i1 = min(i0 + p.tok / kShrinkTok, (p.T + kShrinkTok - 1) / kShrinkTok);
+    const int a = p.info[i0];
+    for (int i = i0 + 1; i < i1; ++i)
+        if (p.info[i] != a) return kMixed;
+    return a;
+}
+
+template <bool kHalf>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (kHalf) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(bf16_lo(w), bf16_hi(w));
+}
+
+template <bool kHalf>
+struct Epilogue {
+    const Params& p;
+    Tail& st;
+    uint32_t tmem;
+    int warp, lane, row;      // warp 0..7, row = TMEM lane = row of W in the tile
+    uint32_t meetings = 0;
+
+    __device__ __forceinline__ bool meet() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&st.meet);
+        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
+    }
+
+    // v[j] += z[t0 + j] . B_a(t0 + j)[n] for 16 rows of x, eight ranks at a time
+    __device__ __forceinline__ void expand(float (&v)[kChunk], int t0, int n) {
+        const int id = lane < kChunk && t0 + lane < p.T ? p.ids[t0 + lane] : -1;
+        const int mine = id >= 0 && id < p.L ? id : -1;
+        if (__all_sync(0xffffffffu, mine < 0)) return;
+        float* zs = st.z[warp];
+        for (int r0 = 0; r0 < p.R; r0 += 8) {
+            uint4 b[kChunk];  // all loads before the first use
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                const int a = __shfl_sync(0xffffffffu, mine, j);
+                b[j] = make_uint4(0, 0, 0, 0);
+                if (a >= 0 && n < p.N) b[j] = *reinterpret_cast<const uint4*>(p.lora_b + (size_t(a) * p.N + n) * p.R + r0);
+            }
+            const int a = __shfl_sync(0xffffffffu, mine, lane >> 1);
+            float4 zv = make_float4(0, 0, 0, 0);
+            if (a >= 0) zv = *reinterpret_cast<const float4*>(p.z + size_t(t0 + (lane >> 1)) * p.R + r0 + (lane & 1) * 4);
+            __syncwarp();
+            *reinterpret_cast<float4*>(zs + lane * 4) = zv;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                const float4 z0 = *reinterpret_cast<const float4*>(zs + j * 8), z1 = *reinterpret_cast<const float4*>(zs + j * 8 + 4);
+                const float2 b0 = unpack2<kHalf>(b[j].x), b1 = unpack2<kHalf>(b[j].y), b2 = unpack2<kHalf>(b[j].z), b3 = unpack2<kHalf>(b[j].w);
+                float s = v[j];
+                s = fmaf(b0.x, z0.x, s), s = fmaf(b0.y, z0.y, s), s = fmaf(b1.x, z0.z, s), s = fmaf(b1.y, z0.w, s);
+                s = fmaf(b2.x, z1.x, s), s = fmaf(b2.y, z1.y, s), s = fmaf(b3.x, z1.z, s), s = fmaf(b3.y, z1.w, s);
+                v[j] = s;
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(float (&v)[kChunk], int tt, int c, int n, bool by_thread) {
+        const int t0 = tt * p.tok + c;
+        if (by_thread) expand(v, t0, n);
+        if (n < p.N) {
+            const float bias = p.bias != nullptr ? p.bias[n] : 0.0f;
+            uint16_t* y = p.y + int64_t(t0) * p.ldy + n;
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j)
+                if (t0 + j < p.T) y[j * p.ldy] = to_bits(v[j] + bias, kHalf);
+        }
+    }
+
+    __device__ __forceinline__ void run() {
+        pdl_wait();  // shrink: z, the counters
+        Pieces pieces(p);
+        Piece q;
+        for (int acc = 0; pieces.next(&q); ++acc) {
+            const int tt = q.tile / p.n_tiles, n = (q.tile - tt * p.n_tiles) * kRows + row;
+            const int adapter = p.by_mma ? tile_adapter(p, tt) : kMixed;
+            const int buf = acc & 1;
+            if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (acc >> 1) & 1, &st.abort_flag, kWaitLimit)) return;
+            ptx::tc_fence_after();
+            const uint32_t from = tmem + (uint32_t((warp & 3) * 32) << 16) + buf * p.tok;
+            // columns in use; the two warps of a lane quarter take chunks in turn
+            const int cols = min(p.tok, p.T - tt * p.tok);
+            for (int c = (warp >> 2) * kChunk; c < cols; c += 2 * kChunk) {
+                float v[kChunk];
+                ptx::tmem_read<kChunk>(from + c, v);
+                ptx::tmem_landed<kChunk>(v);
+                if (q.part < 0) {
+                    store(v, tt, c, n, adapter == kMixed);
+                } else {
+                    float* to = p.part + (size_t(q.part) * p.tok + c) * kRows + row;
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) to[j * kRows] = v[j];
+                }
+            }
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf]);
+            if (q.part < 0) continue;
+            const int local = q.tile - p.whole, units = (p.tiles - p.whole) * p.kbs;
+            const int first = streamk::share_of(local * p.kbs, p.shares, units), last = streamk::share_of((local + 1) * p.kbs - 1, p.shares, units);
+            __threadfence();
+            if (!meet()) return;
+            if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(&p.counters[local], 1) == last - first;
+            if (!meet()) return;
+            if (*const_cast<volatile int*>(&st.last_part) == 0) continue;
+            __threadfence();
+            for (int c = (warp >> 2) * kChunk; c < cols; c += 2 * kChunk) {
+                float v[kChunk];
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
+                for (int o = first; o <= last; ++o) {
+                    const int slot = 2 * o + (local == streamk::first_unit(o, p.shares, units) / p.kbs ? 0 : 1);
+                    const float* part = p.part + (size_t(slot) * p.tok + c) * kRows + row;
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) v[j] += streamk::ld_partial(part + j * kRows);
+                }
+                store(v, tt, c, n, adapter == kMixed);
+            }
+        }
+    }
+};
+
+template <bool kHalf>
+__global__ void __launch_bounds__(kThreads, 1)
+lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_z,
+                    const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params p) {
+    pdl_launch();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Tail& st = *reinterpret_cast<Tail*>(ring + kRingBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stage = kABytes + p.tok * kKBytes;
+    const uint32_t tmem_cols = uint32_t(2 * p.tok);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            ptx::mbar_init(&st.full[i], 1);
+            ptx::mbar_init(&st.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&st.tmem_full[i], 1);
+            ptx::mbar_init(&st.tmem_empty[i], 8);
+        }
+        ptx::mbar_init(&st.meet, 8);
+        st.abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(&st.tmem_base, tmem_cols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
+
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            Pieces pieces(p);
+            Piece q;
+            int it = 0;
+            bool ok = true, waited = false;
+            auto slot_free = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
+            while (ok && pieces.next(&q)) {
+                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows;
+                for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
+                    if (!(ok = slot_free())) break;
+                    const int s = it % p.stages;
+                    ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
+                    ptx::tma_load_2d(ring + s * stage, &map_w, kb * kKElems, n0, &st.full[s]);
+                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_x, kb * kKElems, tt * p.tok, &st.full[s]);
+                }
+                if (!ok || !p.by_mma || q.kb1 < p.kbs) continue;
+                if (!waited) pdl_wait();  // shrink
+                waited = true;
+                const int adapter = tile_adapter(p, tt);
+                if (adapter < 0) continue;
+                for (int r0 = 0; r0 < p.R; r0 += kKElems, ++it) {
+                    if (!(ok = slot_free())) break;
+                    const int s = it % p.stages;
+                    ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
+                    ptx::tma_load_3d<false>(ring + s * stage, &map_b, r0, n0, adapter, ptx::smem_u32(&st.full[s]));
+                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_z, r0, tt * p.tok, &st.full[s]);
+                }
+            }
+            if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
+                const long long t0 = clock64();
+                for (int i = max(0, it - p.stages); i < it; ++i)
+                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - t0 < kWaitLimit) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kRows, uint32_t(p.tok));
+            Pieces pieces(p);
+            Piece q;
+            int it = 0;
+            bool ok = true, waited = false;
+            for (int acc = 0; ok && pieces.next(&q); ++acc) {
+                const uint32_t d = tmem + (acc & 1) * p.tok;
+                if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+                ptx::tc_fence_after();
+                auto block = [&](int steps, bool more) {
+                    const int s = it % p.stages;
+                    if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit)) return false;
+                    ptx::tc_fence_after();
+                    const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
+                    const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kABytes));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k < steps) ptx::umma<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
+                    ptx::umma_commit(&st.empty[s]);
+                    ++it;
+                    return true;
+                };
+                for (int kb = q.kb0; ok && kb < q.kb1; ++kb) ok = block(4, kb > q.kb0);
+                if (ok && p.by_mma && q.kb1 == p.kbs) {
+                    if (!waited) pdl_wait();
+                    waited = true;
+                    if (tile_adapter(p, q.tile / p.n_tiles) >= 0)
+                        for (int r0 = 0; ok && r0 < p.R; r0 += kKElems) ok = block(min(4, (p.R - r0 + 15) / 16), true);
+                }
+                if (ok) ptx::umma_commit(&st.tmem_full[acc & 1]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        Epilogue<kHalf> ep{p, st, tmem, warp - 4, lane, (warp & 3) * 32 + lane};
+        ep.run();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0 && st.abort_flag != 0) *p.status = kStatusProject;
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, tmem_cols);
+    }
+}
+
+// ---------------------------------------------------------------- host
+
+static int make_map(CUtensorMap* map, const void* base, bool half, int dims, const cuuint64_t* dim, const cuuint64_t* stride, const cuuint32_t* box) {
+    gemm::EncodeTiledFn fn = gemm::encode_fn();
+    if (fn == nullptr) return fail(DQMOE_ERR_CUDA, __FILE__, __LINE__, "cuTensorMapEncodeTiled", "driver entry point not found");
+    const cuuint32_t one[3] = {1, 1, 1};
+    const CUresult r = fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, cuuint32_t(dims), const_cast<void*>(base),
+                          dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(DQMOE_ERR_CUDA, __FILE__, __LINE__, "cuTensorMapEncodeTiled", "CUresult %d", int(r));
+    return DQMOE_OK;
+}
+static int make_map_2d(CUtensorMap* map, const void* base, bool half, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    const cuuint64_t dim[2] = {cuuint64_t(cols), cuuint64_t(rows)}, stride[1] = {cuuint64_t(ld) * 2};
+    const cuuint32_t box[2] = {kKElems, cuuint32_t(box_rows)};
+    return make_map(map, base, half, 2, dim, stride, box);
+}
+
+struct Layout {
+    size_t counters, info, z, z16, part, total;
+};
+static Layout plan(Params* p, int T, int N, int K, int R) {
+    p->T = T, p->N = N, p->K = K, p->R = R;
+    p->tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : kMaxTok;
+    const int stage = kABytes + p->tok * kKBytes;
+    p->stages = kRingBytes / stage < kMaxStages ? kRingBytes / stage : kMaxStages;
+    p->n_tiles = ceil_div(N, kRows);
+    p->tiles = p->n_tiles * ceil_div(T, p->tok);
+    p->kbs = ceil_div(K, kKElems);
+    p->by_mma = T > 128 ? 1 : 0;
+    const int sms = sm_count(), left = p->tiles % sms;
+    // a last round that is three quarters full is left as it is
+    p->whole = left * 4 >= sms * 3 ? p->tiles : p->tiles - left;
+    const int64_t units = int64_t(p->tiles - p->whole) * p->kbs;
+    p->shares = units < sms ? int(units) : sms;
+    Layout L{};
+    size_t off = 0;
+    auto add = [&](size_t bytes) {
+        const size_t at = off;
+        off += align_up(bytes, 256);
+        return at;
+    };
+    // for the most that a call of fewer rows splits, so that a workspace for the longest batch serves all
+    L.counters = add(size_t(sms) * sizeof(int));
+    L.info = add(size_t(ceil_div(T, kShrinkTok)) * sizeof(int));
+    L.z = add(size_t(T) * R * sizeof(float));
+    L.z16 = add(size_t(T) * R * 2);
+    L.part = add(size_t(sms) * 2 * p->tok * kRows * sizeof(float));
+    L.total = off;
+    return L;
+}
+
+static int check_sizes(int64_t T, int N, int K, int L, int R) {
+    DQ_CHECK(T >= 0 && N > 0 && K > 0 && L > 0 && R > 0);
+    DQ_CHECK_FMT(R % 8 == 0 && R <= kMaxRank, "R=%d: a multiple of 8, at most %d (pad A and B with zeros)", R, kMaxRank);
+    DQ_CHECK_FMT(K % 8 == 0, "K=%d: rows must be a multiple of 16 bytes", K);
+    // tile numbers, K blocks and the rows of the tensor maps are 32-bit
+    DQ_CHECK_FMT(T <= (1 << 24) && N <= (1 << 24) && K <= (1 << 24) && int64_t(L) * R < (int64_t(1) << 31) &&
+                     int64_t(ceil_div(N, kRows)) * ((T + 15) / 16) < (int64_t(1) << 31),
+                 "T=%lld N=%d K=%d L=%d: too large", (long long) T, N, K, L);
+    return DQMOE_OK;
+}
+
+template <class K>
+static int opt_in(K kern, int which, size_t bytes) {
+    static std::mutex mu;
+    static size_t configured[3][64] = {};
+    int dev = 0;
+    DQ_CUDA(cudaGetDevice(&dev));
+    DQ_CHECK(dev >= 0 && dev < 64);
+    std::lock_guard<std::mutex> lk(mu);
+    if (configured[which][dev] < bytes) {
+        DQ_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)));
+        configured[which][dev] = bytes;
+    }
+    return DQMOE_OK;
+}
+
+}  // namespace lora
+}  // namespace dq
+
+using namespace dq;
+
+extern "C" {
+
+size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R) {
+    if (lora::check_sizes(T, N, K, L, R) != DQMOE_OK) return 0;
+    lora::Params p{};
+    return lora::plan(&p, T, N, K, R).total;
+}
+
+int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lora_a, const void* lora_b, const int32_t* ids, const float* scale,
+                      const float* bias, void* y, int64_t ldy, void* workspace, size_t workspace_bytes, int T, int N, int K, int L, int R,
+                      int type, dqmoe_stream_t stream_) {
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    DQ_RC(lora::check_sizes(T, N, K, L, R));
+    DQ_CHECK_FMT(type == DQMOE_DT_BF16 || type == DQMOE_DT_HALF, "type=%d: BF16 or HALF", type);
+    if (T == 0) return DQMOE_OK;
+    DQ_CHECK(x != nullptr && w != nullptr && lora_a != nullptr && lora_b != nullptr && ids != nullptr && y != nullptr);
+    DQ_CHECK(is_aligned(x, 16) && is_aligned(w, 16) && is_aligned(lora_a, 16) && is_aligned(lora_b, 16) && is_aligned(y, 2) && is_aligned(ids, 4));
+    DQ_CHECK(is_aligned(scale, 4) && is_aligned(bias, 4));
+    DQ_CHECK_FMT(ldx >= K && ldx % 8 == 0 && ldx < (int64_t(1) << 36), "ldx=%lld: a multiple of 8, at least K", (long long) ldx);
+    DQ_CHECK_FMT(ldy >= N, "ldy=%lld: at least N", (long long) ldy);
+    DQ_CHECK_FMT(workspace != nullptr && is_aligned(workspace, 256), "workspace pointer %p is not aligned!", workspace);
+    lora::Params p{};
+    const lora::Layout Y = lora::plan(&p, T, N, K, R);
+    if (workspace_bytes != 0 && workspace_bytes < Y.total)
+        return fail(DQMOE_ERR_WORKSPACE, __FILE__, __LINE__, "workspace_bytes >= dqmoe_lora_linear_workspace_bytes(...)",
+                    "workspace has %zu bytes, the projection needs %zu", workspace_bytes, Y.total);
+    const bool half = type == DQMOE_DT_HALF;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    int* status = device_status_word();
+    if (status == nullptr) return DQMOE_ERR_CUDA;
+
+    lora::ShrinkParams sp{};
+    sp.ids = ids, sp.scale = scale;
+    sp.z = reinterpret_cast<float*>(ws + Y.z), sp.z16 = reinterpret_cast<uint16_t*>(ws + Y.z16);
+    sp.info = reinterpret_cast<int*>(ws + Y.info), sp.counters = reinterpret_cast<int*>(ws + Y.counters);
+    sp.n_counters = p.tiles - p.whole;
+    sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status;
+    // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached.
+    const int tiles = ceil_div(T, lora::kShrinkTok), room = 2 * sm_count();
+    int split = lora::kMaxSplit;
+    while (split > 1 && (tiles * split > room || split > p.kbs)) split /= 2;
+    const int most = ceil_div(L < lora::kShrinkTok ? (L < T ? L : T) : (T < lora::kShrinkTok ? T : lora::kShrinkTok), lora::kRows / R);
+    const int fit = room / (tiles * split);
+    sp.slots = fit < 1 ? 1 : fit < most ? fit : most;
+
+    CUtensorMap xs, a, xp, wm, zm{}, bm{};
+    DQ_RC(lora::make_map_2d(&xs, x, half, T, K, ldx, lora::kShrinkTok));
+    DQ_RC(lora::make_map_2d(&a, lora_a, half, int64_t(L) * R, K, K, R));
+    DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, p.tok));
+    DQ_RC(lora::make_map_2d(&wm, w, half, N, K, K, lora::kRows));
+    if (p.by_mma) {
+        DQ_RC(lora::make_map_2d(&zm, sp.z16, half, T, R, R, p.tok));
+        const cuuint64_t dim[3] = {cuuint64_t(R), cuuint64_t(N), cuuint64_t(L)}, stride[2] = {cuuint64_t(R) * 2, cuuint64_t(N) * R * 2};
+        const cuuint32_t box[3] = {lora::kKElems, lora::kRows, 1};
+        DQ_RC(lora::make_map(&bm, lora_b, half, 3, dim, stride, box));
+    }
+    {
+        const size_t smem = lora::shrink_smem(R);
+        DQ_RC(lora::opt_in(lora::lora_shrink_kernel, 0, smem));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(tiles) * sp.slots * split, 1, 1);
+        cfg.blockDim = dim3(lora::kShrinkThreads, 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = unsigned(split);
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        DQ_CUDA(cudaLaunchKernelEx(&cfg, lora::lora_shrink_kernel, xs, a, sp));
+    }
+    p.ids = ids, p.z = sp.z, p.info = sp.info, p.lora_b = static_cast<const uint16_t*>(lora_b), p.bias = bias;
+    p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
+    p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
+    const int sms = sm_count();
+    const int grid = p.whole > 0 ? (p.whole < sms ? (p.whole > p.shares ? p.whole : p.shares) : sms) : p.shares;
+    if (half) {
+        DQ_RC(lora::opt_in(lora::lora_project_kernel<true>, 1, lora::kSmemBytes));
+        return launch_pdl(lora::lora_project_kernel<true>, dim3(grid), lora::kThreads, lora::kSmemBytes, stream, xp, wm, zm, bm, p);
+    }
+    DQ_RC(lora::opt_in(lora::lora_project_kernel<false>, 2, lora::kSmemBytes));
+    return launch_pdl(lora::lora_project_kernel<false>, dim3(grid), lora::kThreads, lora::kSmemBytes, stream, xp, wm, zm, bm, p);
+}
+
+}  // extern "C"

@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_decode_route_kernel(const _
     const int warps = gridDim.x * (kRouteThreads / 32);
     for (int u = blockIdx.x * (kRouteThreads / 32) + warp; u < p.kb1 * p.T; u += warps) lay_out_x<kFp8>(p, u / p.T, u % p.T, tp, lane);
     if (!working) return;  // whole clusters
+    __syncthreads();
     ptx::cluster_sync();
     const int mine = chunk * 8 + rank;  // the expert whose slices this block adds
     if (mine < p.E && threadIdx.x < p.T) {
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_decode_route_kernel(const _
         }
         p.logits[size_t(threadIdx.x) * p.E + mine] = sum;
     }
+    __syncthreads();
     ptx::cluster_sync();  // the other blocks read this one's shared memory
 }
 
@@ -403,30 +405,6 @@ __device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* rin
     }
 }
 
-// columns [c, c + kCount) of this warp's lanes
-template <int kCount>
-__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
-    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
-    uint32_t* u = reinterpret_cast<uint32_t*>(r);
-    if constexpr (kCount == 8) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(taddr) : "memory");
-    } else if constexpr (kCount == 16) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-                       "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]) : "r"(taddr) : "memory");
-    } else {
-        ptx::tmem_ld32(taddr, *reinterpret_cast<uint32_t (*)[32]>(&r));
-    }
-}
-// Wait for the loads; the registers pass through statements behind the wait.
-template <int kCount>
-__device__ __forceinline__ void tmem_landed(float (&a)[kCount], float (&b)[kCount]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i])::"memory");
-}
-
 // Scale of a weight row in a unit: constant over the weights (bf16: 1), an expert, a row, or a 128x128 block.
 __device__ __forceinline__ float weight_scale(const float* scale, int mode, int e, int rows, int row, int blocks_k, int kb) {
     if (mode == DQMOE_QUANT_FP8_BLOCK) return scale[(size_t(e) * ((rows + 127) / 128) + row / 128) * blocks_k + kb];
@@ -476,9 +454,9 @@ struct Epilogue {
     // sum += (hi + lo / 16) * scale of every token of `mask`
     __device__ __forceinline__ void add_scaled(uint32_t taddr, const float* token_scale, float row_scale, uint32_t mask, float (&sum)[kTp]) {
         float hi[kTp], lo[kTp];
-        tmem_read<kTp>(taddr, hi);
-        tmem_read<kTp>(taddr + kTp, lo);
-        tmem_landed<kTp>(hi, lo);
+        ptx::tmem_read<kTp>(taddr, hi);
+        ptx::tmem_read<kTp>(taddr + kTp, lo);
+        ptx::tmem_landed<kTp>(hi, lo);
 #pragma unroll
         for (int t = 0; t < kTp; t += 4) {
             const float4 sc = *reinterpret_cast<const float4*>(token_scale + t);
@@ -591,9 +569,9 @@ struct Epilogue {
                 it += end - u;
                 u = end;
                 if (!acquire()) return false;
-                tmem_read<kTp>(buffer(), g);
-                tmem_read<kTp>(buffer() + S::kN1, v);
-                tmem_landed<kTp>(g, v);
+                ptx::tmem_read<kTp>(buffer(), g);
+                ptx::tmem_read<kTp>(buffer() + S::kN1, v);
+                ptx::tmem_landed<kTp>(g, v);
                 release_buffer();
             }
             const int first = streamk::share_of(tile * p.kb1, shares, units), last = streamk::share_of((tile + 1) * p.kb1 - 1, shares, units);
@@ -665,9 +643,9 @@ struct Epilogue {
                     u = stop;
                     if (!acquire()) return false;
                     float hi[kTp], lo[kTp];
-                    tmem_read<kTp>(buffer(), hi);
-                    tmem_read<kTp>(buffer() + kTp, lo);
-                    tmem_landed<kTp>(hi, lo);
+                    ptx::tmem_read<kTp>(buffer(), hi);
+                    ptx::tmem_read<kTp>(buffer() + kTp, lo);
+                    ptx::tmem_landed<kTp>(hi, lo);
                     release_buffer();
                     const uint32_t mask = st.hit_mask[j];
 #pragma unroll

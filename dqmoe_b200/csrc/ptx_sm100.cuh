@@ -496,6 +496,36 @@ __device__ __forceinline__ void tmem_wait_ld2(uint32_t (&a)[32], uint32_t (&b)[3
                  : "memory");
 }
 
+// 32 lanes x kCount consecutive fp32 columns, as floats: thread i of the warp receives the columns of lane i. Valid behind tmem_landed.
+template <int kCount>
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
+    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
+    uint32_t* u = reinterpret_cast<uint32_t*>(r);
+    if constexpr (kCount == 8) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(taddr) : "memory");
+    } else if constexpr (kCount == 16) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+                       "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]) : "r"(taddr) : "memory");
+    } else {
+        tmem_ld32(taddr, *reinterpret_cast<uint32_t (*)[32]>(&r));
+    }
+}
+// Wait for this thread's outstanding tcgen05.ld; the registers pass through statements behind the wait.
+template <int kCount>
+__device__ __forceinline__ void tmem_landed(float (&a)[kCount], float (&b)[kCount]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i])::"memory");
+}
+template <int kCount>
+__device__ __forceinline__ void tmem_landed(float (&a)[kCount]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i])::"memory");
+}
+
 // 16 lanes x 32 fp32 columns as matrix fragments (the lower or the upper half of the warp's lane quarter, by the lane field of
 // taddr): registers 4g, 4g+1 hold columns 8g + 2 (lane % 4) + {0, 1} of row lane / 4, registers 4g+2, 4g+3 those of row lane / 4 + 8.
 __device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {

@@ -573,3 +573,62 @@ def requant_from_amax(act: torch.Tensor, amax: torch.Tensor, per_row: bool, n_ro
         _lib.check(_lib.load().dqmoe_requant_from_amax_dev(_p(act), n, I, _p(amax), int(per_row), _p(q), _p(s),
                                                            _p(n_rows_device), _stream(act.device)))
     return q, s
+
+
+# ---------------------------------------------------------------------- projections with adapters
+
+def lora_linear_workspace_bytes(T: int, N: int, K: int, L: int, R: int) -> int:
+    """Bytes of workspace for lora_linear; 0 where the sizes are not ones it takes."""
+    return int(_lib.load().dqmoe_lora_linear_workspace_bytes(T, N, K, L, R))
+
+
+def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor, ids: torch.Tensor,
+                scale: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y = x W^T + bias + scale[a] (x A_a^T) B_a^T with a = ids[t] for each row t of x; see dqmoe_lora_linear.
+
+    x [T, K], w [N, K], lora_a [L, R, K], lora_b [L, N, R], all bf16 or all fp16; ids int32 [T] (outside [0, L): no adapter), scale fp32
+    [L], bias fp32 [N]. x and out may have rows that stand apart (columns next to each other). Returns y [T, N]."""
+    for name, t in (("w", w), ("lora_a", lora_a), ("lora_b", lora_b), ("ids", ids)):
+        _cuda(t, name)
+    for name, t in (("x", x), ("out", out)):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name}.is_cuda  Info: dqmoe_b200 has no CPU path")
+        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a matrix whose rows lie apart and whose columns lie together")
+    if x.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != x.dtype for t in (w, lora_a, lora_b)):
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: x, w, lora_a and lora_b are all bf16 or all fp16")
+    T, K = x.shape
+    if w.dim() != 2 or w.shape[1] != K or lora_a.dim() != 3 or lora_a.shape[2] != K:
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: w is [N, K] and lora_a [L, R, K]")
+    N, (L, R) = w.shape[0], lora_a.shape[:2]
+    if tuple(lora_b.shape) != (L, N, R):
+        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: lora_b is [L, N, R]  Info: got {tuple(lora_b.shape)}, want {(L, N, R)}")
+    if ids.dtype != torch.int32 or tuple(ids.shape) != (T,):
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: ids is int32 [T]")
+    for name, t, n in (("scale", scale, L), ("bias", bias, N)):
+        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (n,)):
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor [{n}]")
+    if out is None:
+        out = torch.empty((T, N), dtype=x.dtype, device=x.device)
+    elif tuple(out.shape) != (T, N) or out.dtype != x.dtype:
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is [T, N] of x's type")
+    lib = _lib.load()
+    if workspace is None:
+        need = int(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R))
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
+    else:
+        _cuda(workspace, "workspace")
+    for name, t in (("w", w), ("lora_a", lora_a), ("lora_b", lora_b), ("ids", ids), ("scale", scale), ("bias", bias), ("out", out),
+                    ("workspace", workspace)):
+        if t is not None and t.device != x.device:
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
+    ldx = x.stride(0) if T > 1 else K
+    ldy = out.stride(0) if T > 1 else N
+    with torch.cuda.device(x.device):
+        _lib.check(lib.dqmoe_lora_linear(_p(x), ldx, _p(w), _p(lora_a), _p(lora_b), _p(ids), _p(scale), _p(bias), _p(out), ldy, _p(workspace),
+                                         workspace.numel() * workspace.element_size(), T, N, K, L, R,
+                                         DT_HALF if x.dtype == torch.float16 else DT_BF16, _stream(x.device)))
+    return out

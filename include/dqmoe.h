@@ -490,6 +490,23 @@ int dqmoe_grouped_gemm_nvfp4(const void* a, const uint8_t* a_sf, const float* a_
                              uint8_t* out_sf, const float* out_gscale, const int32_t* dest_to_src,
                              dqmoe_stream_t stream);
 
+/*
+ * A projection that many requests share, each row with its request's low-rank adapter beside it:
+ *   y[t] = x[t] W^T + bias + scale[a] * (x[t] A_a^T) B_a^T,  a = ids[t]
+ * x [T, K] with rows ldx elements apart (ldx a multiple of 8, >= K), w [N, K], lora_a [L, R, K], lora_b [L, N, R], y [T, N] with rows ldy
+ * >= N elements apart, all of `type` (DQMOE_DT_BF16 or DQMOE_DT_HALF); ids [T] int32, scale [L] fp32 or NULL (1), bias [N] fp32 or NULL.
+ * A row whose id is outside [0, L) has no adapter. Adapters of a lower rank are padded with zeros to R, a multiple of 8 up to 128; K is a
+ * multiple of 8; x, w, lora_a, lora_b are aligned to 16 bytes. The ids may come in any order; rows of one request that stand together
+ * are faster from 129 rows on. Sums are fp32, the result is rounded once; x A^T too is rounded to the operands' type where 256 rows
+ * (counted from the first) have one adapter, and held in fp32 elsewhere. No row's result depends on another row's adapter. Any T from 0
+ * on. dqmoe_device_status gives 311 or 312 where a wait ran out. A call has its workspace for itself until it is over. No counterpart in
+ * the reference.
+ */
+size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R);
+int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lora_a, const void* lora_b, const int32_t* ids,
+                      const float* scale, const float* bias, void* y, int64_t ldy, void* workspace, size_t workspace_bytes,
+                      int T, int N, int K, int L, int R, int type, dqmoe_stream_t stream);
+
 /* cumulative 128-row tile counts per expert from offsets[E+1] (device to device) */
 int dqmoe_mtile_prefix(const int32_t* offsets, int E, int32_t* mtile_prefix, dqmoe_stream_t stream);
 
