@@ -1,20 +1,24 @@
 // A projection that many requests share, each row with its request's low-rank adapter beside it, in two launches:
 //   y[t] = x[t] W^T + bias + scale_a (x[t] A_a^T) B_a^T,   a = ids[t]; rows whose id is outside [0, L) have no adapter.
 //
-//   shrink    z[t] = scale_a x[t] A_a^T, fp32 [T, R] and once more in the operands' type
-//   project   y = x W^T, with z B_a^T added to the same fp32 sums
+//   shrink    z[t] = scale_a x[t] A_a^T, [T, R] in the operands' type
+//   project   y = x W^T + z B_a^T, summed in fp32
 //
 // What bounds it: few rows the weights W and the adapters in use from HBM, many rows the tensor cores. project runs with W on the
-// tensor core's first operand (M = 128 rows of W) and up to 256 rows of x on the second, so that a decode batch computes few columns too
+// tensor core's first operand (M = 128 rows of W) and up to 224 rows of x on the second, so that a decode batch computes few columns too
 // many. Tiles that do not fill the chip are cut along K into equal shares per SM (streamk.cuh).
 //
-// Where a row tile of project belongs to one adapter - prefill, where a request's rows stand together - z B_a^T is further K blocks of the
-// same product. Elsewhere (decode batches, the tiles where requests meet) it is added by the threads of the epilogue, row by row with
-// its own B: masks on a mixed product would let one adapter's infinities reach the rows of another, and z keeps its 32 bits.
+// The adapters' part is MMAs, too: B_a on the first operand, rows of z on the second, 16 rows (the least N) at a time. Where 16 rows have
+// one adapter - prefill, where a request's rows stand together - the product goes on top of x W^T, for all such rows that follow one
+// another at once. Where they have several, each adapter's product gets 16 accumulator columns of its own, and the epilogue adds the columns
+// whose rows have that adapter: masks on a mixed product would let one adapter's infinities reach the rows of another. (The first form of
+// this kernel added z B^T in the epilogue's threads, each with its row of B: bound by L1, whose lines hold one row of B each, and on the
+// last block of a tile alone. 64 rows of 64 adapters, K 4096, N 6144, R 16: 70 us; 333 rows of 40 requests, 2880 x 2880, R 64: 489 us.)
+// The list of these products is made from the ids by a warp of each block, and divided among the parts of a tile like its K.
 // shrink takes 64 rows of x at a time against all adapters among them, several adapters' A stacked on M = 128, and keeps from the product
 // what belongs together.
 //
-// project starts while shrink runs: it reads only x, W and ids until a tile is summed up. That is sound because shrink lets it start
+// project starts while shrink runs: it reads only x and W until a tile's K is through. That is sound because shrink lets it start
 // behind its own wait for the kernels before, which wrote those. No counterpart in the reference.
 #include <mutex>
 
@@ -41,14 +45,12 @@ constexpr int kShrinkThreads = 256;             // warp 0 TMA, warp 1 MMA, warps
 constexpr int kShrinkStage = kABytes + kShrinkTok * kKBytes;
 constexpr int kShrinkStages = 4;
 constexpr int kMaxSplit = 8;                    // blocks of a cluster: slices of K
-constexpr int kNone = -1, kMixed = -2;          // a tile's adapter where it has not one
 
 struct ShrinkParams {
     const int* ids;
     const float* scale;     // [L] or null
-    float* z;               // [T, R]
-    uint16_t* z16;          // [T, R] in the operands' type
-    int* info;              // [ceil(T / 64)] adapter of a tile: id, kNone or kMixed
+    uint16_t* z;            // [T, R] in the operands' type
+    float* z_scale;         // [T], fp16: z counts times this power of two (1 but where a row's z would leave fp16's range)
     int* counters;          // project's, cleared here
     int n_counters;
     int T, K, L, R;
@@ -61,7 +63,6 @@ struct alignas(16) ShrinkTail {
     uint32_t tmem_base;
     int abort_flag;
     int distinct;                               // adapters of the tile
-    int overflow;                               // some z does not fit the operands' type
     int id[kShrinkTok];                         // -1 where there is none
     int place[kShrinkTok];                      // place of a row's adapter among the tile's
     int adapter[kShrinkTok];                    // the tile's adapters in the order of their first rows
@@ -96,7 +97,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             ptx::mbar_init(&st.tmem_empty[i], 4);
         }
         st.abort_flag = 0;
-        st.overflow = 0;
         ptx::fence_barrier_init();
     }
     if (warp == 1) {
@@ -214,79 +214,84 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         ptx::tmem_dealloc(tmem, 2 * kShrinkTok);
     }
     __syncwarp();
-    // the slices of K in their order; each block of the cluster adds its share of the values
+    // the slices of K in their order; each block of the cluster adds its share of the rows, a warp per row
     ptx::cluster_sync();
-    bool over = false;
-    for (int i = rank * kShrinkThreads + threadIdx.x; i < kShrinkTok * p.R; i += split * kShrinkThreads) {
-        const int t = i / p.R, r = i - t * p.R;
+    for (int t = warp * split + rank; t < kShrinkTok; t += split * (kShrinkThreads / 32)) {
         const int place = st.place[t];
         if (place < 0 || (place / cap) % p.slots != slot) continue;
-        float sum = 0.0f;
-        for (int c = 0; c < split; ++c) {
-            float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(part + i, c)) : "memory");
-            sum += v;
+        float4 sum = make_float4(0, 0, 0, 0);
+        if (lane * 4 < p.R) {
+            for (int c = 0; c < split; ++c) {
+                float4 v;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                             : "r"(ptx::map_to_cta(part + t * p.R + lane * 4, c)) : "memory");
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            const float scale = p.scale != nullptr ? p.scale[st.id[t]] : 1.0f;
+            sum.x *= scale, sum.y *= scale, sum.z *= scale, sum.w *= scale;
         }
-        if (p.scale != nullptr) sum *= p.scale[st.id[t]];
-        const size_t at = size_t(tile * kShrinkTok + t) * p.R + r;
-        p.z[at] = sum;
-        p.z16[at] = to_bits(sum, p.half);
-        over |= p.half && !(fabsf(sum) <= 65504.0f);
-    }
-    if (over) st.overflow = 1;
-    __syncthreads();
-    ptx::cluster_sync();  // orders the flags, too, and the others read this block's shared memory until here
-    if (slot == 0 && rank == 0 && threadIdx.x == 0) {
-        const int rows = min(kShrinkTok, p.T - tile * kShrinkTok);
-        bool all = true;
-        for (int t = 0; t < rows; ++t) all = all && st.id[t] == st.id[0];
-        int over_any = 0;
-        for (int c = 0; c < split; ++c) {
-            int v;
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::map_to_cta(&st.overflow, c)) : "memory");
-            over_any |= v;
+        const size_t row = size_t(tile) * kShrinkTok + t;
+        if (p.half) {
+            const float most = warp_max(fmaxf(fmaxf(fabsf(sum.x), fabsf(sum.y)), fmaxf(fabsf(sum.z), fabsf(sum.w))));
+            float up = 1.0f, down = 1.0f;
+            if (most > 32768.0f && most <= 3.402823466e38f) {  // 2^(exponent - 14): below 2^15 then
+                const int e = int(__float_as_uint(most) >> 23) - 127 - 14;
+                up = __uint_as_float(uint32_t(127 + e) << 23), down = __uint_as_float(uint32_t(127 - e) << 23);
+            }
+            sum.x *= down, sum.y *= down, sum.z *= down, sum.w *= down;
+            if (lane == 0) p.z_scale[row] = up;
         }
-        p.info[tile] = !all || over_any ? kMixed : st.id[0] >= 0 ? st.id[0] : kNone;
+        if (lane * 4 < p.R)
+            *reinterpret_cast<uint2*>(p.z + row * p.R + lane * 4) =
+                make_uint2(to_bits(sum.x, p.half) | (uint32_t(to_bits(sum.y, p.half)) << 16), to_bits(sum.z, p.half) | (uint32_t(to_bits(sum.w, p.half)) << 16));
     }
     __syncthreads();
-    ptx::cluster_sync();
+    ptx::cluster_sync();  // the others read this block's shared memory until here
 }
 
 // ---------------------------------------------------------------- project
 
-constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warps 4..11 epilogue
-constexpr int kMaxTok = 256;
+constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warp 2 list of the adapters' products, warps 4..11 epilogue
+constexpr int kMaxTok = 224;                    // two accumulators of a tile leave 64 columns of TMEM for four products of 16 rows
+constexpr int kTmemCols = 512;
 constexpr int kRingBytes = 200 * 1024;
 constexpr int kMaxStages = 10;
-constexpr int kChunk = 16;                      // columns that an epilogue warp takes at a time
+constexpr int kChunk = 16;                      // rows of x that are looked at together
+constexpr int kMaxSlots = 8;
 
 struct Params {
     const int* ids;
-    const float* z;
-    const int* info;
-    const uint16_t* lora_b;   // [L, N, R]
+    const float* z_scale;     // null unless fp16
     const float* bias;        // [N] or null
     uint16_t* y;
     int64_t ldy;
     int T, N, K, L, R;
-    int tok;                  // rows of x per tile: 16, 32, 64, 128 or 256
+    int tok;                  // rows of x per tile, a multiple of 16
     int stages;
+    int slots;                // accumulators of 16 columns for the products of mixed rows, for each half of the epilogue
     int n_tiles, tiles;       // tiles along N, and in all
     int kbs;
     int whole;                // tiles that are not split: block b takes b, b + grid, ...; the others are cut into equal shares
     int shares;               // of the others
-    int by_mma;               // z B^T by MMA where a tile has one adapter
     int* counters;            // parts seen of each split tile
     float* part;              // [shares][2][tok][128]
     int* status;
 };
+
+// Products of a part of a tile. Direct: adapter, first chunk | chunks << 8, all of whose rows have it. Mixed: adapter, chunk | its rows << 16.
+struct List {
+    int direct0, direct1, mixed0, mixed1;
+    uint2 direct[kMaxTok / kChunk], mixed[kMaxTok];
+};
 struct alignas(16) Tail {
     uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2];
+    uint64_t slot_full[2][kMaxSlots], slot_empty[2][kMaxSlots];  // by half of the epilogue
+    uint64_t list_full[2], list_empty[2];
     uint64_t meet;            // the epilogue warps
     uint32_t tmem_base;
     int abort_flag;
     int last_part;
-    alignas(16) float z[8][kChunk * 8];  // per epilogue warp: 16 rows' z at eight ranks
+    List list[2];
 };
 constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
@@ -294,53 +299,90 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 struct Piece {
     int tile, kb0, kb1;
     int part;                 // slot of its partial sums, -1 for a whole tile
+    int index, of;            // which of how many parts of its tile
 };
 // The pieces of a block, in order: its whole tiles, then those of its share of the others.
 struct Pieces {
     const Params& p;
-    int whole, u, hi, lo;
-    __device__ __forceinline__ explicit Pieces(const Params& p_) : p(p_), whole(blockIdx.x), u(0), hi(0), lo(0) {
+    int whole, u, hi, lo, units;
+    __device__ __forceinline__ explicit Pieces(const Params& p_) : p(p_), whole(blockIdx.x), u(0), hi(0), lo(0), units((p_.tiles - p_.whole) * p_.kbs) {
         if (int(blockIdx.x) < p.shares) {
-            const int units = (p.tiles - p.whole) * p.kbs;
             lo = u = streamk::first_unit(blockIdx.x, p.shares, units);
             hi = streamk::first_unit(blockIdx.x + 1, p.shares, units);
         }
     }
     __device__ __forceinline__ bool next(Piece* q) {
         if (whole < p.whole) {
-            *q = Piece{whole, 0, p.kbs, -1};
+            *q = Piece{whole, 0, p.kbs, -1, 0, 1};
             whole += gridDim.x;
             return true;
         }
         if (u >= hi) return false;
         const int tile = u / p.kbs, end = min(hi, (tile + 1) * p.kbs);
-        *q = Piece{p.whole + tile, u - tile * p.kbs, end - tile * p.kbs, 2 * int(blockIdx.x) + (tile == lo / p.kbs ? 0 : 1)};
-        if (q->kb0 == 0 && q->kb1 == p.kbs) q->part = -1;
+        const int first = streamk::share_of(tile * p.kbs, p.shares, units), last = streamk::share_of((tile + 1) * p.kbs - 1, p.shares, units);
+        *q = Piece{p.whole + tile, u - tile * p.kbs, end - tile * p.kbs, first == last ? -1 : 2 * int(blockIdx.x) + (tile == lo / p.kbs ? 0 : 1),
+                   int(blockIdx.x) - first, last - first + 1};
         u = end;
         return true;
     }
 };
 
-// The adapter of a row tile: id, kNone or kMixed.
-__device__ __forceinline__ int tile_adapter(const Params& p, int tt) {
-    const int i0 = tt * (p.tok / kShrinkTok), i1 = min(i0 + p.tok / kShrinkTok, (p.T + kShrinkTok - 1) / kShrinkTok);
-    const int a = p.info[i0];
-    for (int i = i0 + 1; i < i1; ++i)
-        if (p.info[i] != a) return kMixed;
-    return a;
-}
-
+// The adapters' products of a tile's rows, by one warp, and which of them belong to this part.
 template <bool kHalf>
-__device__ __forceinline__ float2 unpack2(uint32_t w) {
-    if constexpr (kHalf) return __half22float2(*reinterpret_cast<const __half2*>(&w));
-    else return make_float2(bf16_lo(w), bf16_hi(w));
+__device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane) {
+    int direct = 0, mixed = 0, last = -1, last_end = -1, last_first = 0;
+    const int rows = min(p.tok, p.T - t0), half = lane >> 4;
+    for (int c = 0; c * kChunk < rows; c += 2) {  // two chunks at a time, half a warp each
+        int id = -2;                              // no row
+        bool scaled = false;
+        if (c * kChunk + lane < rows) {
+            id = p.ids[t0 + c * kChunk + lane];
+            if (id < 0 || id >= p.L) id = -1;
+            if constexpr (kHalf) scaled = id >= 0 && p.z_scale[t0 + c * kChunk + lane] != 1.0f;
+        }
+        const uint32_t present = __ballot_sync(0xffffffffu, id >= -1), with = __ballot_sync(0xffffffffu, id >= 0);
+        if (with == 0) continue;
+        const uint32_t scales = __ballot_sync(0xffffffffu, scaled);
+        const uint32_t peers = __match_any_sync(0xffffffffu, 2 * id + half) >> (16 * half);  // of this half
+        bool mixes[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t here = 0xffffu << (16 * h);
+            mixes[h] = false;
+            if ((with & here) == 0) continue;
+            const int a = __shfl_sync(0xffffffffu, id, __ffs(with & here) - 1);
+            const uint32_t same = __ballot_sync(0xffffffffu, id == a) & here;
+            mixes[h] = same != (present & here) || (scales & here) != 0;
+            if (mixes[h]) continue;
+            if (a != last || c + h != last_end) {
+                last = a;
+                last_first = c + h;
+                ++direct;
+            }
+            last_end = c + h + 1;
+            if (lane == 0) l.direct[direct - 1] = make_uint2(uint32_t(a), uint32_t(last_first | ((last_end - last_first) << 8)));
+        }
+        // the two chunks' products in turn: the two halves of the epilogue work side by side
+        const bool leads = id >= 0 && (lane & 15) == __ffs(peers) - 1 && (half ? mixes[1] : mixes[0]);
+        const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+        const int n0 = __popc(leaders & 0xffffu), n1 = __popc(leaders >> 16);
+        const int r = __popc((leaders >> (16 * half)) & ((1u << (lane & 15)) - 1u));
+        if (leads) l.mixed[mixed + r + (half ? min(r + 1, n0) : min(r, n1))] = make_uint2(uint32_t(id), uint32_t(c + half) | (peers << 16));
+        mixed += n0 + n1;
+    }
+    if (lane == 0) {
+        l.direct0 = direct * q.index / q.of;
+        l.direct1 = direct * (q.index + 1) / q.of;
+        l.mixed0 = mixed * q.index / q.of;
+        l.mixed1 = mixed * (q.index + 1) / q.of;
+    }
 }
 
 template <bool kHalf>
 struct Epilogue {
     const Params& p;
     Tail& st;
-    uint32_t tmem;
+    uint32_t tmem;            // this warp's lanes
     int warp, lane, row;      // warp 0..7, row = TMEM lane = row of W in the tile
     uint32_t meetings = 0;
 
@@ -350,98 +392,94 @@ struct Epilogue {
         return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
     }
 
-    // v[j] += z[t0 + j] . B_a(t0 + j)[n] for 16 rows of x, eight ranks at a time
-    __device__ __forceinline__ void expand(float (&v)[kChunk], int t0, int n) {
-        const int id = lane < kChunk && t0 + lane < p.T ? p.ids[t0 + lane] : -1;
-        const int mine = id >= 0 && id < p.L ? id : -1;
-        if (__all_sync(0xffffffffu, mine < 0)) return;
-        float* zs = st.z[warp];
-        for (int r0 = 0; r0 < p.R; r0 += 8) {
-            uint4 b[kChunk];  // all loads before the first use
+    __device__ __forceinline__ void store(float (&v)[kChunk], int t0, int n) {
+        if (n >= p.N) return;
+        const float bias = p.bias != nullptr ? p.bias[n] : 0.0f;
+        uint16_t* y = p.y + int64_t(t0) * p.ldy + n;
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                const int a = __shfl_sync(0xffffffffu, mine, j);
-                b[j] = make_uint4(0, 0, 0, 0);
-                if (a >= 0 && n < p.N) b[j] = *reinterpret_cast<const uint4*>(p.lora_b + (size_t(a) * p.N + n) * p.R + r0);
-            }
-            const int a = __shfl_sync(0xffffffffu, mine, lane >> 1);
-            float4 zv = make_float4(0, 0, 0, 0);
-            if (a >= 0) zv = *reinterpret_cast<const float4*>(p.z + size_t(t0 + (lane >> 1)) * p.R + r0 + (lane & 1) * 4);
-            __syncwarp();
-            *reinterpret_cast<float4*>(zs + lane * 4) = zv;
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                const float4 z0 = *reinterpret_cast<const float4*>(zs + j * 8), z1 = *reinterpret_cast<const float4*>(zs + j * 8 + 4);
-                const float2 b0 = unpack2<kHalf>(b[j].x), b1 = unpack2<kHalf>(b[j].y), b2 = unpack2<kHalf>(b[j].z), b3 = unpack2<kHalf>(b[j].w);
-                float s = v[j];
-                s = fmaf(b0.x, z0.x, s), s = fmaf(b0.y, z0.y, s), s = fmaf(b1.x, z0.z, s), s = fmaf(b1.y, z0.w, s);
-                s = fmaf(b2.x, z1.x, s), s = fmaf(b2.y, z1.y, s), s = fmaf(b3.x, z1.z, s), s = fmaf(b3.y, z1.w, s);
-                v[j] = s;
-            }
-        }
-    }
-
-    __device__ __forceinline__ void store(float (&v)[kChunk], int tt, int c, int n, bool by_thread) {
-        const int t0 = tt * p.tok + c;
-        if (by_thread) expand(v, t0, n);
-        if (n < p.N) {
-            const float bias = p.bias != nullptr ? p.bias[n] : 0.0f;
-            uint16_t* y = p.y + int64_t(t0) * p.ldy + n;
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j)
-                if (t0 + j < p.T) y[j * p.ldy] = to_bits(v[j] + bias, kHalf);
-        }
+        for (int j = 0; j < kChunk; ++j)
+            if (t0 + j < p.T) y[j * p.ldy] = to_bits(v[j] + bias, kHalf);
     }
 
     __device__ __forceinline__ void run() {
-        pdl_wait();  // shrink: z, the counters
+        pdl_wait();  // shrink: the counters, z_scale
         Pieces pieces(p);
         Piece q;
+        const int half = warp >> 2;
+        int slot_it = 0;
         for (int acc = 0; pieces.next(&q); ++acc) {
-            const int tt = q.tile / p.n_tiles, n = (q.tile - tt * p.n_tiles) * kRows + row;
-            const int adapter = p.by_mma ? tile_adapter(p, tt) : kMixed;
-            const int buf = acc & 1;
-            if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (acc >> 1) & 1, &st.abort_flag, kWaitLimit)) return;
+            const int tt = q.tile / p.n_tiles, n = (q.tile - tt * p.n_tiles) * kRows + row, t0 = tt * p.tok;
+            const int buf = acc & 1, parity = (acc >> 1) & 1;
+            if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
+            if (!ptx::mbar_wait_warp(&st.list_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
             ptx::tc_fence_after();
-            const uint32_t from = tmem + (uint32_t((warp & 3) * 32) << 16) + buf * p.tok;
-            // columns in use; the two warps of a lane quarter take chunks in turn
-            const int cols = min(p.tok, p.T - tt * p.tok);
-            for (int c = (warp >> 2) * kChunk; c < cols; c += 2 * kChunk) {
+            const List& l = st.list[buf];
+            // columns in use; the two halves of the epilogue take chunks in turn
+            const int cols = min(p.tok, p.T - t0), mixed1 = l.mixed1;
+            int e = l.mixed0;
+            for (int c = half; c * kChunk < cols; c += 2) {
                 float v[kChunk];
-                ptx::tmem_read<kChunk>(from + c, v);
+                ptx::tmem_read<kChunk>(tmem + buf * p.tok + c * kChunk, v);
                 ptx::tmem_landed<kChunk>(v);
+                for (; e < mixed1 && int(l.mixed[e].y & 0xff) <= (c | 1); ++e) {  // this chunk's and its neighbour's, in turn
+                    if (int(l.mixed[e].y & 0xff) != c) continue;
+                    const int slot = slot_it % p.slots;
+                    if (!ptx::mbar_wait_warp(&st.slot_full[half][slot], (slot_it / p.slots) & 1, &st.abort_flag, kWaitLimit)) return;
+                    ptx::tc_fence_after();
+                    float d[kChunk];
+                    ptx::tmem_read<kChunk>(tmem + 2 * p.tok + (half * p.slots + slot) * kChunk, d);
+                    ptx::tmem_landed<kChunk>(d);
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(&st.slot_empty[half][slot]);
+                    ++slot_it;
+                    const uint32_t rows = l.mixed[e].y >> 16;
+                    if constexpr (kHalf) {
+                        const float mine = (rows >> (lane & 15)) & 1u ? p.z_scale[t0 + c * kChunk + (lane & 15)] : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) {
+                            const float s = __shfl_sync(0xffffffffu, mine, j);
+                            if ((rows >> j) & 1u) v[j] = fmaf(d[j], s, v[j]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j)
+                            if ((rows >> j) & 1u) v[j] += d[j];
+                    }
+                }
                 if (q.part < 0) {
-                    store(v, tt, c, n, adapter == kMixed);
+                    store(v, t0 + c * kChunk, n);
                 } else {
-                    float* to = p.part + (size_t(q.part) * p.tok + c) * kRows + row;
+                    float* to = p.part + (size_t(q.part) * p.tok + c * kChunk) * kRows + row;
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) to[j * kRows] = v[j];
                 }
             }
             ptx::tc_fence_before();
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf]);
+            if (lane == 0) {
+                ptx::mbar_arrive(&st.tmem_empty[buf]);
+                ptx::mbar_arrive(&st.list_empty[buf]);
+            }
             if (q.part < 0) continue;
-            const int local = q.tile - p.whole, units = (p.tiles - p.whole) * p.kbs;
-            const int first = streamk::share_of(local * p.kbs, p.shares, units), last = streamk::share_of((local + 1) * p.kbs - 1, p.shares, units);
             __threadfence();
+            const int local = q.tile - p.whole, first = int(blockIdx.x) - q.index, last = first + q.of - 1;
             if (!meet()) return;
-            if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(&p.counters[local], 1) == last - first;
+            if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(&p.counters[local], 1) == q.of - 1;
             if (!meet()) return;
             if (*const_cast<volatile int*>(&st.last_part) == 0) continue;
             __threadfence();
-            for (int c = (warp >> 2) * kChunk; c < cols; c += 2 * kChunk) {
+            for (int c = half; c * kChunk < cols; c += 2) {
                 float v[kChunk];
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
                 for (int o = first; o <= last; ++o) {
-                    const int slot = 2 * o + (local == streamk::first_unit(o, p.shares, units) / p.kbs ? 0 : 1);
-                    const float* part = p.part + (size_t(slot) * p.tok + c) * kRows + row;
+                    const int slot = 2 * o + (local == streamk::first_unit(o, p.shares, pieces.units) / p.kbs ? 0 : 1);
+                    const float* part = p.part + (size_t(slot) * p.tok + c * kChunk) * kRows + row;
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) v[j] += streamk::ld_partial(part + j * kRows);
                 }
-                store(v, tt, c, n, adapter == kMixed);
+                store(v, t0 + c * kChunk, n);
             }
         }
     }
@@ -457,7 +495,6 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     Tail& st = *reinterpret_cast<Tail*>(ring + kRingBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int stage = kABytes + p.tok * kKBytes;
-    const uint32_t tmem_cols = uint32_t(2 * p.tok);
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
             ptx::mbar_init(&st.full[i], 1);
@@ -466,13 +503,19 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&st.tmem_full[i], 1);
             ptx::mbar_init(&st.tmem_empty[i], 8);
+            ptx::mbar_init(&st.list_full[i], 1);
+            ptx::mbar_init(&st.list_empty[i], 10);  // TMA thread, MMA thread, epilogue warps
+        }
+        for (int i = 0; i < 2 * kMaxSlots; ++i) {
+            ptx::mbar_init(&st.slot_full[0][i], 1);
+            ptx::mbar_init(&st.slot_empty[0][i], 4);
         }
         ptx::mbar_init(&st.meet, 8);
         st.abort_flag = 0;
         ptx::fence_barrier_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc(&st.tmem_base, tmem_cols);
+        ptx::tmem_alloc(&st.tmem_base, kTmemCols);
         ptx::tmem_relinquish();
     }
     ptx::tc_fence_before();
@@ -486,80 +529,108 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             Piece q;
             int it = 0;
             bool ok = true, waited = false;
-            auto slot_free = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
-            while (ok && pieces.next(&q)) {
-                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows;
+            auto next_stage = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
+            for (int n = 0; ok && pieces.next(&q); ++n) {
+                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows, t0 = tt * p.tok;
                 for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
-                    if (!(ok = slot_free())) break;
+                    if (!(ok = next_stage())) break;
                     const int s = it % p.stages;
                     ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
                     ptx::tma_load_2d(ring + s * stage, &map_w, kb * kKElems, n0, &st.full[s]);
-                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_x, kb * kKElems, tt * p.tok, &st.full[s]);
+                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_x, kb * kKElems, t0, &st.full[s]);
                 }
-                if (!ok || !p.by_mma || q.kb1 < p.kbs) continue;
-                if (!waited) pdl_wait();  // shrink
-                waited = true;
-                const int adapter = tile_adapter(p, tt);
-                if (adapter < 0) continue;
-                for (int r0 = 0; r0 < p.R; r0 += kKElems, ++it) {
-                    if (!(ok = slot_free())) break;
-                    const int s = it % p.stages;
-                    ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
-                    ptx::tma_load_3d<false>(ring + s * stage, &map_b, r0, n0, adapter, ptx::smem_u32(&st.full[s]));
-                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_z, r0, tt * p.tok, &st.full[s]);
-                }
+                if (!ok || !(ok = ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+                const List& l = st.list[n & 1];
+                auto load = [&](uint2 e, int chunks) {
+                    if (!waited) pdl_wait();  // shrink: z
+                    waited = true;
+                    const int c = int(e.y & 0xff);
+                    for (int r0 = 0; r0 < p.R; r0 += kKElems, ++it) {
+                        if (!next_stage()) return false;
+                        const int s = it % p.stages;
+                        ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(kABytes + chunks * kChunk * kKBytes));
+                        ptx::tma_load_3d<false>(ring + s * stage, &map_b, r0, n0, int(e.x), ptx::smem_u32(&st.full[s]));
+                        for (int i = 0; i < chunks; ++i)
+                            ptx::tma_load_2d(ring + s * stage + kABytes + i * kChunk * kKBytes, &map_z, r0, t0 + (c + i) * kChunk, &st.full[s]);
+                    }
+                    return true;
+                };
+                for (int e = l.direct0; ok && e < l.direct1; ++e) ok = load(l.direct[e], int(l.direct[e].y >> 8));
+                for (int e = l.mixed0; ok && e < l.mixed1; ++e) ok = load(l.mixed[e], 1);
+                ptx::mbar_arrive(&st.list_empty[n & 1]);
             }
             if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
-                const long long t0 = clock64();
+                const long long begin = clock64();
                 for (int i = max(0, it - p.stages); i < it; ++i)
-                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - t0 < kWaitLimit) {}
+                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - begin < kWaitLimit) {}
             }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (ptx::elect_one()) {
-            const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kRows, uint32_t(p.tok));
             Pieces pieces(p);
             Piece q;
-            int it = 0;
-            bool ok = true, waited = false;
-            for (int acc = 0; ok && pieces.next(&q); ++acc) {
-                const uint32_t d = tmem + (acc & 1) * p.tok;
-                if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+            int it = 0, slot_it[2] = {0, 0};
+            bool ok = true;
+            // one stage into the accumulator at `d`, `cols` columns of the second operand
+            auto block = [&](uint32_t d, int cols, int steps, bool more) {
+                const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kRows, uint32_t(cols));
+                const int s = it % p.stages;
+                if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit)) return false;
                 ptx::tc_fence_after();
-                auto block = [&](int steps, bool more) {
-                    const int s = it % p.stages;
-                    if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit)) return false;
-                    ptx::tc_fence_after();
-                    const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
-                    const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kABytes));
+                const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
+                const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kABytes));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (k < steps) ptx::umma<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
-                    ptx::umma_commit(&st.empty[s]);
-                    ++it;
-                    return true;
-                };
-                for (int kb = q.kb0; ok && kb < q.kb1; ++kb) ok = block(4, kb > q.kb0);
-                if (ok && p.by_mma && q.kb1 == p.kbs) {
-                    if (!waited) pdl_wait();
-                    waited = true;
-                    if (tile_adapter(p, q.tile / p.n_tiles) >= 0)
-                        for (int r0 = 0; ok && r0 < p.R; r0 += kKElems) ok = block(min(4, (p.R - r0 + 15) / 16), true);
+                for (int k = 0; k < 4; ++k)
+                    if (k < steps) ptx::umma<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
+                ptx::umma_commit(&st.empty[s]);
+                ++it;
+                return true;
+            };
+            for (int n = 0; ok && pieces.next(&q); ++n) {
+                const uint32_t d = tmem + (n & 1) * p.tok;
+                if (!ptx::mbar_wait(&st.tmem_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+                ptx::tc_fence_after();
+                for (int kb = q.kb0; ok && kb < q.kb1; ++kb) ok = block(d, p.tok, 4, kb > q.kb0);
+                if (!ok || !(ok = ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+                const List& l = st.list[n & 1];
+                for (int e = l.direct0; ok && e < l.direct1; ++e)
+                    for (int r0 = 0; ok && r0 < p.R; r0 += kKElems)
+                        ok = block(d + (l.direct[e].y & 0xff) * kChunk, int(l.direct[e].y >> 8) * kChunk, min(4, (p.R - r0 + 15) / 16), true);
+                if (!ok) break;
+                ptx::umma_commit(&st.tmem_full[n & 1]);
+                for (int e = l.mixed0; ok && e < l.mixed1; ++e) {
+                    const bool odd = (l.mixed[e].y & 1u) != 0;  // the half of the epilogue that takes the chunk
+                    const int h = odd ? 1 : 0, at = odd ? slot_it[1]++ : slot_it[0]++, slot = at % p.slots;
+                    if (!(ok = ptx::mbar_wait(&st.slot_empty[h][slot], ((at / p.slots) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+                    ptx::tc_fence_after();
+                    for (int r0 = 0; ok && r0 < p.R; r0 += kKElems)
+                        ok = block(tmem + 2 * p.tok + (h * p.slots + slot) * kChunk, kChunk, min(4, (p.R - r0 + 15) / 16), r0 > 0);
+                    if (ok) ptx::umma_commit(&st.slot_full[h][slot]);
                 }
-                if (ok) ptx::umma_commit(&st.tmem_full[acc & 1]);
+                ptx::mbar_arrive(&st.list_empty[n & 1]);
             }
         }
         __syncwarp();
+    } else if (warp == 2) {
+        pdl_wait();  // shrink: z_scale
+        Pieces pieces(p);
+        Piece q;
+        for (int n = 0; pieces.next(&q); ++n) {
+            if (!ptx::mbar_wait_warp(&st.list_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+            make_list<kHalf>(p, st.list[n & 1], q.tile / p.n_tiles * p.tok, q, lane);
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.list_full[n & 1]);
+        }
     } else if (warp >= 4) {
-        Epilogue<kHalf> ep{p, st, tmem, warp - 4, lane, (warp & 3) * 32 + lane};
+        Epilogue<kHalf> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane};
         ep.run();
     }
     __syncthreads();
     if (threadIdx.x == 0 && st.abort_flag != 0) *p.status = kStatusProject;
     if (warp == 1) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem, tmem_cols);
+        ptx::tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -582,17 +653,19 @@ static int make_map_2d(CUtensorMap* map, const void* base, bool half, int64_t ro
 }
 
 struct Layout {
-    size_t counters, info, z, z16, part, total;
+    size_t counters, z, z_scale, part, total;
 };
 static Layout plan(Params* p, int T, int N, int K, int R) {
+    T = T > 0 ? T : 1;  // an empty batch is asked about like a row
     p->T = T, p->N = N, p->K = K, p->R = R;
-    p->tok = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : kMaxTok;
+    // rows spread evenly over the tiles they need
+    p->tok = (ceil_div(T, ceil_div(T, kMaxTok)) + kChunk - 1) / kChunk * kChunk;
     const int stage = kABytes + p->tok * kKBytes;
     p->stages = kRingBytes / stage < kMaxStages ? kRingBytes / stage : kMaxStages;
+    p->slots = (kTmemCols - 2 * p->tok) / (2 * kChunk) < kMaxSlots ? (kTmemCols - 2 * p->tok) / (2 * kChunk) : kMaxSlots;
     p->n_tiles = ceil_div(N, kRows);
     p->tiles = p->n_tiles * ceil_div(T, p->tok);
     p->kbs = ceil_div(K, kKElems);
-    p->by_mma = T > 128 ? 1 : 0;
     const int sms = sm_count(), left = p->tiles % sms;
     // a last round that is three quarters full is left as it is
     p->whole = left * 4 >= sms * 3 ? p->tiles : p->tiles - left;
@@ -606,11 +679,11 @@ static Layout plan(Params* p, int T, int N, int K, int R) {
         return at;
     };
     // for the most that a call of fewer rows splits, so that a workspace for the longest batch serves all
+    const int most = T < kMaxTok ? (T + kChunk - 1) / kChunk * kChunk : kMaxTok;
     L.counters = add(size_t(sms) * sizeof(int));
-    L.info = add(size_t(ceil_div(T, kShrinkTok)) * sizeof(int));
-    L.z = add(size_t(T) * R * sizeof(float));
-    L.z16 = add(size_t(T) * R * 2);
-    L.part = add(size_t(sms) * 2 * p->tok * kRows * sizeof(float));
+    L.z = add(size_t(T) * R * 2);
+    L.z_scale = add(size_t(T) * sizeof(float));
+    L.part = add(size_t(sms) * 2 * most * kRows * sizeof(float));
     L.total = off;
     return L;
 }
@@ -679,8 +752,8 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
 
     lora::ShrinkParams sp{};
     sp.ids = ids, sp.scale = scale;
-    sp.z = reinterpret_cast<float*>(ws + Y.z), sp.z16 = reinterpret_cast<uint16_t*>(ws + Y.z16);
-    sp.info = reinterpret_cast<int*>(ws + Y.info), sp.counters = reinterpret_cast<int*>(ws + Y.counters);
+    sp.z = reinterpret_cast<uint16_t*>(ws + Y.z), sp.z_scale = reinterpret_cast<float*>(ws + Y.z_scale);
+    sp.counters = reinterpret_cast<int*>(ws + Y.counters);
     sp.n_counters = p.tiles - p.whole;
     sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status;
     // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached.
@@ -691,17 +764,15 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     const int fit = room / (tiles * split);
     sp.slots = fit < 1 ? 1 : fit < most ? fit : most;
 
-    CUtensorMap xs, a, xp, wm, zm{}, bm{};
+    CUtensorMap xs, a, xp, wm, zm, bm;
     DQ_RC(lora::make_map_2d(&xs, x, half, T, K, ldx, lora::kShrinkTok));
     DQ_RC(lora::make_map_2d(&a, lora_a, half, int64_t(L) * R, K, K, R));
     DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, p.tok));
     DQ_RC(lora::make_map_2d(&wm, w, half, N, K, K, lora::kRows));
-    if (p.by_mma) {
-        DQ_RC(lora::make_map_2d(&zm, sp.z16, half, T, R, R, p.tok));
-        const cuuint64_t dim[3] = {cuuint64_t(R), cuuint64_t(N), cuuint64_t(L)}, stride[2] = {cuuint64_t(R) * 2, cuuint64_t(N) * R * 2};
-        const cuuint32_t box[3] = {lora::kKElems, lora::kRows, 1};
-        DQ_RC(lora::make_map(&bm, lora_b, half, 3, dim, stride, box));
-    }
+    DQ_RC(lora::make_map_2d(&zm, sp.z, half, T, R, R, lora::kChunk));
+    const cuuint64_t dim[3] = {cuuint64_t(R), cuuint64_t(N), cuuint64_t(L)}, stride[2] = {cuuint64_t(R) * 2, cuuint64_t(N) * R * 2};
+    const cuuint32_t box[3] = {lora::kKElems, lora::kRows, 1};
+    DQ_RC(lora::make_map(&bm, lora_b, half, 3, dim, stride, box));
     {
         const size_t smem = lora::shrink_smem(R);
         DQ_RC(lora::opt_in(lora::lora_shrink_kernel, 0, smem));
@@ -721,7 +792,7 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
         cfg.numAttrs = 2;
         DQ_CUDA(cudaLaunchKernelEx(&cfg, lora::lora_shrink_kernel, xs, a, sp));
     }
-    p.ids = ids, p.z = sp.z, p.info = sp.info, p.lora_b = static_cast<const uint16_t*>(lora_b), p.bias = bias;
+    p.ids = ids, p.z_scale = half ? sp.z_scale : nullptr, p.bias = bias;
     p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
     p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
     const int sms = sm_count();

@@ -497,9 +497,8 @@ int dqmoe_grouped_gemm_nvfp4(const void* a, const uint8_t* a_sf, const float* a_
  * >= N elements apart, all of `type` (DQMOE_DT_BF16 or DQMOE_DT_HALF); ids [T] int32, scale [L] fp32 or NULL (1), bias [N] fp32 or NULL.
  * A row whose id is outside [0, L) has no adapter. Adapters of a lower rank are padded with zeros to R, a multiple of 8 up to 128; K is a
  * multiple of 8; x, w, lora_a, lora_b are aligned to 16 bytes. The ids may come in any order; rows of one request that stand together
- * are faster from 129 rows on. Sums are fp32, the result is rounded once; x A^T too is rounded to the operands' type where 256 rows
- * (counted from the first) have one adapter, and held in fp32 elsewhere. No row's result depends on another row's adapter. Any T from 0
- * on. dqmoe_device_status gives 311 or 312 where a wait ran out. A call has its workspace for itself until it is over. No counterpart in
+ * are faster. Sums are fp32, scale[a] * (x A_a^T) and the result are rounded to the operands' type (fp16: with a power of two per row
+ * where the former leaves its range). No row's result depends on another row's adapter. Any T from 0 on. dqmoe_device_status gives 311 or 312 where a wait ran out. A call has its workspace for itself until it is over. No counterpart in
  * the reference.
  */
 size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R);

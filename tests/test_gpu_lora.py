@@ -64,7 +64,8 @@ SHAPES = [  # T, N, K, L, R, ids
     (33, 2048, 1024, 3, 64, "random"), (64, 6144, 4096, 64, 16, 1), (65, 200, 2880, 9, 40, 7), (100, 8, 8, 2, 8, "random"),
     (128, 1536, 512, 40, 128, 1), (129, 1536, 512, 40, 128, 1), (200, 640, 1032, 4, 72, 200), (256, 384, 256, 2, 16, 256), (257, 1, 256, 2, 16, 256),
     (333, 2880, 2880, 32, 64, 9), (512, 256, 4096, 7, 32, 100), (1000, 512, 512, 3, 8, "none"), (1023, 896, 640, 6, 96, 300), (2048, 4096, 512, 5, 16, 700),
-    (4099, 1152, 192, 33, 48, 1000), (700, 3000, 64, 64, 8, "random"),
+    (4099, 1152, 192, 33, 48, 1000), (700, 3000, 64, 64, 8, "random"), (224, 384, 256, 2, 16, 100), (225, 384, 200, 5, 128, 3),
+    (481, 256, 128, 8, 72, 16), (960, 128, 64, 3, 64, 17),
 ]
 
 
@@ -113,9 +114,10 @@ def test_rows_do_not_see_other_adapters(T, run, dtype):
     assert torch.equal(again[rest], clean[rest]) and not again[2].isfinite().any()
 
 
-def test_inner_values_beyond_fp16():
+@pytest.mark.parametrize("run", [512, 3])
+def test_inner_values_beyond_fp16(run):
     """x A^T may pass fp16's range where the result does not."""
-    a = make(9, 512, 256, 512, 2, 8, "fp16", 512)
+    a = make(9, 512, 256, 512, 2, 8, "fp16", run)
     a["lora_a"].mul_(3e4)
     a["lora_b"].mul_(1e-4)
     a["scale"].fill_(4.0)
