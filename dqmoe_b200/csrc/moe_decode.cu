@@ -1,6 +1,6 @@
 // The whole MoE layer for up to 32 tokens in two launches: x [T, H] and the router's weights in, out [T, H] out.
 //
-//   route    logits = x Wr^T in fp32 (clusters of eight blocks, a slice of H each), x laid out as the tensor core's second operand
+//   route    logits = x Wr^T in fp32 (clusters of eight blocks, slices of H), x laid out as the tensor core's second operand
 //   experts  top-k of every token (each block for itself), the experts that are hit, fc1 + SwiGLU, fc2, sum over the experts
 //
 // What bounds it: the weights of the experts hit, once from HBM. Everything else is arranged around that stream:
@@ -12,11 +12,18 @@
 //     four more, so the split is exact down to 2^-13 of the group's largest value and off by at most 2^-21 of that below it. hi and lo
 //     are separate columns of the same MMA: N = 2 T, no conversion of weights, which go from memory to the tensor core untouched. The
 //     intermediate (fp32) is split the same way, within 2^-9 of each value (bf16's half step is 2^-8); with bf16 weights into two bf16.
-//   - Each phase is a list of 32 KiB units (fc1: 128 gate and 128 value rows x 128 bytes; fc2: 128 rows x 256 bytes), cut into one
-//     equal share per SM, whatever the tiles (streamk.cuh).
-//   - fc2's weights are fetched into the ring while the last parts of fc1 are still being summed; only the second operand waits.
-// Shares are claimed from a counter, fc1's before fc2's: a block waits for parts of fc1 only when each of them belongs to a block that
-// is running, so the wait ends also where not all blocks fit the GPU at once (another stream's kernels, several of these among them).
+//   - Work comes in units of 32 KiB of weights (fc1: 128 gate and 128 value rows x 128 bytes; fc2: 128 rows x 256 bytes) and pieces of
+//     several units, which the blocks claim one after the other from a counter: fc1's pieces expert by expert, then fc2's in the same order
+//     of experts, ever smaller ones towards the end. fc2's first pieces need only experts that were finished long ago, so the stream does
+//     not pause between the two, and no SM waits for a slower one.
+//   - What takes trips through L2 - sums over the parts of a tile, the activation, the hand-over to fc2 - is done by four warps of
+//     their own beside the stream; the second operand has a thread of its own that may wait for fc1 while weights are still fetched.
+// A block waits for an expert's fc1 only when all of fc1 has been claimed by blocks that are running, and those finish it whatever
+// happens: so the wait ends also where not all blocks fit the GPU at once (other streams' kernels, several of these among them).
+// Sums are added in a fixed order whoever adds them: results do not depend on which block took which piece.
+//
+// With one equal share of the units per SM, static, the sums and the activation on the warps that drain the accumulators, and fc2 behind all of
+// fc1: small_block_5 40.7 us
 //
 // No counterpart in the reference, whose runner (csrc/moe_kernels.h:770-892) takes routed rows and five launches.
 #include <mutex>
@@ -33,15 +40,18 @@ namespace moe_decode {
 constexpr int kMaxTokens = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 32;
-constexpr int kThreads = 256;                 // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue; all of them choose the experts
+constexpr int kThreads = 384;                 // warp 0 weights, warp 1 MMA, warp 2 tokens, warps 4..7 drain, warps 8..11 finish; all choose the experts
 constexpr int kRows = 128;                    // weight rows of an MMA
 constexpr int kKBytes = 128;                  // bytes of a K block: one swizzle row
 constexpr int kTileBytes = kRows * kKBytes;   // 16 KiB
 constexpr int kABytes = 2 * kTileBytes;       // a unit's weights
 constexpr int kRingBytes = 205 * 1024;
+constexpr int kMaxParts = 40;                 // of an fc2 tile
+constexpr int kGroup = 7;                     // parts that are added to one sum first
+constexpr int kGroups = (kMaxParts + kGroup - 1) / kGroup;
 constexpr int kMaxStages = 6;
 constexpr int kScaleBytes = 1024;             // room behind a stage's second operand for its scales
-constexpr int kClaims = 4;
+constexpr int kClaims = 4, kJobs = 4;
 constexpr long long kWaitLimit = 1000000000LL;  // clock cycles before a wait gives up (~0.5 s)
 constexpr int kStatusRing = 301, kStatusPhase = 302;
 constexpr int kSplit = 8;                     // blocks of a route cluster: slices of H
@@ -64,15 +74,18 @@ struct Params {
     int scoring, mode;
     int kb1, pairs2;          // K blocks of fc1; pairs of K blocks of fc2
     int tiles1, tiles2;       // tiles of 128 rows of I and H
-    int shares;
+    int blocks;
+    int max_hit;              // experts hit at most
     int n_counters;
     size_t rec1, rec2;        // bytes of a unit's second operand with its scales
-    int* counters;            // claims of fc1, of fc2, finished tiles of fc1, unused, then the parts seen of each tile
+    int* counters;            // claims; 3 unused; finished fc1 tiles of each expert; parts seen of each fc1 tile, of each group of parts
+                              // of an fc2 tile, groups seen of each fc2 tile
     float* logits;            // [T, E]
     uint8_t* xq;              // [kb1] records: [fc1_cols][128 B] swizzled, scales [token_rows]
     uint8_t* aq;              // [experts hit][pairs2] records: two of [fc2_cols][128 B] swizzled, scales [2][token_rows]
-    float* part1;             // [shares][2][gate, value][token][128]
-    float* part2;             // [shares][2][token][128]
+    float* part1;             // [piece, or kJobs x block][gate, value][token][128]
+    float* part2;             // [tile][part][token][128]
+    float* group2;            // [tile][group][token][128]
     int* status;
 };
 
@@ -100,47 +113,71 @@ __device__ __forceinline__ void split_e4m3x2(float x0, float x1, uint32_t* hi, u
 
 // ---------------------------------------------------------------- route
 
-template <bool kF32>
-__device__ __forceinline__ void load_router8(const void* w, size_t at, float (&f)[8]) {
-    if constexpr (kF32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at);
-        const float4 a = p[0], b = p[1];
-        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(w) + at);
-        f[0] = bf16_lo(v.x), f[1] = bf16_hi(v.x), f[2] = bf16_lo(v.y), f[3] = bf16_hi(v.y);
-        f[4] = bf16_lo(v.z), f[5] = bf16_hi(v.z), f[6] = bf16_lo(v.w), f[7] = bf16_hi(v.w);
+// Three bf16 whose sum is the fp32 value to 2^-24 of it, two values at a time.
+__device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        w[i] = pack_bf16x2(a, b);
+        a -= bf16_lo(w[i]);
+        b -= bf16_hi(w[i]);
     }
 }
-
-// One warp per expert and slice; the eight slices of a cluster are added in their order through distributed shared memory.
-template <bool kF32, int kTp>
-__device__ __forceinline__ void partial_logits(const Params& p, int e, int rank, float* part /*[T]*/, int lane) {
-    const int slice = (p.H + kSplit * 8 - 1) / (kSplit * 8) * 8;
-    const int k0 = rank * slice, k1 = min(p.H, k0 + slice);
-    float acc[kTp];
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// This warp's share of the logits of all tokens and eight experts, over chunks of 32 values of H. A thread loads 16 bytes of a row, eight values
+// that follow one another; which of them an MMA takes for its k is the same for x and the weights, and a sum does not mind.
+// Each value of x and each weight is read once per cluster. (With a warp per expert and fp32 FMAs each warp read all of x, and the kernel
+// took 10.7 us for 32 tokens of H 2048 and 128 experts.)
+template <bool kF32, int kM>
+__device__ __forceinline__ void partial_logits(const Params& p, int e0, int first, int step, float* part /*[T][8]*/, int lane) {
+    const int g = lane >> 2, kk = (lane & 3) * 8;
+    float acc[kM][4] = {};
+#pragma unroll 4
+    for (int k0 = first * 32; k0 < p.H; k0 += step * 32) {
+        const int k = k0 + kk;
+        const bool in = k < p.H;
+        uint4 x[kM][2];
 #pragma unroll
-    for (int t = 0; t < kTp; ++t) acc[t] = 0.0f;
-    for (int k = k0 + lane * 8; k < k1; k += 256) {
-        float w[8];
-        load_router8<kF32>(p.w_router, size_t(e) * p.H + k, w);
+        for (int m = 0; m < kM; ++m)
 #pragma unroll
-        for (int t = 0; t < kTp; ++t)
-            if (t < p.T) {
-                const uint4 v = *reinterpret_cast<const uint4*>(p.x + size_t(t) * p.H + k);
-                float a = acc[t];
-                a = fmaf(bf16_lo(v.x), w[0], a), a = fmaf(bf16_hi(v.x), w[1], a);
-                a = fmaf(bf16_lo(v.y), w[2], a), a = fmaf(bf16_hi(v.y), w[3], a);
-                a = fmaf(bf16_lo(v.z), w[4], a), a = fmaf(bf16_hi(v.z), w[5], a);
-                a = fmaf(bf16_lo(v.w), w[6], a), a = fmaf(bf16_hi(v.w), w[7], a);
-                acc[t] = a;
+            for (int h = 0; h < 2; ++h) {
+                const int t = m * 16 + h * 8 + g;
+                x[m][h] = in && t < p.T ? *reinterpret_cast<const uint4*>(p.x + size_t(t) * p.H + k) : make_uint4(0, 0, 0, 0);
+            }
+        uint32_t w[kF32 ? 3 : 1][4] = {};
+        if (in && e0 + g < p.E) {
+            const size_t at = size_t(e0 + g) * p.H + k;
+            if constexpr (kF32) {
+                const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p.w_router) + at);
+                const float4 a = q[0], b = q[1];
+                const float f[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t s3[3];
+                    split3(f[2 * i], f[2 * i + 1], s3);
+                    w[0][i] = s3[0], w[1][i] = s3[1], w[2][i] = s3[2];
+                }
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.w_router) + at);
+                w[0][0] = v.x, w[0][1] = v.y, w[0][2] = v.z, w[0][3] = v.w;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int i = (kF32 ? 2 : 0); i >= 0; --i) {
+                mma_16x8x16(acc[m], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, w[i][0], w[i][1]);
+                mma_16x8x16(acc[m], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, w[i][2], w[i][3]);
             }
     }
 #pragma unroll
-    for (int t = 0; t < kTp; ++t)
-        if (t < p.T) {
-            const float s = warp_sum(acc[t]);
-            if (lane == 0) part[t] = s;
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = m * 16 + (i >> 1) * 8 + g;
+            if (t < p.T) part[t * 8 + (lane & 3) * 2 + (i & 1)] = acc[m][i];
         }
 }
 
@@ -171,21 +208,28 @@ __device__ __forceinline__ void lay_out_x(const Params& p, int kb, int t, int tp
 template <bool kF32, bool kFp8>
 __global__ void __launch_bounds__(kRouteThreads) moe_decode_route_kernel(const __grid_constant__ Params p) {
     pdl_enter();
-    __shared__ float s_part[kRouteThreads / 32][kMaxTokens];
+    __shared__ float s_part[kRouteThreads / 32][kMaxTokens * 8], s_sum[kMaxTokens * 8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = int(ptx::cluster_ctarank());
-    const int chunk = blockIdx.x / kSplit, e = chunk * 8 + warp;
+    const int chunk = blockIdx.x / kSplit;
     const int tp = token_rows(p.T);
     const bool working = chunk * 8 < p.E;
-    if (e < p.E) {
-        if (tp == 8) partial_logits<kF32, 8>(p, e, rank, s_part[warp], lane);
-        else if (tp == 16) partial_logits<kF32, 16>(p, e, rank, s_part[warp], lane);
-        else partial_logits<kF32, 32>(p, e, rank, s_part[warp], lane);
+    if (working) {
+        const int first = rank * (kRouteThreads / 32) + warp, step = kSplit * (kRouteThreads / 32);
+        if (tp <= 16) partial_logits<kF32, 1>(p, chunk * 8, first, step, s_part[warp], lane);
+        else partial_logits<kF32, 2>(p, chunk * 8, first, step, s_part[warp], lane);
     }
     for (int i = blockIdx.x * kRouteThreads + threadIdx.x; i < p.n_counters; i += gridDim.x * kRouteThreads) p.counters[i] = 0;
     const int warps = gridDim.x * (kRouteThreads / 32);
     for (int u = blockIdx.x * (kRouteThreads / 32) + warp; u < p.kb1 * p.T; u += warps) lay_out_x<kFp8>(p, u / p.T, u % p.T, tp, lane);
     if (!working) return;  // whole clusters
+    __syncthreads();
+    if (threadIdx.x < p.T * 8) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRouteThreads / 32; ++w) sum += s_part[w][threadIdx.x];
+        s_sum[threadIdx.x] = sum;
+    }
     __syncthreads();
     ptx::cluster_sync();
     const int mine = chunk * 8 + rank;  // the expert whose slices this block adds
@@ -194,7 +238,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_decode_route_kernel(const _
 #pragma unroll
         for (int r = 0; r < kSplit; ++r) {
             float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(&s_part[rank][threadIdx.x], r)) : "memory");
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(ptx::map_to_cta(&s_sum[threadIdx.x * 8 + rank], r)) : "memory");
             sum += v;
         }
         p.logits[size_t(threadIdx.x) * p.E + mine] = sum;
@@ -209,13 +253,17 @@ struct alignas(16) Tail {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t tmem_full[4], tmem_empty[4];
     uint64_t claim_full[kClaims], claim_empty[kClaims];
-    uint64_t meet;                             // the four epilogue warps
-    int claim[kClaims];
+    uint64_t job_full[kJobs], job_empty[kJobs];        // pieces from the draining warps to the finishing ones
+    uint64_t meet;                             // the finishing warps
+    int claim[kClaims], job[kJobs];
     uint32_t tmem_base;
     int abort_flag;
     int n_hit;
+    int split1, pieces1;                       // parts of an fc1 tile; pieces of fc1
+    int parts2, pieces2;                       // parts of an fc2 tile; pieces of both
+    int bound2[kMaxParts + 1];                 // first unit of each part of an fc2 tile
     uint32_t bad_tokens;                       // tokens without a number among their weights
-    int last_part;
+    int last;
     uint32_t amax[4][kMaxTokens];
     int topk_index[kMaxTokens][kMaxTopk];
     float topk_weight[kMaxTokens][kMaxTopk];
@@ -226,36 +274,64 @@ struct alignas(16) Tail {
 constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 
-struct Share {
-    int phase, lo, hi, index;  // units [lo, hi) of phase 0 (fc1) or 1 (fc2); phase 2 = no more
-};
-__device__ __forceinline__ int phase_units(const Params& p, const Tail& st, int phase) {
-    return st.n_hit * (phase == 0 ? p.tiles1 * p.kb1 : p.tiles2 * p.pairs2);
+// Pieces of the work, from the experts that are hit. fc1: a tile in split1 equal parts, three pieces per block at least, of four units or
+// more. fc2: the units of a tile ([expert][pair of K blocks]) in parts, each half of what would be left for a block if all were
+// shared out evenly, so that the blocks end together however fast each is; not under two units unless there are few in all.
+__device__ __forceinline__ void plan_pieces(const Params& p, Tail& st) {
+    const int tiles1 = st.n_hit * p.tiles1;
+    st.split1 = max(1, min((3 * p.blocks + tiles1 - 1) / max(tiles1, 1), p.kb1 / 4));
+    st.pieces1 = tiles1 * st.split1;
+    const int units = st.n_hit * p.pairs2;
+    const float per_block = float(p.tiles2) / float(2 * p.blocks);  // of a unit of every tile, halved
+    const int least = max(1, min(4, int(float(units) * per_block)));
+    int q = 0, at = 0;
+    while (at < units) {
+        const int rest = units - at;
+        const int n = max(max(least, int(float(rest) * per_block)), int(__fdividef(float(rest), float(kMaxParts - q))) + 1);
+        st.bound2[q++] = at;
+        at += min(n, rest);
+    }
+    st.bound2[q] = units;
+    st.parts2 = q;
+    st.pieces2 = st.pieces1 + q * p.tiles2;
 }
-// none of them empty: the parts of a tile are those of all shares between its first unit's and its last one's
-__device__ __forceinline__ int phase_shares(const Params& p, int units) { return min(p.shares, units); }
-__device__ __forceinline__ Share share_at(const Params& p, const Tail& st, int code) {
-    Share s;
-    s.phase = code >> 28;
-    s.index = code & 0xfffffff;
-    const int units = phase_units(p, st, s.phase & 1);
-    s.lo = streamk::first_unit(s.index, phase_shares(p, units), units);
-    s.hi = streamk::first_unit(s.index + 1, phase_shares(p, units), units);
-    return s;
-}
-constexpr int kEnd = 2 << 28;
 
-// The next share, as the producer announces it to the other roles.
+struct Piece {
+    int phase;       // 0 fc1, 1 fc2, 2 no more, 3 a wait has run out
+    int tile, part;  // fc1: tile = expert's place * tiles1 + tile of I; fc2: tile of H
+    int lo, hi;      // units of the tile
+};
+__device__ __forceinline__ Piece piece_at(const Params& p, const Tail& st, int c) {
+    Piece q;
+    if (c >= st.pieces2) return Piece{2, 0, 0, 0, 0};
+    if (c < st.pieces1) {
+        q.phase = 0;
+        q.tile = c / st.split1;
+        q.part = c - q.tile * st.split1;
+        q.lo = q.part * p.kb1 / st.split1;
+        q.hi = (q.part + 1) * p.kb1 / st.split1;
+    } else {
+        q.phase = 1;
+        q.part = (c - st.pieces1) / p.tiles2;
+        q.tile = c - st.pieces1 - q.part * p.tiles2;
+        q.lo = st.bound2[q.part];
+        q.hi = st.bound2[q.part + 1];
+    }
+    return q;
+}
+
+// The next piece, as the weights' thread announces it to the other roles.
 template <bool kWarp>
-__device__ __forceinline__ int next_claim(Tail& st, int it, int lane) {
+__device__ __forceinline__ Piece next_piece(const Params& p, Tail& st, int it, int lane, int* code = nullptr) {
     const int slot = it % kClaims, parity = (it / kClaims) & 1;
     const bool ok = kWarp ? ptx::mbar_wait_warp(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit)
                           : ptx::mbar_wait(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit);
-    if (!ok) return kEnd;
-    const int code = *const_cast<volatile int*>(&st.claim[slot]);
+    if (!ok) return Piece{3, 0, 0, 0, 0};
+    const int c = *const_cast<volatile int*>(&st.claim[slot]);
     if constexpr (kWarp) __syncwarp();
     if (!kWarp || lane == 0) ptx::mbar_arrive(&st.claim_empty[slot]);
-    return code;
+    if (code != nullptr) *code = c;
+    return piece_at(p, st, c);
 }
 
 template <bool kFp8, int kTp>
@@ -264,102 +340,95 @@ struct Shape {
     static constexpr int kKElems = kFp8 ? kKBytes : kKBytes / 2;
     static constexpr int kStages = stages(kTp);
     static constexpr int kStage = stage_bytes(kTp);
-    // FP8: the accumulators of one unit per buffer, handed over unit by unit; bf16: those of one tile and expert
+    // FP8: the accumulators of one unit per buffer, handed over unit by unit; bf16: those of one piece and expert
     static constexpr int kBufCols = kFp8 ? 2 * kN1 : (2 * kN1 > kN2 ? 2 * kN1 : kN2);
     static constexpr int kBufs = kFp8 ? 4 : 2;
     static constexpr int kTmemCols = kBufs * kBufCols;  // 128 / 256 / 512 and 64 / 64 / 128
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM allocation");
+    static constexpr size_t kPart1 = size_t(2) * kTp * kRows, kPart2 = size_t(kTp) * kRows;  // floats
 };
 
+// A stage is filled by two threads; nobody may leave with copies in flight. Where all went well the other roles have waited for each.
+template <int kStages>
+__device__ __forceinline__ void drain_copies(Tail& st, int it) {
+    if (*const_cast<volatile int*>(&st.abort_flag) == 0) return;
+    const long long t0 = clock64();
+    for (int i = max(0, it - kStages); i < it; ++i)
+        while (!ptx::mbar_try_wait(&st.full[i % kStages], (i / kStages) & 1) && clock64() - t0 < kWaitLimit) {}
+}
+
 template <bool kFp8, int kTp>
-__device__ __forceinline__ void produce(const Params& p, const CUtensorMap& map_b, const CUtensorMap& map_b1, Tail& st, uint8_t* ring, int claim) {
+__device__ __forceinline__ void load_weights(const Params& p, const CUtensorMap& map_b, const CUtensorMap& map_b1, Tail& st, uint8_t* ring, int claim) {
     using S = Shape<kFp8, kTp>;
-    int it = 0;        // units whose weights were asked for
-    int pushed = 0;
-    bool ready = false;
+    int it = 0;
     bool ok = true;
-    auto stage_at = [&](int i) { return ring + (i % S::kStages) * S::kStage; };
-    auto load_weights = [&](const Share& s, int u, int i) {
-        const int slot = i % S::kStages;
-        if (!ptx::mbar_wait(&st.empty[slot], ((i / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
-        uint8_t* a = stage_at(i);
-        if (s.phase == 0) {
-            const int tile = u / p.kb1, kb = u - tile * p.kb1;
-            const int j = tile / p.tiles1, row = st.hit[j] * 2 * p.I + (tile - j * p.tiles1) * kRows;
-            ptx::mbar_arrive_expect_tx(&st.full[slot], kABytes + uint32_t(p.rec1));
-            ptx::tma_load_2d(a, &map_b, kb * S::kKElems, row, &st.full[slot]);
-            ptx::tma_load_2d(a + kTileBytes, &map_b, kb * S::kKElems, row + p.I, &st.full[slot]);
-        } else {
-            const int per_tile = st.n_hit * p.pairs2;
-            const int tile = u / per_tile, rest = u - tile * per_tile, j = rest / p.pairs2, pair = rest - j * p.pairs2;
-            const int row = st.hit[j] * p.H + tile * kRows;
-            // a last pair's second block may lie past I, where the copy writes zeros
-            ptx::mbar_arrive_expect_tx(&st.full[slot], kABytes + uint32_t(p.rec2));
-            ptx::tma_load_2d(a, &map_b1, pair * 2 * S::kKElems, row, &st.full[slot]);
-            ptx::tma_load_2d(a + kTileBytes, &map_b1, (pair * 2 + 1) * S::kKElems, row, &st.full[slot]);
-        }
-        return true;
-    };
-    auto load_tokens = [&](const Share& s, int u, int i) {
-        const int slot = i % S::kStages;
-        if (s.phase == 0) {
-            ptx::bulk_load(stage_at(i) + kABytes, p.xq + size_t(u % p.kb1) * p.rec1, uint32_t(p.rec1), &st.full[slot]);
-        } else {
-            const int rest = u % (st.n_hit * p.pairs2);  // [expert][pair]
-            ptx::bulk_load(stage_at(i) + kABytes, p.aq + size_t(rest) * p.rec2, uint32_t(p.rec2), &st.full[slot]);
-        }
-    };
-    auto push = [&](int code) {
-        const int slot = pushed % kClaims;
-        if (!ptx::mbar_wait(&st.claim_empty[slot], ((pushed / kClaims) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
-        *const_cast<volatile int*>(&st.claim[slot]) = code;
+    for (int n = 0; ok; ++n) {
+        const int slot = n % kClaims;
+        const int next = claim < st.pieces2 ? atomicAdd(&p.counters[0], 1) : claim;  // known by the time it is needed
+        if (!(ok = ptx::mbar_wait(&st.claim_empty[slot], ((n / kClaims) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+        *const_cast<volatile int*>(&st.claim[slot]) = claim;
         ptx::mbar_arrive(&st.claim_full[slot]);
-        ++pushed;
-        return true;
-    };
-    for (int phase = 0; phase < 2 && ok; ++phase) {
-        if (phase == 1) claim = atomicAdd(&p.counters[1], 1);
-        const int shares = phase_shares(p, phase_units(p, st, phase));
-        for (; ok && claim < shares; claim = atomicAdd(&p.counters[phase], 1)) {
-            const int code = (phase << 28) | claim;
-            const Share s = share_at(p, st, code);
-            if (!push(code)) {
-                ok = false;
-                break;
+        const Piece q = piece_at(p, st, claim);
+        if (q.phase == 2) break;
+        for (int u = q.lo; u < q.hi; ++u, ++it) {
+            const int s = it % S::kStages;
+            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+            uint8_t* a = ring + s * S::kStage;
+            ptx::mbar_arrive_expect_tx(&st.full[s], kABytes);
+            if (q.phase == 0) {
+                const int j = q.tile / p.tiles1, row = st.hit[j] * 2 * p.I + (q.tile - j * p.tiles1) * kRows;
+                ptx::tma_load_2d(a, &map_b, u * S::kKElems, row, &st.full[s]);
+                ptx::tma_load_2d(a + kTileBytes, &map_b, u * S::kKElems, row + p.I, &st.full[s]);
+            } else {
+                const int j = u / p.pairs2, pair = u - j * p.pairs2, row = st.hit[j] * p.H + q.tile * kRows;
+                // a last pair's second block may lie past I, where the copy writes zeros
+                ptx::tma_load_2d(a, &map_b1, pair * 2 * S::kKElems, row, &st.full[s]);
+                ptx::tma_load_2d(a + kTileBytes, &map_b1, (pair * 2 + 1) * S::kKElems, row, &st.full[s]);
             }
-            int u = s.lo;
-            if (phase == 1 && !ready) {
-                // weights into every free stage first, then wait for fc1
-                const int first = it;
-                while (u < s.hi && it - first < S::kStages && (ok = load_weights(s, u, it))) ++u, ++it;
-                const int tiles = st.n_hit * p.tiles1;
+        }
+        claim = next;
+    }
+    drain_copies<S::kStages>(st, it);
+}
+
+template <bool kFp8, int kTp>
+__device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* ring) {
+    using S = Shape<kFp8, kTp>;
+    int it = 0, ready = -1;  // place of the expert whose fc1 was last seen finished
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+        const Piece q = next_piece<false>(p, st, n, 0);
+        if (q.phase >= 2) break;
+        for (int u = q.lo; u < q.hi; ++u, ++it) {
+            const int s = it % S::kStages;
+            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+            uint8_t* b = ring + s * S::kStage + kABytes;
+            if (q.phase == 0) {
+                ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(p.rec1));
+                ptx::bulk_load(b, p.xq + size_t(u) * p.rec1, uint32_t(p.rec1), &st.full[s]);
+                continue;
+            }
+            const int j = u / p.pairs2;
+            if (j != ready) {
                 const long long t0 = clock64();
-                while (ok && streamk::ld_acquire_gpu(&p.counters[2]) < tiles) {
+                while (streamk::ld_acquire_gpu(&p.counters[4 + j]) < p.tiles1) {
                     if (*const_cast<volatile int*>(&st.abort_flag) != 0) ok = false;
-                    else if (clock64() - t0 > kWaitLimit) {
+                    if (clock64() - t0 > kWaitLimit) {
                         *const_cast<volatile int*>(&st.abort_flag) = 1;
                         *p.status = kStatusPhase;
                         ok = false;
                     }
+                    if (!ok) break;
                 }
-                // also where the wait gave up: the copies complete the stages that were announced, so that the block can be left
+                if (!ok) break;
                 asm volatile("fence.proxy.async;" ::: "memory");
-                for (int i = first; i < it; ++i) load_tokens(s, s.lo + i - first, i);
-                ready = true;
+                ready = j;
             }
-            for (; ok && u < s.hi; ++u, ++it) {
-                if (!(ok = load_weights(s, u, it))) break;
-                load_tokens(s, u, it);
-            }
+            ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(p.rec2));
+            ptx::bulk_load(b, p.aq + size_t(u) * p.rec2, uint32_t(p.rec2), &st.full[s]);  // [expert][pair], as the units
         }
     }
-    if (ok) push(kEnd);
-    // Nobody may leave with copies in flight. Where all went well the other roles have waited for each of them.
-    if (*const_cast<volatile int*>(&st.abort_flag) != 0) {
-        const long long t0 = clock64();
-        for (int i = max(0, it - S::kStages); i < it; ++i)
-            while (!ptx::mbar_try_wait(&st.full[i % S::kStages], (i / S::kStages) & 1) && clock64() - t0 < kWaitLimit) {}
-    }
+    drain_copies<S::kStages>(st, it);
 }
 
 template <bool kFp8, int kTp>
@@ -370,12 +439,10 @@ __device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* rin
     constexpr uint32_t kId1 = ptx::make_idesc(kFormat, kRows, S::kN1), kId2 = ptx::make_idesc(kFormat, kRows, S::kN2);
     int it = 0, buf_it = 0;
     for (int n = 0;; ++n) {
-        const int code = next_claim<false>(st, n, 0);
-        if (code == kEnd) return;
-        const Share s = share_at(p, st, code);
-        const int group = s.phase == 0 ? p.kb1 : p.pairs2;  // units of a tile and expert
-        bool fresh = true;                                  // the next unit begins an accumulator buffer
-        for (int u = s.lo; u < s.hi; ++u, ++it) {
+        const Piece q = next_piece<false>(p, st, n, 0);
+        if (q.phase >= 2) return;
+        bool fresh = true;  // the next unit begins an accumulator buffer
+        for (int u = q.lo; u < q.hi; ++u, ++it) {
             const int slot = it % S::kStages, buf = buf_it % S::kBufs;
             if (fresh && !ptx::mbar_wait(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
             if (!ptx::mbar_wait(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit)) return;
@@ -388,14 +455,14 @@ __device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* rin
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t ak = ptx::smem_desc_advance(da, half * kTileBytes + k * 32);
-                    if (s.phase == 0)  // gate rows, value rows
+                    if (q.phase == 0)  // gate rows, value rows
                         ptx::umma<kKind>(d + half * S::kN1, ak, ptx::smem_desc_advance(db, k * 32), kId1, (!kFp8 && !fresh) || k > 0);
                     else               // two K blocks: with their own scales in FP8, one sum in bf16
                         ptx::umma<kKind>(d + (kFp8 ? half * S::kN2 : 0), ak, ptx::smem_desc_advance(db, half * S::kN2 * kKBytes + k * 32), kId2,
                                          (!kFp8 && (!fresh || half > 0)) || k > 0);
                 }
             ptx::umma_commit(&st.empty[slot]);
-            const bool done = kFp8 || u + 1 == s.hi || (u + 1) % group == 0;
+            const bool done = kFp8 || u + 1 == q.hi || (q.phase == 1 && (u + 1) % p.pairs2 == 0);
             if (done) {
                 ptx::umma_commit(&st.tmem_full[buf]);
                 ++buf_it;
@@ -412,23 +479,18 @@ __device__ __forceinline__ float weight_scale(const float* scale, int mode, int 
     return mode == DQMOE_QUANT_FP8_TENSOR ? scale[e] : 1.0f;
 }
 
+// Accumulators to scaled sums of a piece, which go to the piece's place in the workspace.
 template <bool kFp8, int kTp>
-struct Epilogue {
+struct Drain {
     using S = Shape<kFp8, kTp>;
+    static constexpr int kCols = kTp < 16 ? kTp : 16;  // columns in registers at a time
     const Params& p;
     Tail& st;
     uint8_t* ring;
     uint32_t tmem;
-    int warp, lane, row;  // warp 0..3 of the epilogue, row = TMEM lane = weight row of the tile
+    int warp, lane, row;  // warp 0..3, row = TMEM lane = weight row of the tile
     int it = 0, buf_it = 0;
-    uint32_t meetings = 0;
 
-    // The epilogue warps wait for one another at an mbarrier, whose wait ends also where one of them has given up.
-    __device__ __forceinline__ bool meet() {
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&st.meet);
-        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
-    }
     __device__ __forceinline__ bool acquire() {
         const int buf = buf_it % S::kBufs;
         if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (buf_it / S::kBufs) & 1, &st.abort_flag, kWaitLimit)) return false;
@@ -439,42 +501,164 @@ struct Epilogue {
     __device__ __forceinline__ bool stage_full() {
         return ptx::mbar_wait_warp(&st.full[it % S::kStages], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit);
     }
-    __device__ __forceinline__ void release_stage() {
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&st.empty[it % S::kStages]);
-    }
-    __device__ __forceinline__ void release_buffer() {
+    __device__ __forceinline__ void release(bool stage) {
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
+        if (lane == 0) {
+            ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
+            if (stage) ptx::mbar_arrive(&st.empty[it % S::kStages]);
+        }
         ++buf_it;
     }
-    __device__ __forceinline__ uint32_t buffer() const { return tmem + (uint32_t(warp * 32) << 16) + (buf_it % S::kBufs) * S::kBufCols; }
+    __device__ __forceinline__ uint32_t buffer() const { return tmem + (buf_it % S::kBufs) * S::kBufCols; }
 
     // sum += (hi + lo / 16) * scale of every token of `mask`
     __device__ __forceinline__ void add_scaled(uint32_t taddr, const float* token_scale, float row_scale, uint32_t mask, float (&sum)[kTp]) {
-        float hi[kTp], lo[kTp];
-        ptx::tmem_read<kTp>(taddr, hi);
-        ptx::tmem_read<kTp>(taddr + kTp, lo);
-        ptx::tmem_landed<kTp>(hi, lo);
 #pragma unroll
-        for (int t = 0; t < kTp; t += 4) {
-            const float4 sc = *reinterpret_cast<const float4*>(token_scale + t);
-            const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+        for (int c = 0; c < kTp; c += kCols) {
+            if (((mask >> c) & ((1u << kCols) - 1u)) == 0) continue;
+            float hi[kCols], lo[kCols];
+            ptx::tmem_read<kCols>(taddr + c, hi);
+            ptx::tmem_read<kCols>(taddr + kTp + c, lo);
+            ptx::tmem_landed<kCols>(hi, lo);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if ((mask >> (t + i)) & 1u) sum[t + i] = fmaf(fmaf(lo[t + i], 0.0625f, hi[t + i]), s4[i] * row_scale, sum[t + i]);
+            for (int t = 0; t < kCols; t += 4) {
+                const float4 sc = *reinterpret_cast<const float4*>(token_scale + c + t);
+                const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((mask >> (c + t + i)) & 1u) sum[c + t + i] = fmaf(fmaf(lo[t + i], 0.0625f, hi[t + i]), s4[i] * row_scale, sum[c + t + i]);
+            }
         }
     }
 
-    // Counts this block's part of a tile in: 1 for the block whose part is the last, 0 for another, -1 where a warp has given up.
-    __device__ __forceinline__ int last_part(int* counter, int parts) {
-        __threadfence();
+    __device__ __forceinline__ bool fc1(const Piece& q, float* to) {
+        const int j = q.tile / p.tiles1, e = st.hit[j], i = min((q.tile - j * p.tiles1) * kRows + row, p.I - 1);
+        const uint32_t mask = st.hit_mask[j];
+        float g[kTp], v[kTp];
+        if constexpr (kFp8) {
+#pragma unroll
+            for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
+            float sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, q.lo);
+            float sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, q.lo);
+            for (int kb = q.lo; kb < q.hi; ++kb, ++it) {
+                const float gs = sg, vs = sv;
+                if (kb + 1 < q.hi) {  // the next unit's, while this one's MMAs are on their way
+                    sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb + 1);
+                    sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb + 1);
+                }
+                if (!stage_full() || !acquire()) return false;
+                const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + S::kN1 * kKBytes);
+                add_scaled(buffer(), token_scale, gs, mask, g);
+                add_scaled(buffer() + S::kN1, token_scale, vs, mask, v);
+                release(true);
+            }
+        } else {
+            if (!acquire()) return false;
+            ptx::tmem_read<kTp>(buffer(), g);
+            ptx::tmem_read<kTp>(buffer() + S::kN1, v);
+            ptx::tmem_landed<kTp>(g, v);
+            release(false);
+        }
+#pragma unroll
+        for (int t = 0; t < kTp; ++t)
+            if ((mask >> t) & 1u) {
+                to[t * kRows + row] = g[t];
+                to[(kTp + t) * kRows + row] = v[t];
+            }
+        return true;
+    }
+
+    __device__ __forceinline__ bool fc2(const Piece& q, float* to) {
+        const int kb2 = (p.I + S::kKElems - 1) / S::kKElems;
+        const int h = min(q.tile * kRows + row, p.H - 1);
+        float sum[kTp];
+#pragma unroll
+        for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
+        if constexpr (kFp8) {
+            float scale[2];
+            auto scales_of = [&](int u) {
+                const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
+                scale[0] = weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb);
+                scale[1] = kb + 1 < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb + 1) : 0.0f;
+            };
+            scales_of(q.lo);
+            for (int u = q.lo; u < q.hi; ++u, ++it) {
+                const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
+                const float s0 = scale[0], s1 = scale[1];
+                if (u + 1 < q.hi) scales_of(u + 1);
+                const uint32_t mask = st.hit_mask[j];
+                if (!stage_full() || !acquire()) return false;
+                const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + 2 * S::kN2 * kKBytes);
+                add_scaled(buffer(), token_scale, s0, mask, sum);
+                if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale + kTp, s1, mask, sum);  // nothing was laid out for a block past I
+                release(true);
+            }
+        } else {
+            for (int u = q.lo; u < q.hi;) {  // expert by expert: only the tokens that chose it take part
+                const int j = u / p.pairs2;
+                u = min(q.hi, (j + 1) * p.pairs2);
+                if (!acquire()) return false;
+                float hi[kTp], lo[kTp];
+                ptx::tmem_read<kTp>(buffer(), hi);
+                ptx::tmem_read<kTp>(buffer() + kTp, lo);
+                ptx::tmem_landed<kTp>(hi, lo);
+                release(false);
+                const uint32_t mask = st.hit_mask[j];
+#pragma unroll
+                for (int t = 0; t < kTp; ++t)
+                    if ((mask >> t) & 1u) sum[t] += hi[t] + lo[t];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kTp; ++t)
+            if (t < p.T) to[t * kRows + row] = sum[t];
+        return true;
+    }
+
+    __device__ __forceinline__ void run() {
+        for (int n = 0;; ++n) {
+            int code = 0;
+            const Piece q = next_piece<true>(p, st, n, lane, &code);
+            // the finishing warps are through with what used this note, and this place for a tile in one part, before
+            const int slot = n % kJobs;
+            if (q.phase == 3 || !ptx::mbar_wait_warp(&st.job_empty[slot], ((n / kJobs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
+            if (q.phase == 0) {
+                if (!fc1(q, p.part1 + (st.split1 > 1 ? size_t(code) : size_t(blockIdx.x) * kJobs + slot) * S::kPart1)) return;
+            } else if (q.phase == 1) {
+                if (!fc2(q, p.part2 + (size_t(q.tile) * kMaxParts + q.part) * S::kPart2)) return;
+            }
+            if (warp == 0 && lane == 0) *const_cast<volatile int*>(&st.job[slot]) = code;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.job_full[slot]);
+            if (q.phase == 2) return;
+        }
+    }
+};
+
+// Sums over the parts of a tile; fc1: the activation, laid out as fc2's second operand; fc2: the output.
+template <bool kFp8, int kTp>
+struct Finish {
+    using S = Shape<kFp8, kTp>;
+    const Params& p;
+    Tail& st;
+    int warp, lane, row;
+    uint32_t meetings = 0;
+
+    // The finishing warps wait for one another at an mbarrier, whose wait ends also where one of them has given up.
+    __device__ __forceinline__ bool meet() {
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&st.meet);
+        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
+    }
+    // Counts a part in (all of it is written, and seen by the counting thread): 1 where it is the last of `parts`, 0 where not, -1 where a
+    // warp has given up.
+    __device__ __forceinline__ int count_in(int* counter, int parts) {
+        if (parts == 1) return 1;
+        if (warp == 0 && lane == 0) st.last = streamk::atomic_add_acq_rel_gpu(counter, 1) == parts - 1;
         if (!meet()) return -1;
-        if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(counter, 1) == parts - 1;
-        if (!meet()) return -1;
-        const int last = *const_cast<volatile int*>(&st.last_part);
-        __threadfence();
+        const int last = *const_cast<volatile int*>(&st.last);
+        if (!meet()) return -1;  // all have read it
         return last;
     }
 
@@ -485,18 +669,42 @@ struct Epilogue {
         return who == 0 ? 1.0f : st.topk_weight[t][__ffs(who) - 1];  // shared experts are not in the list
     }
 
-    __device__ __forceinline__ bool finish_fc1(int tile, float (&g)[kTp], float (&v)[kTp]) {
-        const int j = tile / p.tiles1, it_tile = tile - j * p.tiles1, e = st.hit[j];
+    // sum[t] of parts first, first + 1, ..., `parts` of them, over the tokens of `mask`
+    __device__ __forceinline__ void add_parts(const float* part, int parts, size_t stride, uint32_t mask, float (&sum)[kTp]) const {
+#pragma unroll
+        for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
+#pragma unroll 2
+        for (int i = 0; i < parts; ++i) {
+            float v[kTp];  // all loads before the first use
+#pragma unroll
+            for (int t = 0; t < kTp; ++t) v[t] = (mask >> t) & 1u ? streamk::ld_partial(part + i * stride + t * kRows + row) : 0.0f;
+#pragma unroll
+            for (int t = 0; t < kTp; ++t) sum[t] += v[t];
+        }
+    }
+
+    __device__ __forceinline__ bool fc1(const Piece& q, const float* part) {
+        const int now = count_in(&p.counters[4 + p.max_hit + q.tile], st.split1);
+        if (now <= 0) return now == 0;
+        const int j = q.tile / p.tiles1, tile = q.tile - j * p.tiles1, e = st.hit[j];
         const uint32_t mask = st.hit_mask[j];
-        const bool inside = it_tile * kRows + row < p.I;
-        uint8_t* rec = p.aq + (size_t(j) * p.pairs2 + (kFp8 ? it_tile >> 1 : it_tile)) * p.rec2;
+        float g[kTp], v[kTp];
+        if (st.split1 > 1) part -= q.part * S::kPart1;
+        add_parts(part, st.split1, S::kPart1, mask, g);
+        add_parts(part + kTp * kRows, st.split1, S::kPart1, mask, v);
+        const bool inside = tile * kRows + row < p.I;
+        uint8_t* rec = p.aq + (size_t(j) * p.pairs2 + (kFp8 ? tile >> 1 : tile)) * p.rec2;
+#pragma unroll
+        for (int t = 0; t < kTp; ++t)
+            if ((mask >> t) & 1u) {              // the same for all threads
+                const float w = weight_of(t, e);  // all lanes, also those of rows past I
+                g[t] = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
+            }
         if constexpr (kFp8) {
-            const int half = it_tile & 1;
+            const int half = tile & 1;
 #pragma unroll
             for (int t = 0; t < kTp; ++t)
-                if ((mask >> t) & 1u) {  // the same for all threads
-                    const float w = weight_of(t, e);  // all lanes, also those of rows past I
-                    g[t] = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
+                if ((mask >> t) & 1u) {
                     const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(g[t]) & 0x7fffffffu);
                     if (lane == 0) st.amax[warp][t] = most;
                 }
@@ -520,176 +728,58 @@ struct Epilogue {
 #pragma unroll
             for (int t = 0; t < kTp; ++t)
                 if ((mask >> t) & 1u) {
-                    const float w = weight_of(t, e);  // all lanes, also those of rows past I
-                    const float a = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
-                    const uint32_t hi = f2bf_bits(a);
-                    const float rest = a - __uint_as_float(hi << 16);
+                    const uint32_t hi = f2bf_bits(g[t]);
+                    const float rest = g[t] - __uint_as_float(hi << 16);
                     // an infinite value has no rest
                     const uint32_t lo = (hi & 0x7fffu) < 0x7f80u ? f2bf_bits(rest) : 0u;
                     *reinterpret_cast<uint16_t*>(data + swizzled(t, byte)) = uint16_t(hi);
                     *reinterpret_cast<uint16_t*>(data + swizzled(kTp + t, byte)) = uint16_t(lo);
                 }
         }
-        // to the bulk copies of other blocks
-        asm volatile("fence.proxy.async;" ::: "memory");
-        __threadfence();
+        asm volatile("fence.proxy.async;" ::: "memory");  // to the bulk copies of other blocks
         if (!meet()) return false;
-        if (warp == 0 && lane == 0) streamk::atomic_add_acq_rel_gpu(&p.counters[2], 1);
+        if (warp == 0 && lane == 0) streamk::atomic_add_acq_rel_gpu(&p.counters[4 + j], 1);
         return true;
     }
 
-    __device__ __forceinline__ bool fc1(const Share& s, int units) {
-        const int shares = phase_shares(p, units);
-        for (int u = s.lo; u < s.hi;) {
-            const int tile = u / p.kb1, end = min(s.hi, (tile + 1) * p.kb1);
-            const int j = tile / p.tiles1, e = st.hit[j], i = min((tile - j * p.tiles1) * kRows + row, p.I - 1);
-            float g[kTp], v[kTp];
-            if constexpr (kFp8) {
+    __device__ __forceinline__ bool fc2(const Piece& q) {
+        const int group = q.part / kGroup, groups = (st.parts2 + kGroup - 1) / kGroup, in_group = min(kGroup, st.parts2 - group * kGroup);
+        const uint32_t all = p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u;
+        int* counters = p.counters + 4 + p.max_hit + p.max_hit * p.tiles1;
+        int now = count_in(&counters[q.tile * kGroups + group], in_group);
+        if (now <= 0) return now == 0;
+        float sum[kTp];
+        add_parts(p.part2 + (size_t(q.tile) * kMaxParts + group * kGroup) * S::kPart2, in_group, S::kPart2, all, sum);
+        if (groups > 1) {
+            float* to = p.group2 + size_t(q.tile) * kGroups * S::kPart2;
 #pragma unroll
-                for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
-                const uint32_t mask = st.hit_mask[j];
-                const int kb0 = u - tile * p.kb1;
-                float sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb0);
-                float sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb0);
-                for (; u < end; ++u, ++it) {
-                    const int kb = u - tile * p.kb1;
-                    const float gs = sg, vs = sv;
-                    if (kb + 1 < p.kb1) {  // the next unit's, while this one's MMAs are on their way
-                        sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb + 1);
-                        sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb + 1);
-                    }
-                    if (!stage_full() || !acquire()) return false;
-                    const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + S::kN1 * kKBytes);
-                    add_scaled(buffer(), token_scale, gs, mask, g);
-                    add_scaled(buffer() + S::kN1, token_scale, vs, mask, v);
-                    release_buffer();
-                    release_stage();
-                }
-            } else {
-                it += end - u;
-                u = end;
-                if (!acquire()) return false;
-                ptx::tmem_read<kTp>(buffer(), g);
-                ptx::tmem_read<kTp>(buffer() + S::kN1, v);
-                ptx::tmem_landed<kTp>(g, v);
-                release_buffer();
-            }
-            const int first = streamk::share_of(tile * p.kb1, shares, units), last = streamk::share_of((tile + 1) * p.kb1 - 1, shares, units);
-            if (first < last) {
-                // a share's first tile has slot 0, a later one slot 1: only the first and the last can be shared with others
-                const size_t block = size_t(2) * kTp * kRows;
-                float* mine = p.part1 + (size_t(s.index) * 2 + (tile == s.lo / p.kb1 ? 0 : 1)) * block + row;
-#pragma unroll
-                for (int t = 0; t < kTp; ++t)
-                    if (t < p.T) {
-                        mine[t * kRows] = g[t];
-                        mine[(kTp + t) * kRows] = v[t];
-                    }
-                const int now = last_part(&p.counters[4 + tile], last - first + 1);
-                if (now < 0) return false;
-                if (now == 0) continue;
-#pragma unroll
-                for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
-                for (int o = first; o <= last; ++o) {
-                    const int o_lo = streamk::first_unit(o, shares, units);
-                    const float* part = p.part1 + (size_t(o) * 2 + (tile == o_lo / p.kb1 ? 0 : 1)) * block + row;
-#pragma unroll
-                    for (int t = 0; t < kTp; ++t)
-                        if (t < p.T) {
-                            g[t] += streamk::ld_partial(part + t * kRows);
-                            v[t] += streamk::ld_partial(part + (kTp + t) * kRows);
-                        }
-                }
-            }
-            if (!finish_fc1(tile, g, v)) return false;
+            for (int t = 0; t < kTp; ++t)
+                if (t < p.T) to[group * S::kPart2 + t * kRows + row] = sum[t];
+            if (!meet()) return false;
+            now = count_in(&counters[p.tiles2 * kGroups + q.tile], groups);
+            if (now <= 0) return now == 0;
+            add_parts(to, groups, S::kPart2, all, sum);
         }
-        return true;
-    }
-
-    __device__ __forceinline__ bool fc2(const Share& s, int units) {
-        const int shares = phase_shares(p, units);
-        const int per_tile = st.n_hit * p.pairs2;
-        const int kb2 = (p.I + S::kKElems - 1) / S::kKElems;
-        for (int u = s.lo; u < s.hi;) {
-            const int tile = u / per_tile, end = min(s.hi, (tile + 1) * per_tile);
-            const int h = min(tile * kRows + row, p.H - 1);
-            float sum[kTp];
+        const int h = q.tile * kRows + row;
+        if (h < p.H) {
+            const uint32_t bad = st.bad_tokens;
 #pragma unroll
-            for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
-            if constexpr (kFp8) {
-                float scale[2];
-                auto scales_of = [&](int unit) {
-                    const int rest = unit - tile * per_tile, j = rest / p.pairs2, kb = (rest - j * p.pairs2) * 2;
-                    scale[0] = weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb);
-                    scale[1] = kb + 1 < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb + 1) : 0.0f;
-                };
-                scales_of(u);
-                for (; u < end; ++u, ++it) {
-                    const int rest = u - tile * per_tile, j = rest / p.pairs2, kb = (rest - j * p.pairs2) * 2;
-                    const float s0 = scale[0], s1 = scale[1];
-                    if (u + 1 < end) scales_of(u + 1);
-                    const uint32_t mask = st.hit_mask[j];
-                    if (!stage_full() || !acquire()) return false;
-                    const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + 2 * S::kN2 * kKBytes);
-                    add_scaled(buffer(), token_scale, s0, mask, sum);
-                    if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale + kTp, s1, mask, sum);  // nothing was laid out for a block past I
-                    release_buffer();
-                    release_stage();
-                }
-            } else {
-                while (u < end) {  // expert by expert: only the tokens that chose it take part
-                    const int j = (u - tile * per_tile) / p.pairs2, stop = min(end, tile * per_tile + (j + 1) * p.pairs2);
-                    it += stop - u;
-                    u = stop;
-                    if (!acquire()) return false;
-                    float hi[kTp], lo[kTp];
-                    ptx::tmem_read<kTp>(buffer(), hi);
-                    ptx::tmem_read<kTp>(buffer() + kTp, lo);
-                    ptx::tmem_landed<kTp>(hi, lo);
-                    release_buffer();
-                    const uint32_t mask = st.hit_mask[j];
-#pragma unroll
-                    for (int t = 0; t < kTp; ++t)
-                        if ((mask >> t) & 1u) sum[t] += hi[t] + lo[t];
-                }
-            }
-            const int first = streamk::share_of(tile * per_tile, shares, units), last = streamk::share_of((tile + 1) * per_tile - 1, shares, units);
-            if (first < last) {
-                const size_t block = size_t(kTp) * kRows;
-                float* mine = p.part2 + (size_t(s.index) * 2 + (tile == s.lo / per_tile ? 0 : 1)) * block + row;
-#pragma unroll
-                for (int t = 0; t < kTp; ++t)
-                    if (t < p.T) mine[t * kRows] = sum[t];
-                const int now = last_part(&p.counters[4 + st.n_hit * p.tiles1 + tile], last - first + 1);
-                if (now < 0) return false;
-                if (now == 0) continue;
-#pragma unroll
-                for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
-                for (int o = first; o <= last; ++o) {
-                    const int o_lo = streamk::first_unit(o, shares, units);
-                    const float* part = p.part2 + (size_t(o) * 2 + (tile == o_lo / per_tile ? 0 : 1)) * block + row;
-#pragma unroll
-                    for (int t = 0; t < kTp; ++t)
-                        if (t < p.T) sum[t] += streamk::ld_partial(part + t * kRows);
-                }
-            }
-            if (tile * kRows + row < p.H) {
-                const uint32_t bad = st.bad_tokens;
-#pragma unroll
-                for (int t = 0; t < kTp; ++t)
-                    if (t < p.T) p.out[size_t(t) * p.H + h] = __float2bfloat16_rn((bad >> t) & 1u ? __uint_as_float(0x7fffffffu) : sum[t]);
-            }
+            for (int t = 0; t < kTp; ++t)
+                if (t < p.T) p.out[size_t(t) * p.H + h] = __float2bfloat16_rn((bad >> t) & 1u ? __uint_as_float(0x7fffffffu) : sum[t]);
         }
         return true;
     }
 
     __device__ __forceinline__ void run() {
         for (int n = 0;; ++n) {
-            const int code = next_claim<true>(st, n, lane);
-            if (code == kEnd) return;
-            const Share s = share_at(p, st, code);
-            const int units = phase_units(p, st, s.phase);
-            if (!(s.phase == 0 ? fc1(s, units) : fc2(s, units))) return;
+            const int slot = n % kJobs;
+            if (!ptx::mbar_wait_warp(&st.job_full[slot], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
+            const int code = *const_cast<volatile int*>(&st.job[slot]);
+            const Piece q = piece_at(p, st, code);
+            if (q.phase == 2) return;
+            if (!(q.phase == 0 ? fc1(q, p.part1 + (st.split1 > 1 ? size_t(code) : size_t(blockIdx.x) * kJobs + slot) * S::kPart1) : fc2(q))) return;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.job_empty[slot]);
         }
     }
 };
@@ -730,7 +820,10 @@ __device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int 
             st.hit[count + i] = uint16_t(p.E + i);
             st.hit_mask[count + i] = p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u;
         }
-        if (lane == 0) st.n_hit = count + p.n_shared;
+        if (lane == 0) {
+            st.n_hit = count + p.n_shared;
+            plan_pieces(p, st);
+        }
     }
 }
 
@@ -746,8 +839,8 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
-            ptx::mbar_init(&st.full[i], 1);
-            ptx::mbar_init(&st.empty[i], kFp8 ? 5 : 1);  // the tensor core's reads, and the epilogue warps' of the scales
+            ptx::mbar_init(&st.full[i], 2);              // weights, tokens
+            ptx::mbar_init(&st.empty[i], kFp8 ? 5 : 1);  // the tensor core's reads, and the draining warps' of the scales
         }
         for (int i = 0; i < 4; ++i) {
             ptx::mbar_init(&st.tmem_full[i], 1);
@@ -755,7 +848,11 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         }
         for (int i = 0; i < kClaims; ++i) {
             ptx::mbar_init(&st.claim_full[i], 1);
-            ptx::mbar_init(&st.claim_empty[i], 5);
+            ptx::mbar_init(&st.claim_empty[i], 6);  // tokens, MMA, draining warps
+        }
+        for (int i = 0; i < kJobs; ++i) {
+            ptx::mbar_init(&st.job_full[i], 4);
+            ptx::mbar_init(&st.job_empty[i], 4);
         }
         ptx::mbar_init(&st.meet, 4);
         st.abort_flag = 0;
@@ -781,14 +878,20 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         for (int i = blockIdx.x * kThreads + threadIdx.x; i < p.T * p.H; i += gridDim.x * kThreads)
             p.out[i] = __float2bfloat16_rn((st.bad_tokens >> (i / p.H)) & 1u ? __uint_as_float(0x7fffffffu) : 0.0f);
     } else if (warp == 0) {
-        if (ptx::elect_one()) produce<kFp8, kTp>(p, map_b, map_b1, st, ring, claim);
+        if (ptx::elect_one()) load_weights<kFp8, kTp>(p, map_b, map_b1, st, ring, claim);
         __syncwarp();
     } else if (warp == 1) {
         if (ptx::elect_one()) multiply<kFp8, kTp>(p, st, ring, tmem);
         __syncwarp();
+    } else if (warp == 2) {
+        if (ptx::elect_one()) load_tokens<kFp8, kTp>(p, st, ring);
+        __syncwarp();
+    } else if (warp >= 8) {
+        Finish<kFp8, kTp> f{p, st, warp - 8, lane, (warp - 8) * 32 + lane};
+        f.run();
     } else if (warp >= 4) {
-        Epilogue<kFp8, kTp> ep{p, st, ring, tmem, warp - 4, lane, (warp - 4) * 32 + lane};
-        ep.run();
+        Drain<kFp8, kTp> d{p, st, ring, tmem + (uint32_t((warp - 4) * 32) << 16), warp - 4, lane, (warp - 4) * 32 + lane};
+        d.run();
     }
     __syncthreads();
     if (threadIdx.x == 0 && st.abort_flag != 0 && *const_cast<volatile int*>(p.status) == 0) *p.status = kStatusRing;
@@ -801,20 +904,20 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
 // ---------------------------------------------------------------- host
 
 struct Layout {
-    size_t counters, logits, xq, aq, part1, part2, total;
+    size_t counters, logits, xq, aq, part1, part2, group2, total;
 };
 static Layout plan(Params* p, bool fp8) {
     const int tp = token_rows(p->T);
     const int ke = fp8 ? 128 : 64;
-    const int hit = (p->T * p->k < p->E ? p->T * p->k : p->E) + p->n_shared;
+    p->max_hit = (p->T * p->k < p->E ? p->T * p->k : p->E) + p->n_shared;
     p->kb1 = ceil_div(p->H, ke);
     p->pairs2 = ceil_div(ceil_div(p->I, ke), 2);
     p->tiles1 = ceil_div(p->I, kRows);
     p->tiles2 = ceil_div(p->H, kRows);
     p->rec1 = size_t(fc1_cols(fp8, tp)) * kKBytes + (fp8 ? size_t(tp) * sizeof(float) : 0);
     p->rec2 = size_t(2) * fc2_cols(tp) * kKBytes + (fp8 ? size_t(2) * tp * sizeof(float) : 0);
-    p->shares = sm_count();
-    p->n_counters = 4 + hit * p->tiles1 + p->tiles2;
+    p->blocks = sm_count();
+    p->n_counters = 4 + p->max_hit + p->max_hit * p->tiles1 + p->tiles2 * (kGroups + 1);
     Layout L{};
     size_t off = 0;
     auto add = [&](size_t bytes) {
@@ -825,9 +928,11 @@ static Layout plan(Params* p, bool fp8) {
     L.counters = add(size_t(p->n_counters) * sizeof(int));
     L.logits = add(size_t(p->T) * p->E * sizeof(float));
     L.xq = add(size_t(p->kb1) * p->rec1);
-    L.aq = add(size_t(hit) * p->pairs2 * p->rec2);
-    L.part1 = add(size_t(p->shares) * 4 * tp * kRows * sizeof(float));
-    L.part2 = add(size_t(p->shares) * 2 * tp * kRows * sizeof(float));
+    L.aq = add(size_t(p->max_hit) * p->pairs2 * p->rec2);
+    // fc1's parts: fewer than 6 per block where tiles are split (up to 3 per block round up to twice as many), else kJobs places per block
+    L.part1 = add(size_t(p->blocks) * 6 * 2 * tp * kRows * sizeof(float));
+    L.part2 = add(size_t(p->tiles2) * kMaxParts * tp * kRows * sizeof(float));
+    L.group2 = add(size_t(p->tiles2) * kGroups * tp * kRows * sizeof(float));
     L.total = off;
     return L;
 }
@@ -840,7 +945,7 @@ static int check_sizes(int T, int H, int I, int E, int k, int n_shared, int quan
     DQ_CHECK(H > 0 && I > 0 && E > 0 && k > 0 && k <= E && k <= kMaxTopk && n_shared >= 0);
     DQ_CHECK_FMT(int64_t(E) + n_shared <= kMaxExperts, "E=%d and n_shared=%d: at most %d experts", E, n_shared, kMaxExperts);
     DQ_CHECK_FMT(H % 16 == 0 && I % 16 == 0, "hidden_size=%d and inter_size=%d must be multiples of 16", H, I);
-    // row numbers of the tensor maps, unit numbers and offsets in a tile are 32-bit
+    // row numbers of the tensor maps and unit numbers are 32-bit
     DQ_CHECK_FMT(H <= (1 << 17) && I <= (1 << 17) && int64_t(E + n_shared) * (int64_t(2) * I + H) < (int64_t(1) << 31) &&
                      int64_t(E + n_shared) * ceil_div(I, 64) * ceil_div(H, 64) < (int64_t(1) << 30),
                  "H=%d I=%d E=%d: too large", H, I, E);
@@ -865,7 +970,7 @@ static int opt_in(K kern, int which) {
 template <bool kFp8, int kTp>
 static int launch_experts(const CUtensorMap& b, const CUtensorMap& b1, const Params& p, cudaStream_t stream) {
     DQ_RC(opt_in(moe_decode_experts_kernel<kFp8, kTp>, (kFp8 ? 3 : 0) + (kTp == 8 ? 0 : kTp == 16 ? 1 : 2)));
-    return launch_pdl(moe_decode_experts_kernel<kFp8, kTp>, dim3(p.shares), kThreads, kSmemBytes, stream, b, b1, p);
+    return launch_pdl(moe_decode_experts_kernel<kFp8, kTp>, dim3(p.blocks), kThreads, kSmemBytes, stream, b, b1, p);
 }
 
 template <bool kF32, bool kFp8>
@@ -938,6 +1043,7 @@ int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, 
     p.aq = ws + L.aq;
     p.part1 = reinterpret_cast<float*>(ws + L.part1);
     p.part2 = reinterpret_cast<float*>(ws + L.part2);
+    p.group2 = reinterpret_cast<float*>(ws + L.group2);
     p.status = device_status_word();
     if (p.status == nullptr) return DQMOE_ERR_CUDA;
     const int esz = fp8 ? 1 : 2;

