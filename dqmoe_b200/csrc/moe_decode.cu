@@ -40,14 +40,16 @@ namespace moe_decode {
 constexpr int kMaxTokens = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 32;
-constexpr int kThreads = 384;                 // warp 0 weights, warp 1 MMA, warp 2 tokens, warps 4..7 drain, warps 8..11 finish; all choose the experts
+constexpr int kThreads = 384;                 // warp 0 weights, 1 MMA, 2 tokens, 3 count, warps 4..7 drain, warps 8..11 finish; all choose the experts
 constexpr int kRows = 128;                    // weight rows of an MMA
 constexpr int kKBytes = 128;                  // bytes of a K block: one swizzle row
 constexpr int kTileBytes = kRows * kKBytes;   // 16 KiB
 constexpr int kABytes = 2 * kTileBytes;       // a unit's weights
 constexpr int kRingBytes = 205 * 1024;
-constexpr int kMaxParts = 40;                 // of an fc2 tile
-constexpr int kGroup = 7;                     // parts that are added to one sum first
+constexpr int kMaxSplit1 = 6;                 // parts of an fc1 tile
+constexpr int kMaxParts = 40;                 // of an fc2 tile: this many at most shrink, the others are equal
+constexpr int kMaxShrinking = 16;
+constexpr int kGroup = 8;                     // parts that are added to one sum first
 constexpr int kGroups = (kMaxParts + kGroup - 1) / kGroup;
 constexpr int kMaxStages = 6;
 constexpr int kScaleBytes = 1024;             // room behind a stage's second operand for its scales
@@ -83,9 +85,10 @@ struct Params {
     float* logits;            // [T, E]
     uint8_t* xq;              // [kb1] records: [fc1_cols][128 B] swizzled, scales [token_rows]
     uint8_t* aq;              // [experts hit][pairs2] records: two of [fc2_cols][128 B] swizzled, scales [2][token_rows]
-    float* part1;             // [piece, or kJobs x block][gate, value][token][128]
-    float* part2;             // [tile][part][token][128]
-    float* group2;            // [tile][group][token][128]
+    // partial sums, four tokens of a weight row together: [token / 4][128][4]
+    float* part1;             // [kJobs of each block, then pieces of split tiles][gate, value]
+    float* part2;             // [tile][part]
+    float* group2;            // [tile][group]
     int* status;
 };
 
@@ -253,13 +256,14 @@ struct alignas(16) Tail {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t tmem_full[4], tmem_empty[4];
     uint64_t claim_full[kClaims], claim_empty[kClaims];
-    uint64_t job_full[kJobs], job_empty[kJobs];        // pieces from the draining warps to the finishing ones
+    uint64_t job_full[kJobs], job_empty[kJobs];  // pieces whose sums are written, from the draining warps to the counting one
+    uint64_t last_full[kJobs];                   // those that complete a tile or a group of parts, from there to the finishing warps
     uint64_t meet;                             // the finishing warps
-    int claim[kClaims], job[kJobs];
+    int claim[kClaims], job[kJobs], last_job[kJobs];
     uint32_t tmem_base;
     int abort_flag;
     int n_hit;
-    int split1, pieces1;                       // parts of an fc1 tile; pieces of fc1
+    int whole1, split1, pieces1;               // fc1 tiles in one piece; parts of each of the others; pieces of fc1
     int parts2, pieces2;                       // parts of an fc2 tile; pieces of both
     int bound2[kMaxParts + 1];                 // first unit of each part of an fc2 tile
     uint32_t bad_tokens;                       // tokens without a number among their weights
@@ -274,31 +278,40 @@ struct alignas(16) Tail {
 constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 
-// Pieces of the work, from the experts that are hit. fc1: a tile in split1 equal parts, three pieces per block at least, of four units or
-// more. fc2: the units of a tile ([expert][pair of K blocks]) in parts, each half of what would be left for a block if all were
-// shared out evenly, so that the blocks end together however fast each is; not under two units unless there are few in all.
-__device__ __forceinline__ void plan_pieces(const Params& p, Tail& st) {
-    const int tiles1 = st.n_hit * p.tiles1;
-    st.split1 = max(1, min((3 * p.blocks + tiles1 - 1) / max(tiles1, 1), p.kb1 / 4));
-    st.pieces1 = tiles1 * st.split1;
-    const int units = st.n_hit * p.pairs2;
-    const float per_block = float(p.tiles2) / float(2 * p.blocks);  // of a unit of every tile, halved
-    const int least = max(1, min(4, int(float(units) * per_block)));
-    int q = 0, at = 0;
-    while (at < units) {
-        const int rest = units - at;
-        const int n = max(max(least, int(float(rest) * per_block)), int(__fdividef(float(rest), float(kMaxParts - q))) + 1);
-        st.bound2[q++] = at;
-        at += min(n, rest);
+// Pieces of the work, from the experts that are hit; by one warp.
+// fc1: whole tiles, but the last ones, about one per block, in parts of some eight units, so that fc1's end is not waited for long.
+// fc2: the units of a tile ([expert][pair of K blocks]) in parts, each half of what would be left for a block if all were shared out
+// evenly, so that the blocks end together however fast each is: what is left shrinks by a constant factor per part, down to where the parts
+// have the least size, from where on they are equal. Parts are not empty: each is a unit or more before rounding.
+__device__ __forceinline__ void plan_pieces(const Params& p, Tail& st, int n_hit, int lane) {
+    const int tiles1 = n_hit * p.tiles1, cut = min(tiles1, p.blocks);
+    const int split = max(1, min(max(p.kb1 / 8, (3 * p.blocks + tiles1 - 1) / max(tiles1, 1)), min(kMaxSplit1, p.kb1 / 2)));
+    const int units = n_hit * p.pairs2;
+    const float share = fminf(0.5f, float(p.tiles2) / float(2 * p.blocks));  // of what is left, per part
+    const float least = fmaxf(1.0f, fminf(4.0f, float(units) * share));
+    float knee = fminf(float(units), least / share);
+    int shrinking = 0;
+    if (knee < float(units)) shrinking = min(kMaxShrinking, int(log2f(float(units) / knee) / -log2f(1.0f - share)));
+    if (shrinking == 0) knee = float(units);
+    const int equal = max(1, min(kMaxParts - kMaxShrinking, int(knee / least)));
+    const float step = shrinking > 0 ? log2f(knee / float(units)) / float(shrinking) : 0.0f;
+    for (int q = lane; q < shrinking + equal; q += 32)
+        st.bound2[q] = int(0.001f +  // against a whole number that came out a little less
+                           (q < shrinking ? float(units) * (1.0f - exp2f(step * float(q))) : float(units) - knee * (1.0f - float(q - shrinking) / float(equal))));
+    if (lane == 0) {
+        st.n_hit = n_hit;
+        st.whole1 = tiles1 - cut;
+        st.split1 = split;
+        st.pieces1 = tiles1 - cut + cut * split;
+        st.bound2[shrinking + equal] = units;
+        st.parts2 = units > 0 ? shrinking + equal : 0;
+        st.pieces2 = st.pieces1 + st.parts2 * p.tiles2;
     }
-    st.bound2[q] = units;
-    st.parts2 = q;
-    st.pieces2 = st.pieces1 + q * p.tiles2;
 }
 
 struct Piece {
     int phase;       // 0 fc1, 1 fc2, 2 no more, 3 a wait has run out
-    int tile, part;  // fc1: tile = expert's place * tiles1 + tile of I; fc2: tile of H
+    int tile, part;  // fc1: tile = expert's place * tiles1 + tile of I, part -1 for all of it; fc2: tile of H
     int lo, hi;      // units of the tile
 };
 __device__ __forceinline__ Piece piece_at(const Params& p, const Tail& st, int c) {
@@ -306,10 +319,15 @@ __device__ __forceinline__ Piece piece_at(const Params& p, const Tail& st, int c
     if (c >= st.pieces2) return Piece{2, 0, 0, 0, 0};
     if (c < st.pieces1) {
         q.phase = 0;
-        q.tile = c / st.split1;
-        q.part = c - q.tile * st.split1;
-        q.lo = q.part * p.kb1 / st.split1;
-        q.hi = (q.part + 1) * p.kb1 / st.split1;
+        const int cut = c - st.whole1;
+        if (cut < 0) {
+            q.tile = c, q.part = -1;
+            q.lo = 0, q.hi = p.kb1;
+        } else {
+            const int tile = cut / st.split1;
+            q.tile = st.whole1 + tile, q.part = cut - tile * st.split1;
+            q.lo = q.part * p.kb1 / st.split1, q.hi = (q.part + 1) * p.kb1 / st.split1;
+        }
     } else {
         q.phase = 1;
         q.part = (c - st.pieces1) / p.tiles2;
@@ -318,6 +336,13 @@ __device__ __forceinline__ Piece piece_at(const Params& p, const Tail& st, int c
         q.hi = st.bound2[q.part + 1];
     }
     return q;
+}
+
+// Where the sums of an fc1 piece stand: places that a block uses in turn, or one for each part of a split tile.
+template <size_t kFloats>
+__device__ __forceinline__ float* place1(const Params& p, const Tail& st, const Piece& q, int slot) {
+    const size_t at = q.part < 0 ? size_t(blockIdx.x) * kJobs + slot : size_t(p.blocks) * kJobs + size_t(q.tile - st.whole1) * st.split1 + q.part;
+    return p.part1 + at * kFloats;
 }
 
 // The next piece, as the weights' thread announces it to the other roles.
@@ -479,6 +504,20 @@ __device__ __forceinline__ float weight_scale(const float* scale, int mode, int 
     return mode == DQMOE_QUANT_FP8_TENSOR ? scale[e] : 1.0f;
 }
 
+__device__ __forceinline__ uint32_t all_tokens(const Params& p) { return p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u; }
+// Sums of the tokens of `mask` (and some beside them) of a weight row.
+template <int kTp>
+__device__ __forceinline__ void put_sums(float* to, int row, uint32_t mask, const float (&sum)[kTp]) {
+#pragma unroll
+    for (int t = 0; t < kTp; t += 4)
+        if ((mask >> t) & 15u) *reinterpret_cast<float4*>(to + t * kRows + row * 4) = make_float4(sum[t], sum[t + 1], sum[t + 2], sum[t + 3]);
+}
+__device__ __forceinline__ float4 ld_partial4(const float* p) {
+    float4 v;
+    asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // Accumulators to scaled sums of a piece, which go to the piece's place in the workspace.
 template <bool kFp8, int kTp>
 struct Drain {
@@ -560,12 +599,8 @@ struct Drain {
             ptx::tmem_landed<kTp>(g, v);
             release(false);
         }
-#pragma unroll
-        for (int t = 0; t < kTp; ++t)
-            if ((mask >> t) & 1u) {
-                to[t * kRows + row] = g[t];
-                to[(kTp + t) * kRows + row] = v[t];
-            }
+        put_sums<kTp>(to, row, mask, g);
+        put_sums<kTp>(to + kTp * kRows, row, mask, v);
         return true;
     }
 
@@ -582,7 +617,7 @@ struct Drain {
                 scale[0] = weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb);
                 scale[1] = kb + 1 < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb + 1) : 0.0f;
             };
-            scales_of(q.lo);
+            if (q.lo < q.hi) scales_of(q.lo);
             for (int u = q.lo; u < q.hi; ++u, ++it) {
                 const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
                 const float s0 = scale[0], s1 = scale[1];
@@ -610,9 +645,7 @@ struct Drain {
                     if ((mask >> t) & 1u) sum[t] += hi[t] + lo[t];
             }
         }
-#pragma unroll
-        for (int t = 0; t < kTp; ++t)
-            if (t < p.T) to[t * kRows + row] = sum[t];
+        put_sums<kTp>(to, row, all_tokens(p), sum);
         return true;
     }
 
@@ -624,7 +657,7 @@ struct Drain {
             const int slot = n % kJobs;
             if (q.phase == 3 || !ptx::mbar_wait_warp(&st.job_empty[slot], ((n / kJobs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
             if (q.phase == 0) {
-                if (!fc1(q, p.part1 + (st.split1 > 1 ? size_t(code) : size_t(blockIdx.x) * kJobs + slot) * S::kPart1)) return;
+                if (!fc1(q, place1<S::kPart1>(p, st, q, slot))) return;
             } else if (q.phase == 1) {
                 if (!fc2(q, p.part2 + (size_t(q.tile) * kMaxParts + q.part) * S::kPart2)) return;
             }
@@ -636,7 +669,37 @@ struct Drain {
     }
 };
 
-// Sums over the parts of a tile; fc1: the activation, laid out as fc2's second operand; fc2: the output.
+// Counts the pieces in whose sums are written, and passes those on that complete a tile of fc1 or a group of parts of fc2. A counter takes
+// some trips through L2 (2-5 thousand cycles while the weights stream), which nobody else has to wait for.
+__device__ __forceinline__ void count_pieces(const Params& p, Tail& st) {
+    int passed = 0;
+    for (int n = 0;; ++n) {
+        const int slot = n % kJobs;
+        if (!ptx::mbar_wait(&st.job_full[slot], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
+        const int code = *const_cast<volatile int*>(&st.job[slot]);
+        const Piece q = piece_at(p, st, code);
+        bool last = true;
+        if (q.phase == 0 && q.part >= 0 && st.split1 > 1) {
+            last = streamk::atomic_add_acq_rel_gpu(&p.counters[4 + p.max_hit + q.tile], 1) == st.split1 - 1;
+        } else if (q.phase == 1) {
+            const int group = q.part / kGroup, in_group = min(kGroup, st.parts2 - group * kGroup);
+            int* counters = p.counters + 4 + p.max_hit + p.max_hit * p.tiles1;
+            if (in_group > 1) last = streamk::atomic_add_acq_rel_gpu(&counters[q.tile * kGroups + group], 1) == in_group - 1;
+        }
+        if (last) {  // at most kJobs of them are under way, each with its slot of `job`
+            *const_cast<volatile int*>(&st.last_job[passed % kJobs]) = code * kJobs + slot;
+            ptx::mbar_arrive(&st.last_full[passed % kJobs]);
+            ++passed;
+        } else {
+            for (int i = 0; i < 4; ++i) ptx::mbar_arrive(&st.job_empty[slot]);
+        }
+        if (q.phase == 2) return;
+    }
+}
+
+// Sums over the parts of a tile; fc1: the activation, laid out as fc2's second operand; fc2: the output. Eight tokens at a time in a loop:
+// unrolled over 32 tokens, of which a tile has two or three, this was 77 KB of code, whose fetches through a busy L2 took up to 69000 cycles
+// a tile.
 template <bool kFp8, int kTp>
 struct Finish {
     using S = Shape<kFp8, kTp>;
@@ -651,16 +714,6 @@ struct Finish {
         if (lane == 0) ptx::mbar_arrive(&st.meet);
         return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
     }
-    // Counts a part in (all of it is written, and seen by the counting thread): 1 where it is the last of `parts`, 0 where not, -1 where a
-    // warp has given up.
-    __device__ __forceinline__ int count_in(int* counter, int parts) {
-        if (parts == 1) return 1;
-        if (warp == 0 && lane == 0) st.last = streamk::atomic_add_acq_rel_gpu(counter, 1) == parts - 1;
-        if (!meet()) return -1;
-        const int last = *const_cast<volatile int*>(&st.last);
-        if (!meet()) return -1;  // all have read it
-        return last;
-    }
 
     // Weight of token t for the expert e (routed ids only), by all lanes together.
     __device__ __forceinline__ float weight_of(int t, int e) const {
@@ -669,115 +722,127 @@ struct Finish {
         return who == 0 ? 1.0f : st.topk_weight[t][__ffs(who) - 1];  // shared experts are not in the list
     }
 
-    // sum[t] of parts first, first + 1, ..., `parts` of them, over the tokens of `mask`
-    __device__ __forceinline__ void add_parts(const float* part, int parts, size_t stride, uint32_t mask, float (&sum)[kTp]) const {
+    // sum of `parts` parts in their order for tokens t0 .. t0 + 7, those of `mask8`; all loads of kAtOnce parts before the first use
+    template <int kAtOnce>
+    __device__ __forceinline__ void add_parts(const float* part, int parts, size_t stride, int t0, uint32_t mask8, float (&sum)[8]) const {
 #pragma unroll
-        for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
-#pragma unroll 2
-        for (int i = 0; i < parts; ++i) {
-            float v[kTp];  // all loads before the first use
+        for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+        float4 v[kAtOnce][2];
 #pragma unroll
-            for (int t = 0; t < kTp; ++t) v[t] = (mask >> t) & 1u ? streamk::ld_partial(part + i * stride + t * kRows + row) : 0.0f;
+        for (int o = 0; o < kAtOnce; ++o)
 #pragma unroll
-            for (int t = 0; t < kTp; ++t) sum[t] += v[t];
-        }
+            for (int h = 0; h < 2; ++h)
+                v[o][h] = o < parts && ((mask8 >> (4 * h)) & 15u) != 0 ? ld_partial4(part + o * stride + (t0 + 4 * h) * kRows + row * 4)
+                                                                        : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int o = 0; o < kAtOnce; ++o)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                sum[4 * h] += v[o][h].x, sum[4 * h + 1] += v[o][h].y;
+                sum[4 * h + 2] += v[o][h].z, sum[4 * h + 3] += v[o][h].w;
+            }
     }
 
     __device__ __forceinline__ bool fc1(const Piece& q, const float* part) {
-        const int now = count_in(&p.counters[4 + p.max_hit + q.tile], st.split1);
-        if (now <= 0) return now == 0;
+        const int parts = q.part < 0 ? 1 : st.split1;
         const int j = q.tile / p.tiles1, tile = q.tile - j * p.tiles1, e = st.hit[j];
-        const uint32_t mask = st.hit_mask[j];
-        float g[kTp], v[kTp];
-        if (st.split1 > 1) part -= q.part * S::kPart1;
-        add_parts(part, st.split1, S::kPart1, mask, g);
-        add_parts(part + kTp * kRows, st.split1, S::kPart1, mask, v);
+        if (q.part > 0) part -= q.part * S::kPart1;
         const bool inside = tile * kRows + row < p.I;
         uint8_t* rec = p.aq + (size_t(j) * p.pairs2 + (kFp8 ? tile >> 1 : tile)) * p.rec2;
+#pragma unroll 1
+        for (int t0 = 0; t0 < kTp; t0 += 8) {
+            const uint32_t mask8 = (st.hit_mask[j] >> t0) & 255u;  // the same for all threads
+            if (mask8 == 0) continue;
+            float g[8], v[8];
+            add_parts<kMaxSplit1>(part, parts, S::kPart1, t0, mask8, g);
+            add_parts<kMaxSplit1>(part + kTp * kRows, parts, S::kPart1, t0, mask8, v);
 #pragma unroll
-        for (int t = 0; t < kTp; ++t)
-            if ((mask >> t) & 1u) {              // the same for all threads
-                const float w = weight_of(t, e);  // all lanes, also those of rows past I
-                g[t] = inside ? w * (g[t] / (1.0f + expf(-g[t])) * v[t]) : 0.0f;
+            for (int i = 0; i < 8; ++i)
+                if ((mask8 >> i) & 1u) {
+                    const float w = weight_of(t0 + i, e);  // all lanes, also those of rows past I
+                    g[i] = inside ? w * (silu_approx(g[i]) * v[i]) : 0.0f;
+                    if constexpr (kFp8) {
+                        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(g[i]) & 0x7fffffffu);
+                        if (lane == 0) st.amax[warp][t0 + i] = most;
+                    }
+                }
+            if constexpr (kFp8) {
+                if (!meet()) return false;
+                uint8_t* data = rec + (tile & 1) * S::kN2 * kKBytes;
+                float* scales = reinterpret_cast<float*>(rec + 2 * S::kN2 * kKBytes) + (tile & 1) * kTp;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((mask8 >> i) & 1u) {
+                        const int t = t0 + i;
+                        float inv;
+                        const float s = split_scale(max(max(st.amax[0][t], st.amax[1][t]), max(st.amax[2][t], st.amax[3][t])), &inv);
+                        uint32_t hi, lo;
+                        split_e4m3x2(g[i] * inv, 0.0f, &hi, &lo);
+                        data[swizzled(t, row)] = uint8_t(hi);
+                        data[swizzled(kTp + t, row)] = uint8_t(lo);
+                        if (row == 0) scales[t] = s;
+                    }
+            } else {
+                uint8_t* data = rec + (row >> 6) * S::kN2 * kKBytes;
+                const int byte = (row & 63) * 2;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if ((mask8 >> i) & 1u) {
+                        const uint32_t hi = f2bf_bits(g[i]);
+                        const float rest = g[i] - __uint_as_float(hi << 16);
+                        // an infinite value has no rest
+                        const uint32_t lo = (hi & 0x7fffu) < 0x7f80u ? f2bf_bits(rest) : 0u;
+                        *reinterpret_cast<uint16_t*>(data + swizzled(t0 + i, byte)) = uint16_t(hi);
+                        *reinterpret_cast<uint16_t*>(data + swizzled(kTp + t0 + i, byte)) = uint16_t(lo);
+                    }
             }
-        if constexpr (kFp8) {
-            const int half = tile & 1;
-#pragma unroll
-            for (int t = 0; t < kTp; ++t)
-                if ((mask >> t) & 1u) {
-                    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(g[t]) & 0x7fffffffu);
-                    if (lane == 0) st.amax[warp][t] = most;
-                }
-            if (!meet()) return false;
-            uint8_t* data = rec + half * S::kN2 * kKBytes;
-            float* scales = reinterpret_cast<float*>(rec + 2 * S::kN2 * kKBytes) + half * kTp;
-#pragma unroll
-            for (int t = 0; t < kTp; ++t)
-                if ((mask >> t) & 1u) {
-                    float inv;
-                    const float s = split_scale(max(max(st.amax[0][t], st.amax[1][t]), max(st.amax[2][t], st.amax[3][t])), &inv);
-                    uint32_t hi, lo;
-                    split_e4m3x2(g[t] * inv, 0.0f, &hi, &lo);
-                    data[swizzled(t, row)] = uint8_t(hi);
-                    data[swizzled(kTp + t, row)] = uint8_t(lo);
-                    if (row == 0) scales[t] = s;
-                }
-        } else {
-            uint8_t* data = rec + (row >> 6) * S::kN2 * kKBytes;
-            const int byte = (row & 63) * 2;
-#pragma unroll
-            for (int t = 0; t < kTp; ++t)
-                if ((mask >> t) & 1u) {
-                    const uint32_t hi = f2bf_bits(g[t]);
-                    const float rest = g[t] - __uint_as_float(hi << 16);
-                    // an infinite value has no rest
-                    const uint32_t lo = (hi & 0x7fffu) < 0x7f80u ? f2bf_bits(rest) : 0u;
-                    *reinterpret_cast<uint16_t*>(data + swizzled(t, byte)) = uint16_t(hi);
-                    *reinterpret_cast<uint16_t*>(data + swizzled(kTp + t, byte)) = uint16_t(lo);
-                }
         }
         asm volatile("fence.proxy.async;" ::: "memory");  // to the bulk copies of other blocks
         if (!meet()) return false;
-        if (warp == 0 && lane == 0) streamk::atomic_add_acq_rel_gpu(&p.counters[4 + j], 1);
+        if (warp == 0 && lane == 0) streamk::red_add_release_gpu(&p.counters[4 + j], 1);
         return true;
     }
 
     __device__ __forceinline__ bool fc2(const Piece& q) {
         const int group = q.part / kGroup, groups = (st.parts2 + kGroup - 1) / kGroup, in_group = min(kGroup, st.parts2 - group * kGroup);
-        const uint32_t all = p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u;
-        int* counters = p.counters + 4 + p.max_hit + p.max_hit * p.tiles1;
-        int now = count_in(&counters[q.tile * kGroups + group], in_group);
-        if (now <= 0) return now == 0;
-        float sum[kTp];
-        add_parts(p.part2 + (size_t(q.tile) * kMaxParts + group * kGroup) * S::kPart2, in_group, S::kPart2, all, sum);
-        if (groups > 1) {
-            float* to = p.group2 + size_t(q.tile) * kGroups * S::kPart2;
-#pragma unroll
-            for (int t = 0; t < kTp; ++t)
-                if (t < p.T) to[group * S::kPart2 + t * kRows + row] = sum[t];
-            if (!meet()) return false;
-            now = count_in(&counters[p.tiles2 * kGroups + q.tile], groups);
-            if (now <= 0) return now == 0;
-            add_parts(to, groups, S::kPart2, all, sum);
-        }
+        const uint32_t all = all_tokens(p), bad = st.bad_tokens;
         const int h = q.tile * kRows + row;
-        if (h < p.H) {
-            const uint32_t bad = st.bad_tokens;
+        float* group_sums = p.group2 + size_t(q.tile) * kGroups * S::kPart2;
+        auto put_out = [&](int t0, const float (&sum)[8]) {
+            if (h < p.H)
 #pragma unroll
-            for (int t = 0; t < kTp; ++t)
-                if (t < p.T) p.out[size_t(t) * p.H + h] = __float2bfloat16_rn((bad >> t) & 1u ? __uint_as_float(0x7fffffffu) : sum[t]);
+                for (int i = 0; i < 8; ++i)
+                    if (t0 + i < p.T) p.out[size_t(t0 + i) * p.H + h] = __float2bfloat16_rn((bad >> (t0 + i)) & 1u ? __uint_as_float(0x7fffffffu) : sum[i]);
+        };
+#pragma unroll 1
+        for (int t0 = 0; t0 < p.T; t0 += 8) {
+            float sum[8];
+            add_parts<kGroup>(p.part2 + (size_t(q.tile) * kMaxParts + group * kGroup) * S::kPart2, in_group, S::kPart2, t0, (all >> t0) & 255u, sum);
+            if (groups == 1) put_out(t0, sum);
+            else put_sums<8>(group_sums + group * S::kPart2 + t0 * kRows, row, 255u, sum);
+        }
+        if (groups == 1) return true;
+        if (!meet()) return false;
+        if (warp == 0 && lane == 0)
+            st.last = streamk::atomic_add_acq_rel_gpu(p.counters + 4 + p.max_hit + p.max_hit * p.tiles1 + p.tiles2 * kGroups + q.tile, 1) == groups - 1;
+        if (!meet()) return false;
+        if (*const_cast<volatile int*>(&st.last) == 0) return true;  // read by all before they meet for the next job's
+#pragma unroll 1
+        for (int t0 = 0; t0 < p.T; t0 += 8) {
+            float sum[8];
+            add_parts<kGroups>(group_sums, groups, S::kPart2, t0, (all >> t0) & 255u, sum);
+            put_out(t0, sum);
         }
         return true;
     }
 
     __device__ __forceinline__ void run() {
         for (int n = 0;; ++n) {
-            const int slot = n % kJobs;
-            if (!ptx::mbar_wait_warp(&st.job_full[slot], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
-            const int code = *const_cast<volatile int*>(&st.job[slot]);
-            const Piece q = piece_at(p, st, code);
+            if (!ptx::mbar_wait_warp(&st.last_full[n % kJobs], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
+            const int note = *const_cast<volatile int*>(&st.last_job[n % kJobs]), slot = note % kJobs;
+            const Piece q = piece_at(p, st, note / kJobs);
             if (q.phase == 2) return;
-            if (!(q.phase == 0 ? fc1(q, p.part1 + (st.split1 > 1 ? size_t(code) : size_t(blockIdx.x) * kJobs + slot) * S::kPart1) : fc2(q))) return;
+            if (!(q.phase == 0 ? fc1(q, place1<S::kPart1>(p, st, q, slot)) : fc2(q))) return;
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&st.job_empty[slot]);
         }
@@ -785,24 +850,24 @@ struct Finish {
 };
 
 // Chosen experts of every token into shared memory, and the list of experts that any token chose, shared ones at its end.
-__device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int lane) {
-    for (int i = threadIdx.x; i < p.E; i += kThreads) st.mask[i] = 0;
-    if (threadIdx.x == 0) st.bad_tokens = 0;
-    __syncthreads();
+template <int kPerLane>
+__device__ __forceinline__ void choose_topk(const Params& p, Tail& st, int warp, int lane) {
     for (int t = warp; t < p.T; t += kThreads / 32) {
-        const float* row = p.logits + size_t(t) * p.E;
         int* index = st.topk_index[t];
         float* weight = st.topk_weight[t];
-        if (p.E <= 32) route::topk_of_token<1>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
-        else if (p.E <= 128) route::topk_of_token<4>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
-        else if (p.E <= 256) route::topk_of_token<8>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
-        else route::topk_of_token<32>(row, p.E, p.k, p.k, p.scoring, lane, index, weight);
+        route::topk_of_token<kPerLane>(p.logits + size_t(t) * p.E, p.E, p.k, p.k, p.scoring, lane, index, weight);
         __syncwarp();
         if (lane < p.k) {
             if (index[lane] < p.E) atomicOr(&st.mask[index[lane]], 1u << t);
             if (isnan(weight[lane])) atomicOr(&st.bad_tokens, 1u << t);
         }
     }
+}
+__device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int lane) {
+    if (p.E <= 32) choose_topk<1>(p, st, warp, lane);
+    else if (p.E <= 128) choose_topk<4>(p, st, warp, lane);
+    else if (p.E <= 256) choose_topk<8>(p, st, warp, lane);
+    else choose_topk<32>(p, st, warp, lane);
     __syncthreads();
     if (warp == 0) {
         int count = 0;
@@ -818,12 +883,9 @@ __device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int 
         }
         for (int i = lane; i < p.n_shared; i += 32) {
             st.hit[count + i] = uint16_t(p.E + i);
-            st.hit_mask[count + i] = p.T == 32 ? 0xffffffffu : (1u << p.T) - 1u;
+            st.hit_mask[count + i] = all_tokens(p);
         }
-        if (lane == 0) {
-            st.n_hit = count + p.n_shared;
-            plan_pieces(p, st);
-        }
+        plan_pieces(p, st, count + p.n_shared, lane);
     }
 }
 
@@ -852,7 +914,8 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         }
         for (int i = 0; i < kJobs; ++i) {
             ptx::mbar_init(&st.job_full[i], 4);
-            ptx::mbar_init(&st.job_empty[i], 4);
+            ptx::mbar_init(&st.job_empty[i], 4);   // the finishing warps, or the counting thread for them
+            ptx::mbar_init(&st.last_full[i], 1);
         }
         ptx::mbar_init(&st.meet, 4);
         st.abort_flag = 0;
@@ -862,6 +925,11 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         ptx::tmem_alloc(&st.tmem_base, S::kTmemCols);
         ptx::tmem_relinquish();
     }
+    for (int i = threadIdx.x; i < p.E; i += kThreads) st.mask[i] = 0;
+    if (threadIdx.x == 0) st.bad_tokens = 0;
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
     if (threadIdx.x == 32 * 2) ptx::prefetch_tensormap(&map_b);
     if (threadIdx.x == 32 * 3) ptx::prefetch_tensormap(&map_b1);
     pdl_wait();
@@ -869,9 +937,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
     if (threadIdx.x == 0) claim = atomicAdd(&p.counters[0], 1);
     claim = __shfl_sync(0xffffffffu, claim, 0);
     choose(p, st, warp, lane);
-    ptx::tc_fence_before();
     __syncthreads();
-    ptx::tc_fence_after();
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
 
     if (st.n_hit == 0) {  // no token has an expert
@@ -885,6 +951,9 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         __syncwarp();
     } else if (warp == 2) {
         if (ptx::elect_one()) load_tokens<kFp8, kTp>(p, st, ring);
+        __syncwarp();
+    } else if (warp == 3) {
+        if (ptx::elect_one()) count_pieces(p, st);
         __syncwarp();
     } else if (warp >= 8) {
         Finish<kFp8, kTp> f{p, st, warp - 8, lane, (warp - 8) * 32 + lane};
@@ -929,8 +998,7 @@ static Layout plan(Params* p, bool fp8) {
     L.logits = add(size_t(p->T) * p->E * sizeof(float));
     L.xq = add(size_t(p->kb1) * p->rec1);
     L.aq = add(size_t(p->max_hit) * p->pairs2 * p->rec2);
-    // fc1's parts: fewer than 6 per block where tiles are split (up to 3 per block round up to twice as many), else kJobs places per block
-    L.part1 = add(size_t(p->blocks) * 6 * 2 * tp * kRows * sizeof(float));
+    L.part1 = add(size_t(p->blocks) * (kJobs + kMaxSplit1) * 2 * tp * kRows * sizeof(float));
     L.part2 = add(size_t(p->tiles2) * kMaxParts * tp * kRows * sizeof(float));
     L.group2 = add(size_t(p->tiles2) * kGroups * tp * kRows * sizeof(float));
     L.total = off;

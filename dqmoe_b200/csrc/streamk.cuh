@@ -26,6 +26,9 @@ __device__ __forceinline__ int atomic_add_acq_rel_gpu(int* p, int v) {
     asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
     return old;
 }
+__device__ __forceinline__ void red_add_release_gpu(int* p, int v) {
+    asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
 // Partial sums pass between blocks through L2 only.
 __device__ __forceinline__ float ld_partial(const float* p) {
     float v;
