@@ -197,7 +197,6 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             for (int c = 0; c < kShrinkTok; c += 32) {
                 float v[32];
                 ptx::tmem_read<32>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
-                ptx::tmem_landed<32>(v);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
                     if (mine < cap && st.place[c + i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
@@ -420,7 +419,6 @@ struct Epilogue {
             for (int c = half; c * kChunk < cols; c += 2) {
                 float v[kChunk];
                 ptx::tmem_read<kChunk>(tmem + buf * p.tok + c * kChunk, v);
-                ptx::tmem_landed<kChunk>(v);
                 for (; e < mixed1 && int(l.mixed[e].y & 0xff) <= (c | 1); ++e) {  // this chunk's and its neighbour's, in turn
                     if (int(l.mixed[e].y & 0xff) != c) continue;
                     const int slot = slot_it % p.slots;
@@ -428,7 +426,6 @@ struct Epilogue {
                     ptx::tc_fence_after();
                     float d[kChunk];
                     ptx::tmem_read<kChunk>(tmem + 2 * p.tok + (half * p.slots + slot) * kChunk, d);
-                    ptx::tmem_landed<kChunk>(d);
                     ptx::tc_fence_before();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(&st.slot_empty[half][slot]);

@@ -557,9 +557,7 @@ struct Drain {
         for (int c = 0; c < kTp; c += kCols) {
             if (((mask >> c) & ((1u << kCols) - 1u)) == 0) continue;
             float hi[kCols], lo[kCols];
-            ptx::tmem_read<kCols>(taddr + c, hi);
-            ptx::tmem_read<kCols>(taddr + kTp + c, lo);
-            ptx::tmem_landed<kCols>(hi, lo);
+            ptx::tmem_read2<kCols>(taddr + c, taddr + kTp + c, hi, lo);
 #pragma unroll
             for (int t = 0; t < kCols; t += 4) {
                 const float4 sc = *reinterpret_cast<const float4*>(token_scale + c + t);
@@ -594,9 +592,7 @@ struct Drain {
             }
         } else {
             if (!acquire()) return false;
-            ptx::tmem_read<kTp>(buffer(), g);
-            ptx::tmem_read<kTp>(buffer() + S::kN1, v);
-            ptx::tmem_landed<kTp>(g, v);
+            ptx::tmem_read2<kTp>(buffer(), buffer() + S::kN1, g, v);
             release(false);
         }
         put_sums<kTp>(to, row, mask, g);
@@ -611,17 +607,16 @@ struct Drain {
 #pragma unroll
         for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
         if constexpr (kFp8) {
-            float scale[2];
-            auto scales_of = [&](int u) {
-                const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
-                scale[0] = weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb);
-                scale[1] = kb + 1 < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb + 1) : 0.0f;
+            auto scale_of = [&](int u, int half) {
+                const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2 + half;
+                return kb < kb2 ? weight_scale(p.b1_scale, p.mode, st.hit[j], p.H, h, kb2, kb) : 0.0f;
             };
-            if (q.lo < q.hi) scales_of(q.lo);
+            float next0 = 0.0f, next1 = 0.0f;
+            if (q.lo < q.hi) next0 = scale_of(q.lo, 0), next1 = scale_of(q.lo, 1);
             for (int u = q.lo; u < q.hi; ++u, ++it) {
                 const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
-                const float s0 = scale[0], s1 = scale[1];
-                if (u + 1 < q.hi) scales_of(u + 1);
+                const float s0 = next0, s1 = next1;
+                if (u + 1 < q.hi) next0 = scale_of(u + 1, 0), next1 = scale_of(u + 1, 1);
                 const uint32_t mask = st.hit_mask[j];
                 if (!stage_full() || !acquire()) return false;
                 const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + 2 * S::kN2 * kKBytes);
@@ -635,9 +630,7 @@ struct Drain {
                 u = min(q.hi, (j + 1) * p.pairs2);
                 if (!acquire()) return false;
                 float hi[kTp], lo[kTp];
-                ptx::tmem_read<kTp>(buffer(), hi);
-                ptx::tmem_read<kTp>(buffer() + kTp, lo);
-                ptx::tmem_landed<kTp>(hi, lo);
+                ptx::tmem_read2<kTp>(buffer(), buffer() + kTp, hi, lo);
                 release(false);
                 const uint32_t mask = st.hit_mask[j];
 #pragma unroll

@@ -496,34 +496,70 @@ __device__ __forceinline__ void tmem_wait_ld2(uint32_t (&a)[32], uint32_t (&b)[3
                  : "memory");
 }
 
-// 32 lanes x kCount consecutive fp32 columns, as floats: thread i of the warp receives the columns of lane i. Valid behind tmem_landed.
+// 32 lanes x kCount consecutive fp32 columns, as floats: thread i of the warp receives the columns of lane i. The loads and their wait are one
+// statement. The hardware writes the registers at some time until the wait: had the compiler them as results before it, it could move or
+// spill them, and give the registers to something else, while they are still to be written.
 template <int kCount>
 __device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
     static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
-    uint32_t* u = reinterpret_cast<uint32_t*>(r);
-    if constexpr (kCount == 8) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(taddr) : "memory");
-    } else if constexpr (kCount == 16) {
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
-                       "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]) : "r"(taddr) : "memory");
-    } else {
-        tmem_ld32(taddr, *reinterpret_cast<uint32_t (*)[32]>(&r));
-    }
+    if constexpr (kCount == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7])
+                     : "r"(taddr) : "memory");
+    else if constexpr (kCount == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
+                       "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15])
+                     : "r"(taddr) : "memory");
+    else if constexpr (kCount == 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                     "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+                     "%31}, [%32];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
+                       "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15]), "=&f"(r[16]),
+                       "=&f"(r[17]), "=&f"(r[18]), "=&f"(r[19]), "=&f"(r[20]), "=&f"(r[21]), "=&f"(r[22]), "=&f"(r[23]), "=&f"(r[24]),
+                       "=&f"(r[25]), "=&f"(r[26]), "=&f"(r[27]), "=&f"(r[28]), "=&f"(r[29]), "=&f"(r[30]), "=&f"(r[31])
+                     : "r"(taddr) : "memory");
 }
-// Wait for this thread's outstanding tcgen05.ld; the registers pass through statements behind the wait.
 template <int kCount>
-__device__ __forceinline__ void tmem_landed(float (&a)[kCount], float (&b)[kCount]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i]), "+f"(b[i])::"memory");
-}
-template <int kCount>
-__device__ __forceinline__ void tmem_landed(float (&a)[kCount]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) asm volatile("" : "+f"(a[i])::"memory");
+__device__ __forceinline__ void tmem_read2(uint32_t taddr_a, uint32_t taddr_b, float (&a)[kCount], float (&b)[kCount]) {
+    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
+    if constexpr (kCount == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+                     "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(a[0]), "=&f"(a[1]), "=&f"(a[2]), "=&f"(a[3]), "=&f"(a[4]), "=&f"(a[5]), "=&f"(a[6]), "=&f"(a[7]),
+                       "=&f"(b[0]), "=&f"(b[1]), "=&f"(b[2]), "=&f"(b[3]), "=&f"(b[4]), "=&f"(b[5]), "=&f"(b[6]), "=&f"(b[7])
+                     : "r"(taddr_a), "r"(taddr_b) : "memory");
+    else if constexpr (kCount == 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%32];\n\t"
+                     "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%33];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(a[0]), "=&f"(a[1]), "=&f"(a[2]), "=&f"(a[3]), "=&f"(a[4]), "=&f"(a[5]), "=&f"(a[6]), "=&f"(a[7]), "=&f"(a[8]),
+                       "=&f"(a[9]), "=&f"(a[10]), "=&f"(a[11]), "=&f"(a[12]), "=&f"(a[13]), "=&f"(a[14]), "=&f"(a[15]),
+                       "=&f"(b[0]), "=&f"(b[1]), "=&f"(b[2]), "=&f"(b[3]), "=&f"(b[4]), "=&f"(b[5]), "=&f"(b[6]), "=&f"(b[7]), "=&f"(b[8]),
+                       "=&f"(b[9]), "=&f"(b[10]), "=&f"(b[11]), "=&f"(b[12]), "=&f"(b[13]), "=&f"(b[14]), "=&f"(b[15])
+                     : "r"(taddr_a), "r"(taddr_b) : "memory");
+    else if constexpr (kCount == 32)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                     "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+                     "%31}, [%64];\n\t"
+                     "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+                     "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,"
+                     "%61,%62,%63}, [%65];\n\t"
+                     "tcgen05.wait::ld.sync.aligned;"
+                     : "=&f"(a[0]), "=&f"(a[1]), "=&f"(a[2]), "=&f"(a[3]), "=&f"(a[4]), "=&f"(a[5]), "=&f"(a[6]), "=&f"(a[7]), "=&f"(a[8]),
+                       "=&f"(a[9]), "=&f"(a[10]), "=&f"(a[11]), "=&f"(a[12]), "=&f"(a[13]), "=&f"(a[14]), "=&f"(a[15]), "=&f"(a[16]),
+                       "=&f"(a[17]), "=&f"(a[18]), "=&f"(a[19]), "=&f"(a[20]), "=&f"(a[21]), "=&f"(a[22]), "=&f"(a[23]), "=&f"(a[24]),
+                       "=&f"(a[25]), "=&f"(a[26]), "=&f"(a[27]), "=&f"(a[28]), "=&f"(a[29]), "=&f"(a[30]), "=&f"(a[31]),
+                       "=&f"(b[0]), "=&f"(b[1]), "=&f"(b[2]), "=&f"(b[3]), "=&f"(b[4]), "=&f"(b[5]), "=&f"(b[6]), "=&f"(b[7]), "=&f"(b[8]),
+                       "=&f"(b[9]), "=&f"(b[10]), "=&f"(b[11]), "=&f"(b[12]), "=&f"(b[13]), "=&f"(b[14]), "=&f"(b[15]), "=&f"(b[16]),
+                       "=&f"(b[17]), "=&f"(b[18]), "=&f"(b[19]), "=&f"(b[20]), "=&f"(b[21]), "=&f"(b[22]), "=&f"(b[23]), "=&f"(b[24]),
+                       "=&f"(b[25]), "=&f"(b[26]), "=&f"(b[27]), "=&f"(b[28]), "=&f"(b[29]), "=&f"(b[30]), "=&f"(b[31])
+                     : "r"(taddr_a), "r"(taddr_b) : "memory");
 }
 
 // 16 lanes x 32 fp32 columns as matrix fragments (the lower or the upper half of the warp's lane quarter, by the lane field of

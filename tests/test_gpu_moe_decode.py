@@ -243,6 +243,18 @@ def test_a_step_after_a_step():
         check(y, *reference({**a, "x": x}))
 
 
+@pytest.mark.parametrize("T", [1, 8, 16, 32])
+@pytest.mark.parametrize("mode", list(MODES))
+def test_many_calls_without_waiting(mode, T):
+    """The next call's blocks take over an SM as soon as this one's leave it."""
+    a = make(37, mode, T, 2048, 768, 128, 8)
+    want = ops.moe_decode(**a)
+    torch.cuda.synchronize()
+    outs = [ops.moe_decode(**a) for _ in range(40)]
+    assert ops.device_status() == 0
+    assert all(torch.equal(o, want) for o in outs)
+
+
 def test_empty_batch():
     a = make(31, "block", 3, 256, 128, 4, 2)
     out = ops.moe_decode(**{**a, "x": a["x"][:0]})
