@@ -15,8 +15,6 @@
 // this kernel added z B^T in the epilogue's threads, each with its row of B: bound by L1, whose lines hold one row of B each, and on the
 // last block of a tile alone. 64 rows of 64 adapters, K 4096, N 6144, R 16: 70 us; 333 rows of 40 requests, 2880 x 2880, R 64: 489 us.)
 // The list of these products is made from the ids by a warp of each block, and divided among the parts of a tile like its K.
-// shrink takes 64 rows of x at a time against all adapters among them, several adapters' A stacked on M = 128, and keeps from the product
-// what belongs together.
 //
 // project starts while shrink runs: it reads only x and W until a tile's K is through. That is sound because shrink lets it start
 // behind its own wait for the kernels before, which wrote those. No counterpart in the reference.
@@ -42,11 +40,23 @@ constexpr int kStatusShrink = 311, kStatusProject = 312;
 
 constexpr int kShrinkTok = 64;                  // rows of x per tile
 constexpr int kShrinkThreads = 256;             // warp 0 TMA, warp 1 MMA, warps 4..7 epilogue
-constexpr int kShrinkStage = kABytes + kShrinkTok * kKBytes;
-constexpr int kShrinkStages = 4;
+constexpr int kShrinkXBytes = kShrinkTok * kKBytes;
+constexpr int kShrinkStages = 8;                // at most
 constexpr int kMaxSplit = 8;                    // blocks of a cluster: slices of K
 
+__device__ __forceinline__ uint16_t to_bits(float f, bool half) {
+    return half ? __half_as_ushort(__float2half_rn(f)) : uint16_t(f2bf_bits(f));
+}
+template <bool kHalf>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if constexpr (kHalf) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    else return make_float2(bf16_lo(w), bf16_hi(w));
+}
+
 struct ShrinkParams {
+    const uint16_t* x;      // rows form
+    int64_t ldx;
+    const uint16_t* lora_a; // [L, R, K]
     const int* ids;
     const float* scale;     // [L] or null
     uint16_t* z;            // [T, R] in the operands' type
@@ -55,9 +65,88 @@ struct ShrinkParams {
     int n_counters;
     int T, K, L, R;
     int half;               // operands fp16, else bf16
+    int cap;                // tile form: adapters of a product,
+    int stages;             // stages of the ring,
     int slots;              // clusters that share a tile's groups of adapters
     int* status;
 };
+
+// A row's z in the operands' type, by a warp whose lanes hold four values each (lane * 4 < R).
+__device__ __forceinline__ void put_z(const ShrinkParams& p, int64_t t, int id, float4 v, int lane) {
+    const float scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+    v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
+    if (p.half) {
+        const float most = warp_max(lane * 4 < p.R ? fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) : 0.0f);
+        float up = 1.0f, down = 1.0f;
+        if (most > 32768.0f && most <= 3.402823466e38f) {  // 2^(exponent - 14): below 2^15 then
+            const int e = int(__float_as_uint(most) >> 23) - 127 - 14;
+            up = __uint_as_float(uint32_t(127 + e) << 23), down = __uint_as_float(uint32_t(127 - e) << 23);
+        }
+        v.x *= down, v.y *= down, v.z *= down, v.w *= down;
+        if (lane == 0) p.z_scale[t] = up;
+    }
+    if (lane * 4 < p.R)
+        *reinterpret_cast<uint2*>(p.z + t * p.R + lane * 4) =
+            make_uint2(to_bits(v.x, p.half) | (uint32_t(to_bits(v.y, p.half)) << 16), to_bits(v.z, p.half) | (uint32_t(to_bits(v.w, p.half)) << 16));
+}
+
+// Rows form, for few rows: a block per row and 16 ranks (fp16: all ranks, whose common power of two it needs), a warp per rank. A warp has
+// all its loads of A on their way at once, before project, which starts beside it, fills the path to memory.
+constexpr int kRowWarps = 16;
+constexpr int kRowValues = 4096;                // of K at a time: 16 loads of 16 bytes per lane
+template <bool kHalf>
+__global__ void __launch_bounds__(kRowWarps * 32) lora_shrink_rows_kernel(const __grid_constant__ ShrinkParams p) {
+    pdl_wait();    // x, ids and the workspace
+    pdl_launch();  // project: what is there before this kernel, it may read from now on
+    __shared__ alignas(16) uint16_t s_x[kRowValues];
+    __shared__ alignas(16) float s_z[kMaxRank];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * kRowWarps * 32 + threadIdx.x; i < p.n_counters; i += gridDim.x * gridDim.y * kRowWarps * 32)
+        p.counters[i] = 0;
+    const int t = blockIdx.x, id = p.ids[t];
+    if (id < 0 || id >= p.L) return;
+    const int first = blockIdx.y * kRowWarps, ranks = gridDim.y > 1 ? min(p.R, first + kRowWarps) : p.R;
+    for (int r0 = first; r0 < ranks; r0 += kRowWarps) {
+        const int r = r0 + warp;
+        float sum = 0.0f;
+        for (int k0 = 0; k0 < p.K; k0 += kRowValues) {
+            const uint16_t* a = p.lora_a + (size_t(id) * p.R + r) * p.K + k0 + lane * 8;
+            uint4 w[kRowValues / 256];
+#pragma unroll
+            for (int i = 0; i < kRowValues / 256; ++i)
+                w[i] = r < ranks && k0 + i * 256 + lane * 8 < p.K ? *reinterpret_cast<const uint4*>(a + i * 256) : make_uint4(0, 0, 0, 0);
+            const int k = k0 + threadIdx.x * 8;
+            const uint4 x = k < p.K ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+            __syncthreads();  // the values before have been read
+            *reinterpret_cast<uint4*>(s_x + threadIdx.x * 8) = x;
+            __syncthreads();
+            static_assert(kRowValues == kRowWarps * 32 * 8, "a thread's share of x");
+#pragma unroll
+            for (int i = 0; i < kRowValues / 256; ++i) {
+                if (k0 + i * 256 + lane * 8 >= p.K) continue;  // past K, where x may not be finite in the place of nothing
+                const uint4 v = *reinterpret_cast<const uint4*>(s_x + i * 256 + lane * 8);
+                const uint32_t xs[4] = {v.x, v.y, v.z, v.w}, ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = unpack2<kHalf>(xs[j]), g = unpack2<kHalf>(ws[j]);
+                    sum = fmaf(f.x, g.x, sum);
+                    sum = fmaf(f.y, g.y, sum);
+                }
+            }
+        }
+        sum = warp_sum(sum);
+        if (lane == 0 && r < ranks) s_z[r] = sum;
+    }
+    __syncthreads();
+    if (warp > 0) return;
+    if (gridDim.y == 1) {
+        put_z(p, t, id, lane * 4 < p.R ? *reinterpret_cast<const float4*>(s_z + lane * 4) : make_float4(0, 0, 0, 0), lane);
+    } else if (lane < ranks - first) {  // bf16: no power of two
+        const float scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+        p.z[int64_t(t) * p.R + first + lane] = to_bits(s_z[first + lane] * scale, false);
+    }
+}
+
 struct alignas(16) ShrinkTail {
     uint64_t full[kShrinkStages], empty[kShrinkStages], tmem_full[2], tmem_empty[2];
     uint32_t tmem_base;
@@ -68,7 +157,12 @@ struct alignas(16) ShrinkTail {
     int adapter[kShrinkTok];                    // the tile's adapters in the order of their first rows
     uint32_t firsts[2];
 };
-static size_t shrink_smem(int R) { return 1024 + size_t(kShrinkStages) * kShrinkStage + size_t(kShrinkTok) * R * sizeof(float) + sizeof(ShrinkTail); }
+// x first, so that an MMA's 128 rows of A, of which a stage has cap * R, end inside shared memory: behind the last stage lie the sums and what
+// is left of an A tile.
+static size_t shrink_smem(int R, int cap, int stages) {
+    const size_t behind = size_t(kShrinkTok) * R * sizeof(float) + sizeof(ShrinkTail), tile = kABytes - size_t(cap) * R * kKBytes;
+    return 1024 + size_t(stages) * (kShrinkXBytes + cap * R * kKBytes) + (behind > tile ? behind : tile);
+}
 
 __device__ __forceinline__ uint32_t cluster_nctarank() {
     uint32_t n;
@@ -76,19 +170,18 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
     return n;
 }
 
-__device__ __forceinline__ uint16_t to_bits(float f, bool half) {
-    return half ? __half_as_ushort(__float2half_rn(f)) : uint16_t(f2bf_bits(f));
-}
-
+// Tile form: 64 rows of x against all adapters among them, several adapters' A stacked on M = 128; of the product is kept what belongs together.
+// K over a cluster of blocks where there are few tiles.
 __global__ void __launch_bounds__(kShrinkThreads)
-lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ShrinkParams p) {
+lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ShrinkParams p) {
+    const int stage = kShrinkXBytes + p.cap * p.R * kKBytes;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* part = reinterpret_cast<float*>(ring + kShrinkStages * kShrinkStage);  // [64][R] of this block's slice of K
+    float* part = reinterpret_cast<float*>(ring + p.stages * stage);  // [64][R] of this block's slice of K
     ShrinkTail& st = *reinterpret_cast<ShrinkTail*>(part + kShrinkTok * p.R);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kShrinkStages; ++i) {
+        for (int i = 0; i < p.stages; ++i) {
             ptx::mbar_init(&st.full[i], 1);
             ptx::mbar_init(&st.empty[i], 1);
         }
@@ -137,7 +230,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
     }
     __syncthreads();
 
-    const int cap = kRows / p.R, groups = (st.distinct + cap - 1) / cap;  // adapters of a product, products of the tile
+    const int cap = p.cap, groups = (st.distinct + cap - 1) / cap;  // adapters of a product, products of the tile
     const int kbs = (p.K + kKElems - 1) / kKElems;
     const int kb0 = rank * kbs / split, kb1 = (rank + 1) * kbs / split;
     if (kb0 == kb1)
@@ -149,19 +242,19 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             for (int g = slot; ok && g < groups; g += p.slots) {
                 const int n = min(cap, st.distinct - g * cap);
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % kShrinkStages;
-                    if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / kShrinkStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
-                    uint8_t* a = ring + s * kShrinkStage;
+                    const int s = it % p.stages;
+                    if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+                    uint8_t* a = ring + s * stage + kShrinkXBytes;
                     ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(n * p.R + kShrinkTok) * kKBytes);
-                    ptx::tma_load_2d(a + kABytes, &map_x, kb * kKElems, tile * kShrinkTok, &st.full[s]);
+                    ptx::tma_load_2d(ring + s * stage, &map_x, kb * kKElems, tile * kShrinkTok, &st.full[s]);
                     for (int i = 0; i < n; ++i)
                         ptx::tma_load_2d(a + i * p.R * kKBytes, &map_a, kb * kKElems, st.adapter[g * cap + i] * p.R, &st.full[s]);
                 }
             }
             if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
                 const long long t0 = clock64();
-                for (int i = max(0, it - kShrinkStages); i < it; ++i)
-                    while (!ptx::mbar_try_wait(&st.full[i % kShrinkStages], (i / kShrinkStages) & 1) && clock64() - t0 < kWaitLimit) {}
+                for (int i = max(0, it - p.stages); i < it; ++i)
+                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - t0 < kWaitLimit) {}
             }
         }
         __syncwarp();
@@ -173,11 +266,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
             for (int g = slot; ok && g < groups; g += p.slots, ++acc) {
                 if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % kShrinkStages;
-                    if (!(ok = ptx::mbar_wait(&st.full[s], (it / kShrinkStages) & 1, &st.abort_flag, kWaitLimit))) break;
+                    const int s = it % p.stages;
+                    if (!(ok = ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit))) break;
                     ptx::tc_fence_after();
-                    const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * kShrinkStage));
-                    const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * kShrinkStage + kABytes));
+                    const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kShrinkXBytes));
+                    const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         ptx::umma<1>(tmem + (acc & 1) * kShrinkTok, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc,
@@ -194,11 +287,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         for (int g = slot; g < groups; g += p.slots, ++acc) {
             if (!ptx::mbar_wait_warp(&st.tmem_full[acc & 1], (acc >> 1) & 1, &st.abort_flag, kWaitLimit)) break;
             ptx::tc_fence_after();
-            for (int c = 0; c < kShrinkTok; c += 32) {
-                float v[32];
-                ptx::tmem_read<32>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
+            const int rows = min(kShrinkTok, p.T - tile * kShrinkTok);
+#pragma unroll 1
+            for (int c = 0; c < rows; c += 16) {
+                float v[16];
+                ptx::tmem_read<16>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
+                for (int i = 0; i < 16; ++i)
                     if (mine < cap && st.place[c + i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
             }
             ptx::tc_fence_before();
@@ -219,30 +314,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_const
         const int place = st.place[t];
         if (place < 0 || (place / cap) % p.slots != slot) continue;
         float4 sum = make_float4(0, 0, 0, 0);
-        if (lane * 4 < p.R) {
+        if (lane * 4 < p.R)
             for (int c = 0; c < split; ++c) {
                 float4 v;
                 asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                              : "r"(ptx::map_to_cta(part + t * p.R + lane * 4, c)) : "memory");
                 sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
             }
-            const float scale = p.scale != nullptr ? p.scale[st.id[t]] : 1.0f;
-            sum.x *= scale, sum.y *= scale, sum.z *= scale, sum.w *= scale;
-        }
-        const size_t row = size_t(tile) * kShrinkTok + t;
-        if (p.half) {
-            const float most = warp_max(fmaxf(fmaxf(fabsf(sum.x), fabsf(sum.y)), fmaxf(fabsf(sum.z), fabsf(sum.w))));
-            float up = 1.0f, down = 1.0f;
-            if (most > 32768.0f && most <= 3.402823466e38f) {  // 2^(exponent - 14): below 2^15 then
-                const int e = int(__float_as_uint(most) >> 23) - 127 - 14;
-                up = __uint_as_float(uint32_t(127 + e) << 23), down = __uint_as_float(uint32_t(127 - e) << 23);
-            }
-            sum.x *= down, sum.y *= down, sum.z *= down, sum.w *= down;
-            if (lane == 0) p.z_scale[row] = up;
-        }
-        if (lane * 4 < p.R)
-            *reinterpret_cast<uint2*>(p.z + row * p.R + lane * 4) =
-                make_uint2(to_bits(sum.x, p.half) | (uint32_t(to_bits(sum.y, p.half)) << 16), to_bits(sum.z, p.half) | (uint32_t(to_bits(sum.w, p.half)) << 16));
+        put_z(p, int64_t(tile) * kShrinkTok + t, st.id[t], sum, lane);
     }
     __syncthreads();
     ptx::cluster_sync();  // the others read this block's shared memory until here
@@ -257,6 +336,7 @@ constexpr int kRingBytes = 200 * 1024;
 constexpr int kMaxStages = 10;
 constexpr int kChunk = 16;                      // rows of x that are looked at together
 constexpr int kMaxSlots = 8;
+constexpr int kAtOnce = 5;                      // parts of a tile that are loaded at once
 
 struct Params {
     const int* ids;
@@ -273,7 +353,7 @@ struct Params {
     int whole;                // tiles that are not split: block b takes b, b + grid, ...; the others are cut into equal shares
     int shares;               // of the others
     int* counters;            // parts seen of each split tile
-    float* part;              // [shares][2][tok][128]
+    float* part;              // [shares][2] sums of a part of a tile, four rows of x together: [tok / 4][128][4]
     int* status;
 };
 
@@ -292,7 +372,7 @@ struct alignas(16) Tail {
     int last_part;
     List list[2];
 };
-constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
+constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);  // at most: a launch asks for the stages that it has
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 
 struct Piece {
@@ -324,6 +404,7 @@ struct Pieces {
         u = end;
         return true;
     }
+    __device__ __forceinline__ int left() const { return (whole < p.whole ? 1 : 0) + (u < hi ? 1 : 0); }  // 0: none
 };
 
 // The adapters' products of a tile's rows, by one warp, and which of them belong to this part.
@@ -335,7 +416,7 @@ __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, cons
         int id = -2;                              // no row
         bool scaled = false;
         if (c * kChunk + lane < rows) {
-            id = p.ids[t0 + c * kChunk + lane];
+            id = ld_relaxed_gpu(p.ids + t0 + c * kChunk + lane);  // bf16: before this kernel's wait, so past L1
             if (id < 0 || id >= p.L) id = -1;
             if constexpr (kHalf) scaled = id >= 0 && p.z_scale[t0 + c * kChunk + lane] != 1.0f;
         }
@@ -447,9 +528,10 @@ struct Epilogue {
                 if (q.part < 0) {
                     store(v, t0 + c * kChunk, n);
                 } else {
-                    float* to = p.part + (size_t(q.part) * p.tok + c * kChunk) * kRows + row;
+                    float* to = p.part + (size_t(q.part) * p.tok + c * kChunk) * kRows + row * 4;
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) to[j * kRows] = v[j];
+                    for (int j = 0; j < kChunk; j += 4)
+                        if (c * kChunk + j < cols) *reinterpret_cast<float4*>(to + j * kRows) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                 }
             }
             ptx::tc_fence_before();
@@ -470,11 +552,21 @@ struct Epilogue {
                 float v[kChunk];
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
-                for (int o = first; o <= last; ++o) {
-                    const int slot = 2 * o + (local == streamk::first_unit(o, p.shares, pieces.units) / p.kbs ? 0 : 1);
-                    const float* part = p.part + (size_t(slot) * p.tok + c * kChunk) * kRows + row;
+                for (int o0 = first; o0 <= last; o0 += kAtOnce) {  // the parts in their order, some of them loaded at once
+                    float4 f[kAtOnce][kChunk / 4];
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) v[j] += streamk::ld_partial(part + j * kRows);
+                    for (int i = 0; i < kAtOnce; ++i) {
+                        const int o = o0 + i, slot = 2 * o + (local == streamk::first_unit(o, p.shares, pieces.units) / p.kbs ? 0 : 1);
+                        const float* part = p.part + (size_t(slot) * p.tok + c * kChunk) * kRows + row * 4;
+#pragma unroll
+                        for (int j = 0; j < kChunk / 4; ++j)
+                            f[i][j] = o <= last && c * kChunk + 4 * j < cols ? streamk::ld_partial4(part + 4 * j * kRows) : make_float4(0, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                        for (int j = 0; j < kChunk / 4; ++j)
+                            v[4 * j] += f[i][j].x, v[4 * j + 1] += f[i][j].y, v[4 * j + 2] += f[i][j].z, v[4 * j + 3] += f[i][j].w;
                 }
                 store(v, t0 + c * kChunk, n);
             }
@@ -489,9 +581,9 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     pdl_launch();
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    Tail& st = *reinterpret_cast<Tail*>(ring + kRingBytes);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int stage = kABytes + p.tok * kKBytes;
+    Tail& st = *reinterpret_cast<Tail*>(ring + p.stages * stage);
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
             ptx::mbar_init(&st.full[i], 1);
@@ -523,38 +615,50 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     if (warp == 0) {
         if (ptx::elect_one()) {
             Pieces pieces(p);
-            Piece q;
+            Piece q, held;
             int it = 0;
             bool ok = true, waited = false;
             auto next_stage = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
-            for (int n = 0; ok && pieces.next(&q); ++n) {
+            auto sums = [&](const Piece& q) {  // x W^T
                 const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows, t0 = tt * p.tok;
                 for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
-                    if (!(ok = next_stage())) break;
+                    if (!next_stage()) return false;
                     const int s = it % p.stages;
                     ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
                     ptx::tma_load_2d(ring + s * stage, &map_w, kb * kKElems, n0, &st.full[s]);
                     ptx::tma_load_2d(ring + s * stage + kABytes, &map_x, kb * kKElems, t0, &st.full[s]);
                 }
-                if (!ok || !(ok = ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+                return true;
+            };
+            auto products = [&](const Piece& q, int n) {  // z B^T
+                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows, t0 = tt * p.tok;
+                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit)) return false;
                 const List& l = st.list[n & 1];
-                auto load = [&](uint2 e, int chunks) {
-                    if (!waited) pdl_wait();  // shrink: z
+                const int direct = l.direct1 - l.direct0, all = direct + l.mixed1 - l.mixed0;
+                if (all > 0 && !waited) {
+                    pdl_wait();  // shrink: z
                     waited = true;
-                    const int c = int(e.y & 0xff);
+                }
+                for (int i = 0; i < all; ++i) {
+                    const uint2 e = i < direct ? l.direct[l.direct0 + i] : l.mixed[l.mixed0 + i - direct];
+                    const int c = int(e.y & 0xff), chunks = i < direct ? int(e.y >> 8) : 1;
                     for (int r0 = 0; r0 < p.R; r0 += kKElems, ++it) {
                         if (!next_stage()) return false;
                         const int s = it % p.stages;
                         ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(kABytes + chunks * kChunk * kKBytes));
                         ptx::tma_load_3d<false>(ring + s * stage, &map_b, r0, n0, int(e.x), ptx::smem_u32(&st.full[s]));
-                        for (int i = 0; i < chunks; ++i)
-                            ptx::tma_load_2d(ring + s * stage + kABytes + i * kChunk * kKBytes, &map_z, r0, t0 + (c + i) * kChunk, &st.full[s]);
+                        for (int j = 0; j < chunks; ++j)
+                            ptx::tma_load_2d(ring + s * stage + kABytes + j * kChunk * kKBytes, &map_z, r0, t0 + (c + j) * kChunk, &st.full[s]);
                     }
-                    return true;
-                };
-                for (int e = l.direct0; ok && e < l.direct1; ++e) ok = load(l.direct[e], int(l.direct[e].y >> 8));
-                for (int e = l.mixed0; ok && e < l.mixed1; ++e) ok = load(l.mixed[e], 1);
+                }
                 ptx::mbar_arrive(&st.list_empty[n & 1]);
+                return true;
+            };
+            for (int n = 0; ok && pieces.next(&q); ++n) {
+                ok = sums(q);
+                if (n == 0) held = q;  // shrink may still run: the first piece's products come behind the second one's sums
+                else ok = ok && (n > 1 || products(held, 0)) && products(q, n);
+                if (n == 0 && pieces.left() == 0) ok = ok && products(q, 0);
             }
             if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
                 const long long begin = clock64();
@@ -584,33 +688,42 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 ++it;
                 return true;
             };
-            for (int n = 0; ok && pieces.next(&q); ++n) {
-                const uint32_t d = tmem + (n & 1) * p.tok;
-                if (!ptx::mbar_wait(&st.tmem_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+            auto sums = [&](const Piece& q, int n) {
+                if (!ptx::mbar_wait(&st.tmem_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
                 ptx::tc_fence_after();
-                for (int kb = q.kb0; ok && kb < q.kb1; ++kb) ok = block(d, p.tok, 4, kb > q.kb0);
-                if (!ok || !(ok = ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+                for (int kb = q.kb0; kb < q.kb1; ++kb)
+                    if (!block(tmem + (n & 1) * p.tok, p.tok, 4, kb > q.kb0)) return false;
+                return true;
+            };
+            auto products = [&](int n) {
+                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit)) return false;
                 const List& l = st.list[n & 1];
-                for (int e = l.direct0; ok && e < l.direct1; ++e)
-                    for (int r0 = 0; ok && r0 < p.R; r0 += kKElems)
-                        ok = block(d + (l.direct[e].y & 0xff) * kChunk, int(l.direct[e].y >> 8) * kChunk, min(4, (p.R - r0 + 15) / 16), true);
-                if (!ok) break;
+                for (int e = l.direct0; e < l.direct1; ++e)
+                    for (int r0 = 0; r0 < p.R; r0 += kKElems)
+                        if (!block(tmem + (n & 1) * p.tok + (l.direct[e].y & 0xff) * kChunk, int(l.direct[e].y >> 8) * kChunk, min(4, (p.R - r0 + 15) / 16), true))
+                            return false;
                 ptx::umma_commit(&st.tmem_full[n & 1]);
-                for (int e = l.mixed0; ok && e < l.mixed1; ++e) {
+                for (int e = l.mixed0; e < l.mixed1; ++e) {
                     const bool odd = (l.mixed[e].y & 1u) != 0;  // the half of the epilogue that takes the chunk
                     const int h = odd ? 1 : 0, at = odd ? slot_it[1]++ : slot_it[0]++, slot = at % p.slots;
-                    if (!(ok = ptx::mbar_wait(&st.slot_empty[h][slot], ((at / p.slots) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+                    if (!ptx::mbar_wait(&st.slot_empty[h][slot], ((at / p.slots) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
                     ptx::tc_fence_after();
-                    for (int r0 = 0; ok && r0 < p.R; r0 += kKElems)
-                        ok = block(tmem + 2 * p.tok + (h * p.slots + slot) * kChunk, kChunk, min(4, (p.R - r0 + 15) / 16), r0 > 0);
-                    if (ok) ptx::umma_commit(&st.slot_full[h][slot]);
+                    for (int r0 = 0; r0 < p.R; r0 += kKElems)
+                        if (!block(tmem + 2 * p.tok + (h * p.slots + slot) * kChunk, kChunk, min(4, (p.R - r0 + 15) / 16), r0 > 0)) return false;
+                    ptx::umma_commit(&st.slot_full[h][slot]);
                 }
                 ptx::mbar_arrive(&st.list_empty[n & 1]);
+                return true;
+            };
+            for (int n = 0; ok && pieces.next(&q); ++n) {  // in the order of the copies
+                ok = sums(q, n);
+                if (n > 0) ok = ok && (n > 1 || products(0)) && products(n);
+                if (n == 0 && pieces.left() == 0) ok = ok && products(0);
             }
         }
         __syncwarp();
     } else if (warp == 2) {
-        pdl_wait();  // shrink: z_scale
+        if constexpr (kHalf) pdl_wait();  // shrink: z_scale
         Pieces pieces(p);
         Piece q;
         for (int n = 0; pieces.next(&q); ++n) {
@@ -711,6 +824,47 @@ static int opt_in(K kern, int which, size_t bytes) {
     return DQMOE_OK;
 }
 
+// Rows form while what its blocks read of A (each row's adapter, whoever else has it) is a few microseconds' worth of L2.
+constexpr int64_t kRowsFormBytes = 32 << 20;
+static int launch_shrink(ShrinkParams p, const void* x, cudaStream_t stream) {
+    if (p.T <= 256 && int64_t(p.T) * p.R * p.K * 2 <= kRowsFormBytes) {
+        const dim3 grid(p.T, p.half ? 1 : ceil_div(p.R, kRowWarps));
+        return p.half ? launch_pdl(lora_shrink_rows_kernel<true>, grid, kRowWarps * 32, 0, stream, p)
+                      : launch_pdl(lora_shrink_rows_kernel<false>, grid, kRowWarps * 32, 0, stream, p);
+    }
+    // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached.
+    const int tiles = ceil_div(p.T, kShrinkTok), room = 2 * sm_count(), kbs = ceil_div(p.K, kKElems);
+    int split = kMaxSplit;
+    while (split > 1 && (tiles * split > room || split > kbs)) split /= 2;
+    p.cap = kRows / 2 / p.R > 1 ? kRows / 2 / p.R : 1;
+    const int most = ceil_div(p.L < kShrinkTok ? (p.L < p.T ? p.L : p.T) : (p.T < kShrinkTok ? p.T : kShrinkTok), p.cap);
+    const int fit = room / (tiles * split);
+    p.slots = fit < 1 ? 1 : fit < most ? fit : most;
+    p.stages = kShrinkStages;
+    while (p.stages > 2 && shrink_smem(p.R, p.cap, p.stages) > size_t(112) * 1024) --p.stages;  // two blocks per SM
+    const size_t smem = shrink_smem(p.R, p.cap, p.stages);
+    CUtensorMap xs, a;
+    DQ_RC(make_map_2d(&xs, x, p.half != 0, p.T, p.K, p.ldx, kShrinkTok));
+    DQ_RC(make_map_2d(&a, p.lora_a, p.half != 0, int64_t(p.L) * p.R, p.K, p.K, p.R));
+    DQ_RC(opt_in(lora_shrink_tiles_kernel, 2, size_t(112) * 1024));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(tiles) * p.slots * split, 1, 1);
+    cfg.blockDim = dim3(kShrinkThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(split);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    DQ_CUDA(cudaLaunchKernelEx(&cfg, lora_shrink_tiles_kernel, xs, a, p));
+    return DQMOE_OK;
+}
+
 }  // namespace lora
 }  // namespace dq
 
@@ -748,58 +902,33 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     if (status == nullptr) return DQMOE_ERR_CUDA;
 
     lora::ShrinkParams sp{};
+    sp.x = static_cast<const uint16_t*>(x), sp.ldx = ldx, sp.lora_a = static_cast<const uint16_t*>(lora_a);
     sp.ids = ids, sp.scale = scale;
     sp.z = reinterpret_cast<uint16_t*>(ws + Y.z), sp.z_scale = reinterpret_cast<float*>(ws + Y.z_scale);
     sp.counters = reinterpret_cast<int*>(ws + Y.counters);
     sp.n_counters = p.tiles - p.whole;
     sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status;
-    // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached.
-    const int tiles = ceil_div(T, lora::kShrinkTok), room = 2 * sm_count();
-    int split = lora::kMaxSplit;
-    while (split > 1 && (tiles * split > room || split > p.kbs)) split /= 2;
-    const int most = ceil_div(L < lora::kShrinkTok ? (L < T ? L : T) : (T < lora::kShrinkTok ? T : lora::kShrinkTok), lora::kRows / R);
-    const int fit = room / (tiles * split);
-    sp.slots = fit < 1 ? 1 : fit < most ? fit : most;
 
-    CUtensorMap xs, a, xp, wm, zm, bm;
-    DQ_RC(lora::make_map_2d(&xs, x, half, T, K, ldx, lora::kShrinkTok));
-    DQ_RC(lora::make_map_2d(&a, lora_a, half, int64_t(L) * R, K, K, R));
+    CUtensorMap xp, wm, zm, bm;
     DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, p.tok));
     DQ_RC(lora::make_map_2d(&wm, w, half, N, K, K, lora::kRows));
     DQ_RC(lora::make_map_2d(&zm, sp.z, half, T, R, R, lora::kChunk));
     const cuuint64_t dim[3] = {cuuint64_t(R), cuuint64_t(N), cuuint64_t(L)}, stride[2] = {cuuint64_t(R) * 2, cuuint64_t(N) * R * 2};
     const cuuint32_t box[3] = {lora::kKElems, lora::kRows, 1};
     DQ_RC(lora::make_map(&bm, lora_b, half, 3, dim, stride, box));
-    {
-        const size_t smem = lora::shrink_smem(R);
-        DQ_RC(lora::opt_in(lora::lora_shrink_kernel, 0, smem));
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(unsigned(tiles) * sp.slots * split, 1, 1);
-        cfg.blockDim = dim3(lora::kShrinkThreads, 1, 1);
-        cfg.dynamicSmemBytes = smem;
-        cfg.stream = stream;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = unsigned(split);
-        attr[1].val.clusterDim.y = 1;
-        attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 2;
-        DQ_CUDA(cudaLaunchKernelEx(&cfg, lora::lora_shrink_kernel, xs, a, sp));
-    }
+    DQ_RC(lora::launch_shrink(sp, x, stream));
     p.ids = ids, p.z_scale = half ? sp.z_scale : nullptr, p.bias = bias;
     p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
     p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
     const int sms = sm_count();
     const int grid = p.whole > 0 ? (p.whole < sms ? (p.whole > p.shares ? p.whole : p.shares) : sms) : p.shares;
+    const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + p.tok * lora::kKBytes) + sizeof(lora::Tail);
     if (half) {
-        DQ_RC(lora::opt_in(lora::lora_project_kernel<true>, 1, lora::kSmemBytes));
-        return launch_pdl(lora::lora_project_kernel<true>, dim3(grid), lora::kThreads, lora::kSmemBytes, stream, xp, wm, zm, bm, p);
+        DQ_RC(lora::opt_in(lora::lora_project_kernel<true>, 0, lora::kSmemBytes));
+        return launch_pdl(lora::lora_project_kernel<true>, dim3(grid), lora::kThreads, smem, stream, xp, wm, zm, bm, p);
     }
-    DQ_RC(lora::opt_in(lora::lora_project_kernel<false>, 2, lora::kSmemBytes));
-    return launch_pdl(lora::lora_project_kernel<false>, dim3(grid), lora::kThreads, lora::kSmemBytes, stream, xp, wm, zm, bm, p);
+    DQ_RC(lora::opt_in(lora::lora_project_kernel<false>, 1, lora::kSmemBytes));
+    return launch_pdl(lora::lora_project_kernel<false>, dim3(grid), lora::kThreads, smem, stream, xp, wm, zm, bm, p);
 }
 
 }  // extern "C"

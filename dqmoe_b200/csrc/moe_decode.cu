@@ -512,12 +512,6 @@ __device__ __forceinline__ void put_sums(float* to, int row, uint32_t mask, cons
     for (int t = 0; t < kTp; t += 4)
         if ((mask >> t) & 15u) *reinterpret_cast<float4*>(to + t * kRows + row * 4) = make_float4(sum[t], sum[t + 1], sum[t + 2], sum[t + 3]);
 }
-__device__ __forceinline__ float4 ld_partial4(const float* p) {
-    float4 v;
-    asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
-    return v;
-}
-
 // Accumulators to scaled sums of a piece, which go to the piece's place in the workspace.
 template <bool kFp8, int kTp>
 struct Drain {
@@ -725,7 +719,7 @@ struct Finish {
         for (int o = 0; o < kAtOnce; ++o)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                v[o][h] = o < parts && ((mask8 >> (4 * h)) & 15u) != 0 ? ld_partial4(part + o * stride + (t0 + 4 * h) * kRows + row * 4)
+                v[o][h] = o < parts && ((mask8 >> (4 * h)) & 15u) != 0 ? streamk::ld_partial4(part + o * stride + (t0 + 4 * h) * kRows + row * 4)
                                                                         : make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int o = 0; o < kAtOnce; ++o)
