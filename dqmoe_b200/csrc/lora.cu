@@ -481,6 +481,35 @@ struct Epilogue {
             if (t0 + j < p.T) y[j * p.ldy] = to_bits(v[j] + bias, kHalf);
     }
 
+    // The sums of a tile from its parts, in their order, some of them loaded at once.
+    __device__ __forceinline__ void add_parts(int slot0, int first, int last, int half, int cols, int t0, int n) {
+#pragma unroll 1
+        for (int c = half; c * kChunk < cols; c += 2) {
+            const float* from = p.part + c * kChunk * kRows + row * 4;
+            const size_t stride = size_t(p.tok) * kRows;
+            float v[kChunk];
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
+#pragma unroll 1
+            for (int o0 = first; o0 <= last; o0 += kAtOnce) {
+                float4 f[kAtOnce][kChunk / 4];
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i) {
+                    const float* part = from + (o0 + i == first ? slot0 : 2 * (o0 + i)) * stride;
+#pragma unroll
+                    for (int j = 0; j < kChunk / 4; ++j)
+                        f[i][j] = o0 + i <= last && c * kChunk + 4 * j < cols ? streamk::ld_partial4(part + 4 * j * kRows) : make_float4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                    for (int j = 0; j < kChunk / 4; ++j)
+                        v[4 * j] += f[i][j].x, v[4 * j + 1] += f[i][j].y, v[4 * j + 2] += f[i][j].z, v[4 * j + 3] += f[i][j].w;
+            }
+            store(v, t0 + c * kChunk, n);
+        }
+    }
+
     __device__ __forceinline__ void run() {
         pdl_wait();  // shrink: the counters, z_scale
         Pieces pieces(p);
@@ -541,35 +570,16 @@ struct Epilogue {
                 ptx::mbar_arrive(&st.list_empty[buf]);
             }
             if (q.part < 0) continue;
-            __threadfence();
+            // What the warps wrote, the counting thread has seen at `meet`, and its release and acquire at gpu scope hold for all of them: a fence in
+            // each thread, before and after, took 1 and 3 to 6 us.
             const int local = q.tile - p.whole, first = int(blockIdx.x) - q.index, last = first + q.of - 1;
             if (!meet()) return;
             if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(&p.counters[local], 1) == q.of - 1;
             if (!meet()) return;
             if (*const_cast<volatile int*>(&st.last_part) == 0) continue;
-            __threadfence();
-            for (int c = half; c * kChunk < cols; c += 2) {
-                float v[kChunk];
-#pragma unroll
-                for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
-                for (int o0 = first; o0 <= last; o0 += kAtOnce) {  // the parts in their order, some of them loaded at once
-                    float4 f[kAtOnce][kChunk / 4];
-#pragma unroll
-                    for (int i = 0; i < kAtOnce; ++i) {
-                        const int o = o0 + i, slot = 2 * o + (local == streamk::first_unit(o, p.shares, pieces.units) / p.kbs ? 0 : 1);
-                        const float* part = p.part + (size_t(slot) * p.tok + c * kChunk) * kRows + row * 4;
-#pragma unroll
-                        for (int j = 0; j < kChunk / 4; ++j)
-                            f[i][j] = o <= last && c * kChunk + 4 * j < cols ? streamk::ld_partial4(part + 4 * j * kRows) : make_float4(0, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-                        for (int j = 0; j < kChunk / 4; ++j)
-                            v[4 * j] += f[i][j].x, v[4 * j + 1] += f[i][j].y, v[4 * j + 2] += f[i][j].z, v[4 * j + 3] += f[i][j].w;
-                }
-                store(v, t0 + c * kChunk, n);
-            }
+            // only the first part may be its share's second tile
+            const int slot0 = 2 * first + (local == streamk::first_unit(first, p.shares, pieces.units) / p.kbs ? 0 : 1);
+            add_parts(slot0, first, last, half, cols, t0, n);
         }
     }
 };

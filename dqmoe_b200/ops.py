@@ -22,6 +22,7 @@ QUANT_FP8_BLOCK = 1024
 QUANT_FP8_MX = 2048
 SCORE_SOFTMAX = 0
 SCORE_SIGMOID = 1
+_SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
 DT_FLOAT = 0
 DT_HALF = 1
 DT_BF16 = 7
@@ -43,6 +44,23 @@ def _cuda(t: torch.Tensor, name: str) -> torch.Tensor:
     if not t.is_contiguous():
         raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name}.is_contiguous()")
     return t
+
+
+def _raw_stream(index: int) -> int:
+    """torch's current stream of device `index` as an address."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, current stream) with device `index` current. Entering torch.cuda.device and building a Stream object cost 4 us of a call that
+    takes the GPU 15, so neither is done where the device is current already."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc != 0:
+        _lib.check(rc)
 
 
 def device_status() -> int:
@@ -192,51 +210,56 @@ def moe_decode(x: torch.Tensor, w_router: torch.Tensor, b: torch.Tensor, b_scale
     x [T, H] bf16, w_router [E, H] bf16 or fp32, experts' weights bf16 (quant_mode 0) or e4m3 with that mode's scales
     (256 / 512 / 1024). The activations are not quantised. The last n_shared experts of b / b1 are shared ones that every token
     passes through with weight 1. Returns out [T, H] bf16."""
-    for name, t in (("x", x), ("w_router", w_router), ("b", b), ("b1", b1)):
-        _cuda(t, name)
-        if t.device != x.device:
-            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
     quant_mode = int(quant_mode)
-    weights = torch.bfloat16 if quant_mode == QUANT_NONE else FP8
-    if x.dim() != 2 or x.dtype != torch.bfloat16:
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: x is bf16 [T, H]")
-    T, H = x.shape
-    if b.dim() != 3 or b1.dim() != 3 or b.dtype != weights or b1.dtype != weights:
-        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: b and b1 are {weights} [E, 2I, H] and [E, H, I]")
-    E_all, I = b.shape[0], b1.shape[2]
-    E = E_all - n_shared
-    if tuple(b.shape) != (E_all, 2 * I, H) or tuple(b1.shape) != (E_all, H, I):
-        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: b is [E, 2I, H] and b1 [E, H, I]  Info: got {tuple(b.shape)}, {tuple(b1.shape)}")
-    if n_shared < 0 or E <= 0 or tuple(w_router.shape) != (E, H) or w_router.dtype not in (torch.bfloat16, torch.float32):
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: w_router is bf16 or fp32 [num_experts - n_shared, H]")
-    if quant_mode in (QUANT_FP8_TENSOR, QUANT_FP8_CHANNEL, QUANT_FP8_BLOCK):
-        g = lambda n: (n + 127) // 128
-        want = {QUANT_FP8_TENSOR: (E_all, E_all), QUANT_FP8_CHANNEL: (E_all * 2 * I, E_all * H),
-                QUANT_FP8_BLOCK: (E_all * g(2 * I) * g(H), E_all * g(H) * g(I))}[quant_mode]
-        for name, t, n in (("b_scale", b_scale, want[0]), ("b1_scale", b1_scale, want[1])):
-            if t is None or t.device != x.device or t.dtype != torch.float32 or not t.is_contiguous() or t.numel() != n:
-                raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor of {n} elements on x's device "
-                                   f"for quant mode {quant_mode}")
+    dev, mode = x.device, _SCORES[scoring]
+    T, H, E, I = _moe_decode_sizes(x, w_router, b, b_scale, b1, b1_scale, quant_mode, n_shared, dev)
     lib = _lib.load()
     if workspace is None:
-        need = int(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode))
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
-    else:
-        _cuda(workspace, "workspace")
-        if workspace.device != x.device:
-            raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is on x's device")
+        workspace = torch.empty(max(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode), 256), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
     if out is None:
-        out = torch.empty((T, H), dtype=torch.bfloat16, device=x.device)
-    else:
-        _cuda(out, "out")
-        if tuple(out.shape) != (T, H) or out.dtype != torch.bfloat16 or out.device != x.device:
-            raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is bf16 [T, H] on x's device")
-    mode = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}[scoring]
-    with torch.cuda.device(x.device):
-        _lib.check(lib.dqmoe_moe_decode(_p(x), _p(w_router), DT_FLOAT if w_router.dtype == torch.float32 else DT_BF16, _p(b), _p(b_scale),
-                                        _p(b1), _p(b1_scale), _p(out), _p(workspace), workspace.numel() * workspace.element_size(), T, H, I,
-                                        E, k, n_shared, mode, quant_mode, _stream(x.device)))
+        out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+    elif out.shape != (T, H) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous():
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is contiguous bf16 [T, H] on x's device")
+    fp8 = quant_mode != QUANT_NONE
+    _call(dev.index, lib.dqmoe_moe_decode, x.data_ptr(), w_router.data_ptr(), DT_FLOAT if w_router.dtype is torch.float32 else DT_BF16,
+          b.data_ptr(), b_scale.data_ptr() if fp8 else None, b1.data_ptr(), b1_scale.data_ptr() if fp8 else None, out.data_ptr(),
+          workspace.data_ptr(), workspace.numel() * workspace.element_size(), T, H, I, E, k, n_shared, mode, quant_mode)
     return out
+
+
+def _moe_decode_sizes(x, w_router, b, b_scale, b1, b1_scale, quant_mode, n_shared, dev):
+    """T, H, E, I of operands that moe_decode takes. One test for all that is as it should be; which part fails is found out afterwards."""
+    fp8 = quant_mode != QUANT_NONE
+    weights = FP8 if fp8 else torch.bfloat16
+    if x.dim() == 2 and b.dim() == 3:
+        T, H = x.shape
+        E_all, I = b.shape[0], b.shape[1] // 2
+        E = E_all - n_shared
+        if (x.is_cuda and x.dtype is torch.bfloat16 and b.dtype is weights and b1.dtype is weights and b.shape == (E_all, 2 * I, H)
+                and b1.shape == (E_all, H, I) and n_shared >= 0 and E > 0 and w_router.shape == (E, H)
+                and (w_router.dtype is torch.bfloat16 or w_router.dtype is torch.float32) and w_router.device == dev and b.device == dev
+                and b1.device == dev and x.is_contiguous() and w_router.is_contiguous() and b.is_contiguous() and b1.is_contiguous()):
+            if not fp8:
+                return T, H, E, I
+            g = lambda n: (n + 127) // 128
+            want = {QUANT_FP8_TENSOR: (E_all, E_all), QUANT_FP8_CHANNEL: (E_all * 2 * I, E_all * H),
+                    QUANT_FP8_BLOCK: (E_all * g(2 * I) * g(H), E_all * g(H) * g(I))}.get(quant_mode, (0, 0))  # other modes: the library refuses
+            for name, t, n in (("b_scale", b_scale, want[0]), ("b1_scale", b1_scale, want[1])):
+                if n and (t is None or t.device != dev or t.dtype is not torch.float32 or not t.is_contiguous() or t.numel() != n):
+                    raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor of {n} elements on x's device "
+                                       f"for quant mode {quant_mode}")
+                if t is None:
+                    raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is given")
+            return T, H, E, I
+    for name, t in (("x", x), ("w_router", w_router), ("b", b), ("b1", b1)):
+        _cuda(t, name)
+        if t.device != dev:
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
+    raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: x is bf16 [T, H], w_router bf16 or fp32 [E, H], b and b1 {weights} [E + n_shared, 2I, H] and "
+                       f"[E + n_shared, H, I]  Info: got {x.dtype} {tuple(x.shape)}, {w_router.dtype} {tuple(w_router.shape)}, {b.dtype} "
+                       f"{tuple(b.shape)}, {b1.dtype} {tuple(b1.shape)}, n_shared={n_shared}")
 
 
 # ---------------------------------------------------------------------- routing
@@ -589,46 +612,49 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
 
     x [T, K], w [N, K], lora_a [L, R, K], lora_b [L, N, R], all bf16 or all fp16; ids int32 [T] (outside [0, L): no adapter), scale fp32
     [L], bias fp32 [N]. x and out may have rows that stand apart (columns next to each other). Returns y [T, N]."""
-    for name, t in (("w", w), ("lora_a", lora_a), ("lora_b", lora_b), ("ids", ids)):
-        _cuda(t, name)
-    for name, t in (("x", x), ("out", out)):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name}.is_cuda  Info: dqmoe_b200 has no CPU path")
-        if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a matrix whose rows lie apart and whose columns lie together")
-    if x.dtype not in (torch.bfloat16, torch.float16) or any(t.dtype != x.dtype for t in (w, lora_a, lora_b)):
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: x, w, lora_a and lora_b are all bf16 or all fp16")
-    T, K = x.shape
-    if w.dim() != 2 or w.shape[1] != K or lora_a.dim() != 3 or lora_a.shape[2] != K:
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: w is [N, K] and lora_a [L, R, K]")
-    N, (L, R) = w.shape[0], lora_a.shape[:2]
-    if tuple(lora_b.shape) != (L, N, R):
-        raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: lora_b is [L, N, R]  Info: got {tuple(lora_b.shape)}, want {(L, N, R)}")
-    if ids.dtype != torch.int32 or tuple(ids.shape) != (T,):
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: ids is int32 [T]")
-    for name, t, n in (("scale", scale, L), ("bias", bias, N)):
-        if t is not None and (t.dtype != torch.float32 or not t.is_contiguous() or tuple(t.shape) != (n,)):
-            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor [{n}]")
+    dev, dtype = x.device, x.dtype
+    T, K, N, L, R = _lora_sizes(x, w, lora_a, lora_b, ids, scale, bias, dev)
     if out is None:
-        out = torch.empty((T, N), dtype=x.dtype, device=x.device)
-    elif tuple(out.shape) != (T, N) or out.dtype != x.dtype:
-        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is [T, N] of x's type")
+        out = torch.empty((T, N), dtype=dtype, device=dev)
+    elif out.shape != (T, N) or out.dtype is not dtype or out.device != dev or not _rows_apart(out):
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is [T, N] of x's type, on its device, its rows apart and its columns together")
     lib = _lib.load()
     if workspace is None:
-        need = int(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R))
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=x.device)
-    else:
-        _cuda(workspace, "workspace")
-    for name, t in (("w", w), ("lora_a", lora_a), ("lora_b", lora_b), ("ids", ids), ("scale", scale), ("bias", bias), ("out", out),
-                    ("workspace", workspace)):
-        if t is not None and t.device != x.device:
-            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
-    ldx = x.stride(0) if T > 1 else K
-    ldy = out.stride(0) if T > 1 else N
-    with torch.cuda.device(x.device):
-        _lib.check(lib.dqmoe_lora_linear(_p(x), ldx, _p(w), _p(lora_a), _p(lora_b), _p(ids), _p(scale), _p(bias), _p(out), ldy, _p(workspace),
-                                         workspace.numel() * workspace.element_size(), T, N, K, L, R,
-                                         DT_HALF if x.dtype == torch.float16 else DT_BF16, _stream(x.device)))
+        workspace = torch.empty(max(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R), 256), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
+    _call(dev.index, lib.dqmoe_lora_linear, x.data_ptr(), x.stride(0) if T > 1 else (K + 7) // 8 * 8, w.data_ptr(), lora_a.data_ptr(),
+          lora_b.data_ptr(), ids.data_ptr(), None if scale is None else scale.data_ptr(), None if bias is None else bias.data_ptr(),
+          out.data_ptr(), out.stride(0) if T > 1 else N, workspace.data_ptr(), workspace.numel() * workspace.element_size(), T, N, K, L, R,
+          DT_HALF if dtype is torch.float16 else DT_BF16)
     return out
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+
+
+def _lora_sizes(x, w, lora_a, lora_b, ids, scale, bias, dev):
+    """T, K, N, L, R of operands that lora_linear takes. One test for all that is as it should be; which part fails is found out afterwards."""
+    dtype = x.dtype
+    if x.dim() == 2 and w.dim() == 2 and lora_a.dim() == 3:
+        T, K = x.shape
+        N, (L, R, _) = w.shape[0], lora_a.shape
+        if (x.is_cuda and (dtype is torch.bfloat16 or dtype is torch.float16) and w.dtype is dtype and lora_a.dtype is dtype
+                and lora_b.dtype is dtype and ids.dtype is torch.int32 and w.shape == (N, K) and lora_a.shape == (L, R, K)
+                and lora_b.shape == (L, N, R) and ids.shape == (T,) and w.device == dev and lora_a.device == dev and lora_b.device == dev
+                and ids.device == dev and w.is_contiguous() and lora_a.is_contiguous() and lora_b.is_contiguous() and ids.is_contiguous()
+                and _rows_apart(x)):
+            for name, t, n in (("scale", scale, L), ("bias", bias, N)):
+                if t is not None and (t.dtype is not torch.float32 or t.device != dev or t.shape != (n,) or not t.is_contiguous()):
+                    raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is a contiguous fp32 tensor [{n}] on x's device")
+            return T, K, N, L, R
+    for name, t in (("w", w), ("lora_a", lora_a), ("lora_b", lora_b), ("ids", ids)):
+        _cuda(t, name)
+        if t.device != dev:
+            raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: {name} is on x's device")
+    if x.dim() != 2 or not _rows_apart(x):
+        raise RuntimeError("[ASSERT FAILED] ops.py  Condition: x is a matrix whose rows lie apart and whose columns lie together")
+    raise RuntimeError(f"[ASSERT FAILED] ops.py  Condition: x [T, K], w [N, K], lora_a [L, R, K] and lora_b [L, N, R] are all bf16 or all fp16, ids "
+                       f"int32 [T]  Info: got {x.dtype} {tuple(x.shape)}, {w.dtype} {tuple(w.shape)}, {lora_a.dtype} {tuple(lora_a.shape)}, "
+                       f"{lora_b.dtype} {tuple(lora_b.shape)}, {ids.dtype} {tuple(ids.shape)}")
