@@ -412,14 +412,23 @@ template <bool kHalf>
 __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane) {
     int direct = 0, mixed = 0, last = -1, last_end = -1, last_first = 0;
     const int rows = min(p.tok, p.T - t0), half = lane >> 4;
-    for (int c = 0; c * kChunk < rows; c += 2) {  // two chunks at a time, half a warp each
-        int id = -2;                              // no row
-        bool scaled = false;
-        if (c * kChunk + lane < rows) {
-            id = ld_relaxed_gpu(p.ids + t0 + c * kChunk + lane);  // bf16: before this kernel's wait, so past L1
-            if (id < 0 || id >= p.L) id = -1;
-            if constexpr (kHalf) scaled = id >= 0 && p.z_scale[t0 + c * kChunk + lane] != 1.0f;
-        }
+    int ids[kMaxTok / 32];
+    uint32_t scaled_rows = 0;  // bit c: this lane's row of the c-th pair of chunks has a power of two
+#pragma unroll
+    for (int c = 0; c < kMaxTok / 32; ++c) ids[c] = c * 32 + lane < rows ? ld_relaxed_gpu(p.ids + t0 + c * 32 + lane) : -2;  // bf16: before this kernel's wait, so past L1
+    if constexpr (kHalf) {
+#pragma unroll
+        for (int c = 0; c < kMaxTok / 32; ++c)
+            if (c * 32 + lane < rows && ids[c] >= 0 && ids[c] < p.L && p.z_scale[t0 + c * 32 + lane] != 1.0f) scaled_rows |= 1u << c;
+    }
+#pragma unroll
+    for (int pair = 0; pair < kMaxTok / 32; ++pair) {  // two chunks at a time, half a warp each
+        const int c = 2 * pair;
+        if (c * kChunk >= rows) break;
+        int id = ids[pair];  // -2: no row
+        if (id != -2 && (id < 0 || id >= p.L)) id = -1;
+        if (c * kChunk + lane < rows && id == -2) id = -1;
+        const bool scaled = ((scaled_rows >> pair) & 1u) != 0;
         const uint32_t present = __ballot_sync(0xffffffffu, id >= -1), with = __ballot_sync(0xffffffffu, id >= 0);
         if (with == 0) continue;
         const uint32_t scales = __ballot_sync(0xffffffffu, scaled);
@@ -789,8 +798,11 @@ static Layout plan(Params* p, int T, int N, int K, int R) {
     const int sms = sm_count(), left = p->tiles % sms;
     // a last round that is three quarters full is left as it is
     p->whole = left * 4 >= sms * 3 ? p->tiles : p->tiles - left;
-    const int64_t units = int64_t(p->tiles - p->whole) * p->kbs;
-    p->shares = units < sms ? int(units) : sms;
+    // The others in equal shares, one per SM; in as many equal parts of each tile as the SMs allow, where that leaves no more than one SM in
+    // seven without work: then no share has two pieces, and no tile more parts than it needs.
+    const int split = p->tiles - p->whole, each = split > 0 ? (sms / split < p->kbs ? sms / split : p->kbs) : 0;
+    const int64_t units = int64_t(split) * p->kbs;
+    p->shares = split * each * 7 >= sms * 6 ? split * each : units < sms ? int(units) : sms;
     Layout L{};
     size_t off = 0;
     auto add = [&](size_t bytes) {
