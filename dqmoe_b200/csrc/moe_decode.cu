@@ -268,6 +268,7 @@ struct alignas(16) Tail {
     int bound2[kMaxParts + 1];                 // first unit of each part of an fc2 tile
     uint32_t bad_tokens;                       // tokens without a number among their weights
     int last;
+    alignas(16) float token_scale[4][2 * kMaxTokens];  // of a unit's tokens, by accumulator buffer; fc2: of its two K blocks
     uint32_t amax[4][kMaxTokens];
     int topk_index[kMaxTokens][kMaxTopk];
     float topk_weight[kMaxTokens][kMaxTopk];
@@ -476,42 +477,57 @@ __device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* 
     drain_copies<S::kStages>(st, it);
 }
 
+// The MMAs of every unit, issued by one thread; by the whole warp because it also takes the scales of a unit's tokens out of its stage (FP8), to stand
+// beside the accumulators that they belong to: so the stage is free when the MMAs have read it, not when the accumulators have been drained.
 template <bool kFp8, int kTp>
-__device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* ring, uint32_t tmem) {
+__device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* ring, uint32_t tmem, int lane) {
     using S = Shape<kFp8, kTp>;
     constexpr int kKind = kFp8 ? 0 : 1;
     constexpr uint32_t kFormat = kFp8 ? 0 : 1;
     constexpr uint32_t kId1 = ptx::make_idesc(kFormat, kRows, S::kN1), kId2 = ptx::make_idesc(kFormat, kRows, S::kN2);
     int it = 0, buf_it = 0;
     for (int n = 0;; ++n) {
-        const Piece q = next_piece<false>(p, st, n, 0);
+        const Piece q = next_piece<true>(p, st, n, lane);
         if (q.phase >= 2) return;
         bool fresh = true;  // the next unit begins an accumulator buffer
         for (int u = q.lo; u < q.hi; ++u, ++it) {
             const int slot = it % S::kStages, buf = buf_it % S::kBufs;
-            if (fresh && !ptx::mbar_wait(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
-            if (!ptx::mbar_wait(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit)) return;
+            if (fresh && !ptx::mbar_wait_warp(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
+            if (!ptx::mbar_wait_warp(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit)) return;
             ptx::tc_fence_after();
-            const uint32_t a = ptx::smem_u32(ring + slot * S::kStage);
-            const uint64_t da = ptx::smem_desc_sw128(a), db = ptx::smem_desc_sw128(a + kABytes);
-            const uint32_t d = tmem + buf * S::kBufCols;
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint64_t ak = ptx::smem_desc_advance(da, half * kTileBytes + k * 32);
-                    if (q.phase == 0)  // gate rows, value rows
-                        ptx::umma<kKind>(d + half * S::kN1, ak, ptx::smem_desc_advance(db, k * 32), kId1, (!kFp8 && !fresh) || k > 0);
-                    else               // two K blocks: with their own scales in FP8, one sum in bf16
-                        ptx::umma<kKind>(d + (kFp8 ? half * S::kN2 : 0), ak, ptx::smem_desc_advance(db, half * S::kN2 * kKBytes + k * 32), kId2,
-                                         (!kFp8 && (!fresh || half > 0)) || k > 0);
-                }
-            ptx::umma_commit(&st.empty[slot]);
             const bool done = kFp8 || u + 1 == q.hi || (q.phase == 1 && (u + 1) % p.pairs2 == 0);
-            if (done) {
-                ptx::umma_commit(&st.tmem_full[buf]);
-                ++buf_it;
+            if (ptx::elect_one()) {
+                const uint32_t a = ptx::smem_u32(ring + slot * S::kStage);
+                const uint64_t da = ptx::smem_desc_sw128(a), db = ptx::smem_desc_sw128(a + kABytes);
+                const uint32_t d = tmem + buf * S::kBufCols;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint64_t ak = ptx::smem_desc_advance(da, half * kTileBytes + k * 32);
+                        if (q.phase == 0)  // gate rows, value rows
+                            ptx::umma<kKind>(d + half * S::kN1, ak, ptx::smem_desc_advance(db, k * 32), kId1, (!kFp8 && !fresh) || k > 0);
+                        else               // two K blocks: with their own scales in FP8, one sum in bf16
+                            ptx::umma<kKind>(d + (kFp8 ? half * S::kN2 : 0), ak, ptx::smem_desc_advance(db, half * S::kN2 * kKBytes + k * 32), kId2,
+                                             (!kFp8 && (!fresh || half > 0)) || k > 0);
+                    }
+                ptx::umma_commit(&st.empty[slot]);
+                if (done) ptx::umma_commit(&st.tmem_full[buf]);
             }
+            __syncwarp();
+            if constexpr (kFp8) {
+                const float* from = reinterpret_cast<const float*>(ring + slot * S::kStage + kABytes + (q.phase == 0 ? S::kN1 : 2 * S::kN2) * kKBytes);
+                if (lane < kTp) {
+                    st.token_scale[buf][lane] = from[lane];
+                    if (q.phase == 1) st.token_scale[buf][kTp + lane] = from[kTp + lane];
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(&st.empty[slot]);
+                    ptx::mbar_arrive(&st.tmem_full[buf]);
+                }
+            }
+            if (done) ++buf_it;
             fresh = done;
         }
     }
@@ -539,10 +555,9 @@ struct Drain {
     static constexpr int kCols = kTp < 16 ? kTp : 16;  // columns in registers at a time
     const Params& p;
     Tail& st;
-    uint8_t* ring;
     uint32_t tmem;
     int warp, lane, row;  // warp 0..3, row = TMEM lane = weight row of the tile
-    int it = 0, buf_it = 0;
+    int buf_it = 0;
 
     __device__ __forceinline__ bool acquire() {
         const int buf = buf_it % S::kBufs;
@@ -550,19 +565,13 @@ struct Drain {
         ptx::tc_fence_after();
         return true;
     }
-    // scales of a unit's tokens: they came with the stage, whose barrier this warp has to see for itself
-    __device__ __forceinline__ bool stage_full() {
-        return ptx::mbar_wait_warp(&st.full[it % S::kStages], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit);
-    }
-    __device__ __forceinline__ void release(bool stage) {
+    __device__ __forceinline__ void release() {
         ptx::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-            ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
-            if (stage) ptx::mbar_arrive(&st.empty[it % S::kStages]);
-        }
+        if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
         ++buf_it;
     }
+    __device__ __forceinline__ const float* token_scale() const { return st.token_scale[buf_it % S::kBufs]; }
     __device__ __forceinline__ uint32_t buffer() const { return tmem + (buf_it % S::kBufs) * S::kBufCols; }
 
     // sum += (hi + lo / 16) * scale of every token of `mask`
@@ -592,22 +601,21 @@ struct Drain {
             for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
             float sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, q.lo);
             float sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, q.lo);
-            for (int kb = q.lo; kb < q.hi; ++kb, ++it) {
+            for (int kb = q.lo; kb < q.hi; ++kb) {
                 const float gs = sg, vs = sv;
                 if (kb + 1 < q.hi) {  // the next unit's, while this one's MMAs are on their way
                     sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, kb + 1);
                     sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb + 1);
                 }
-                if (!stage_full() || !acquire()) return false;
-                const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + S::kN1 * kKBytes);
-                add_scaled(buffer(), token_scale, gs, mask, g);
-                add_scaled(buffer() + S::kN1, token_scale, vs, mask, v);
-                release(true);
+                if (!acquire()) return false;
+                add_scaled(buffer(), token_scale(), gs, mask, g);
+                add_scaled(buffer() + S::kN1, token_scale(), vs, mask, v);
+                release();
             }
         } else {
             if (!acquire()) return false;
             ptx::tmem_read2<kTp>(buffer(), buffer() + S::kN1, g, v);
-            release(false);
+            release();
         }
         put_sums<kTp>(to, row, mask, g);
         put_sums<kTp>(to + kTp * kRows, row, mask, v);
@@ -627,16 +635,15 @@ struct Drain {
             };
             float next0 = 0.0f, next1 = 0.0f;
             if (q.lo < q.hi) next0 = scale_of(q.lo, 0), next1 = scale_of(q.lo, 1);
-            for (int u = q.lo; u < q.hi; ++u, ++it) {
+            for (int u = q.lo; u < q.hi; ++u) {
                 const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
                 const float s0 = next0, s1 = next1;
                 if (u + 1 < q.hi) next0 = scale_of(u + 1, 0), next1 = scale_of(u + 1, 1);
                 const uint32_t mask = st.hit_mask[j];
-                if (!stage_full() || !acquire()) return false;
-                const float* token_scale = reinterpret_cast<const float*>(ring + (it % S::kStages) * S::kStage + kABytes + 2 * S::kN2 * kKBytes);
-                add_scaled(buffer(), token_scale, s0, mask, sum);
-                if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale + kTp, s1, mask, sum);  // nothing was laid out for a block past I
-                release(true);
+                if (!acquire()) return false;
+                add_scaled(buffer(), token_scale(), s0, mask, sum);
+                if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale() + kTp, s1, mask, sum);  // nothing was laid out for a block past I
+                release();
             }
         } else {
             for (int u = q.lo; u < q.hi;) {  // expert by expert: only the tokens that chose it take part
@@ -645,7 +652,7 @@ struct Drain {
                 if (!acquire()) return false;
                 float hi[kTp], lo[kTp];
                 ptx::tmem_read2<kTp>(buffer(), buffer() + kTp, hi, lo);
-                release(false);
+                release();
                 const uint32_t mask = st.hit_mask[j];
 #pragma unroll
                 for (int t = 0; t < kTp; ++t)
@@ -909,10 +916,10 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::kStages; ++i) {
             ptx::mbar_init(&st.full[i], 2);              // weights, tokens
-            ptx::mbar_init(&st.empty[i], kFp8 ? 5 : 1);  // the tensor core's reads, and the draining warps' of the scales
+            ptx::mbar_init(&st.empty[i], kFp8 ? 2 : 1);  // the tensor core's reads, and the MMA warp's of the scales
         }
         for (int i = 0; i < 4; ++i) {
-            ptx::mbar_init(&st.tmem_full[i], 1);
+            ptx::mbar_init(&st.tmem_full[i], kFp8 ? 2 : 1);  // the MMAs, and the scales
             ptx::mbar_init(&st.tmem_empty[i], 4);
         }
         for (int i = 0; i < kClaims; ++i) {
@@ -954,8 +961,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         if (ptx::elect_one()) load_weights<kFp8, kTp>(p, map_b, map_b1, st, ring, claim);
         __syncwarp();
     } else if (warp == 1) {
-        if (ptx::elect_one()) multiply<kFp8, kTp>(p, st, ring, tmem);
-        __syncwarp();
+        multiply<kFp8, kTp>(p, st, ring, tmem, lane);
     } else if (warp == 2) {
         if (ptx::elect_one()) load_tokens<kFp8, kTp>(p, st, ring);
         __syncwarp();
@@ -966,7 +972,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         Finish<kFp8, kTp> f{p, st, warp - 8, lane, (warp - 8) * 32 + lane};
         f.run();
     } else if (warp >= 4) {
-        Drain<kFp8, kTp> d{p, st, ring, tmem + (uint32_t((warp - 4) * 32) << 16), warp - 4, lane, (warp - 4) * 32 + lane};
+        Drain<kFp8, kTp> d{p, st, tmem + (uint32_t((warp - 4) * 32) << 16), warp - 4, lane, (warp - 4) * 32 + lane};
         d.run();
     }
     __syncthreads();
