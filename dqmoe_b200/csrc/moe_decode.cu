@@ -40,7 +40,8 @@ namespace moe_decode {
 constexpr int kMaxTokens = 32;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 32;
-constexpr int kThreads = 384;                 // warp 0 weights, 1 MMA, 2 tokens, 3 count, warps 4..7 drain, warps 8..11 finish; all choose the experts
+// warp 0 weights, 1 MMA, 2 tokens, 3 count, warps 4..7 drain, warps 8..11 finish, warps 12..15 drain the second 16 of 32 tokens; all choose the experts
+__host__ __device__ constexpr int threads(int tp) { return tp > 16 ? 512 : 384; }
 constexpr int kRows = 128;                    // weight rows of an MMA
 constexpr int kKBytes = 128;                  // bytes of a K block: one swizzle row
 constexpr int kTileBytes = kRows * kKBytes;   // 16 KiB
@@ -391,6 +392,8 @@ struct Shape {
     static constexpr int kBufs = kFp8 ? 4 : 2;
     static constexpr int kTmemCols = kBufs * kBufCols;  // 128 / 256 / 512 and 64 / 64 / 128
     static_assert((kTmemCols & (kTmemCols - 1)) == 0 && kTmemCols >= 32 && kTmemCols <= 512, "TMEM allocation");
+    static constexpr int kDrainTokens = kTp > 16 ? 16 : kTp;  // of four draining warps
+    static constexpr int kDrainWarps = 4 * kTp / kDrainTokens;
     static constexpr size_t kPart1 = size_t(2) * kTp * kRows, kPart2 = size_t(kTp) * kRows;  // floats
 };
 
@@ -548,15 +551,27 @@ __device__ __forceinline__ void put_sums(float* to, int row, uint32_t mask, cons
     for (int t = 0; t < kTp; t += 4)
         if ((mask >> t) & 15u) *reinterpret_cast<float4*>(to + t * kRows + row * 4) = make_float4(sum[t], sum[t + 1], sum[t + 2], sum[t + 3]);
 }
+// Two fp32 values in a register pair, and their FMA in one instruction.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+}
 // Accumulators to scaled sums of a piece, which go to the piece's place in the workspace.
 template <bool kFp8, int kTp>
 struct Drain {
     using S = Shape<kFp8, kTp>;
-    static constexpr int kCols = kTp < 16 ? kTp : 16;  // columns in registers at a time
+    static constexpr int kCols = S::kDrainTokens;
     const Params& p;
     Tail& st;
     uint32_t tmem;
-    int warp, lane, row;  // warp 0..3, row = TMEM lane = weight row of the tile
+    int warp, lane, row;  // row = TMEM lane = weight row of the tile
+    int t0;               // first of this warp's tokens
     int buf_it = 0;
 
     __device__ __forceinline__ bool acquire() {
@@ -571,34 +586,38 @@ struct Drain {
         if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[buf_it % S::kBufs]);
         ++buf_it;
     }
-    __device__ __forceinline__ const float* token_scale() const { return st.token_scale[buf_it % S::kBufs]; }
-    __device__ __forceinline__ uint32_t buffer() const { return tmem + (buf_it % S::kBufs) * S::kBufCols; }
+    __device__ __forceinline__ const float* token_scale() const { return st.token_scale[buf_it % S::kBufs] + t0; }
+    // columns of this warp's first token
+    __device__ __forceinline__ uint32_t buffer() const { return tmem + (buf_it % S::kBufs) * S::kBufCols + t0; }
 
-    // sum += (hi + lo / 16) * scale of every token of `mask`
-    __device__ __forceinline__ void add_scaled(uint32_t taddr, const float* token_scale, float row_scale, uint32_t mask, float (&sum)[kTp]) {
+    // sum += (hi + lo / 16) * scale, of the tokens of `mask` where the others' columns may hold what is no number
+    template <bool kMasked>
+    __device__ __forceinline__ void add_scaled(uint32_t taddr, const float* token_scale, float row_scale, uint32_t mask, float (&sum)[kCols]) {
+        float hi[kCols], lo[kCols];
+        ptx::tmem_read2<kCols>(taddr, taddr + kTp, hi, lo);
+        const uint64_t row2 = two(row_scale, row_scale), sixteenth = two(0.0625f, 0.0625f);
 #pragma unroll
-        for (int c = 0; c < kTp; c += kCols) {
-            if (((mask >> c) & ((1u << kCols) - 1u)) == 0) continue;
-            float hi[kCols], lo[kCols];
-            ptx::tmem_read2<kCols>(taddr + c, taddr + kTp + c, hi, lo);
+        for (int t = 0; t < kCols; t += 4) {
+            const float4 sc = *reinterpret_cast<const float4*>(token_scale + t);
 #pragma unroll
-            for (int t = 0; t < kCols; t += 4) {
-                const float4 sc = *reinterpret_cast<const float4*>(token_scale + c + t);
-                const float s4[4] = {sc.x, sc.y, sc.z, sc.w};
+            for (int i = 0; i < 4; i += 2) {
+                const uint64_t scale = fma2(i == 0 ? two(sc.x, sc.y) : two(sc.z, sc.w), row2, 0);
+                const uint64_t x = fma2(two(lo[t + i], lo[t + i + 1]), sixteenth, two(hi[t + i], hi[t + i + 1]));
+                const uint64_t v = fma2(x, scale, two(sum[t + i], sum[t + i + 1]));
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if ((mask >> (c + t + i)) & 1u) sum[c + t + i] = fmaf(fmaf(lo[t + i], 0.0625f, hi[t + i]), s4[i] * row_scale, sum[c + t + i]);
+                for (int h = 0; h < 2; ++h)
+                    if (!kMasked || ((mask >> (t + i + h)) & 1u)) sum[t + i + h] = __uint_as_float(uint32_t(v >> (32 * h)));
             }
         }
     }
 
     __device__ __forceinline__ bool fc1(const Piece& q, float* to) {
         const int j = q.tile / p.tiles1, e = st.hit[j], i = min((q.tile - j * p.tiles1) * kRows + row, p.I - 1);
-        const uint32_t mask = st.hit_mask[j];
-        float g[kTp], v[kTp];
+        const uint32_t mask = (st.hit_mask[j] >> t0) & ((1u << kCols) - 1u);  // the sums of other tokens are not used
+        float g[kCols], v[kCols];
         if constexpr (kFp8) {
 #pragma unroll
-            for (int t = 0; t < kTp; ++t) g[t] = v[t] = 0.0f;
+            for (int t = 0; t < kCols; ++t) g[t] = v[t] = 0.0f;
             float sg = weight_scale(p.b_scale, p.mode, e, 2 * p.I, i, p.kb1, q.lo);
             float sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, q.lo);
             for (int kb = q.lo; kb < q.hi; ++kb) {
@@ -608,26 +627,28 @@ struct Drain {
                     sv = weight_scale(p.b_scale, p.mode, e, 2 * p.I, p.I + i, p.kb1, kb + 1);
                 }
                 if (!acquire()) return false;
-                add_scaled(buffer(), token_scale(), gs, mask, g);
-                add_scaled(buffer() + S::kN1, token_scale(), vs, mask, v);
+                if (mask != 0) {
+                    add_scaled<false>(buffer(), token_scale(), gs, mask, g);
+                    add_scaled<false>(buffer() + S::kN1, token_scale(), vs, mask, v);
+                }
                 release();
             }
         } else {
             if (!acquire()) return false;
-            ptx::tmem_read2<kTp>(buffer(), buffer() + S::kN1, g, v);
+            ptx::tmem_read2<kCols>(buffer(), buffer() + S::kN1, g, v);
             release();
         }
-        put_sums<kTp>(to, row, mask, g);
-        put_sums<kTp>(to + kTp * kRows, row, mask, v);
+        put_sums<kCols>(to + t0 * kRows, row, mask, g);
+        put_sums<kCols>(to + (kTp + t0) * kRows, row, mask, v);
         return true;
     }
 
     __device__ __forceinline__ bool fc2(const Piece& q, float* to) {
         const int kb2 = (p.I + S::kKElems - 1) / S::kKElems;
         const int h = min(q.tile * kRows + row, p.H - 1);
-        float sum[kTp];
+        float sum[kCols];
 #pragma unroll
-        for (int t = 0; t < kTp; ++t) sum[t] = 0.0f;
+        for (int t = 0; t < kCols; ++t) sum[t] = 0.0f;
         if constexpr (kFp8) {
             auto scale_of = [&](int u, int half) {
                 const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2 + half;
@@ -639,10 +660,12 @@ struct Drain {
                 const int j = u / p.pairs2, kb = (u - j * p.pairs2) * 2;
                 const float s0 = next0, s1 = next1;
                 if (u + 1 < q.hi) next0 = scale_of(u + 1, 0), next1 = scale_of(u + 1, 1);
-                const uint32_t mask = st.hit_mask[j];
+                const uint32_t mask = (st.hit_mask[j] >> t0) & ((1u << kCols) - 1u);
                 if (!acquire()) return false;
-                add_scaled(buffer(), token_scale(), s0, mask, sum);
-                if (kb + 1 < kb2) add_scaled(buffer() + S::kN2, token_scale() + kTp, s1, mask, sum);  // nothing was laid out for a block past I
+                if (mask != 0) {
+                    add_scaled<true>(buffer(), token_scale(), s0, mask, sum);
+                    if (kb + 1 < kb2) add_scaled<true>(buffer() + S::kN2, token_scale() + kTp, s1, mask, sum);  // nothing was laid out past I
+                }
                 release();
             }
         } else {
@@ -650,16 +673,16 @@ struct Drain {
                 const int j = u / p.pairs2;
                 u = min(q.hi, (j + 1) * p.pairs2);
                 if (!acquire()) return false;
-                float hi[kTp], lo[kTp];
-                ptx::tmem_read2<kTp>(buffer(), buffer() + kTp, hi, lo);
+                float hi[kCols], lo[kCols];
+                ptx::tmem_read2<kCols>(buffer(), buffer() + kTp, hi, lo);
                 release();
-                const uint32_t mask = st.hit_mask[j];
+                const uint32_t mask = st.hit_mask[j] >> t0;
 #pragma unroll
-                for (int t = 0; t < kTp; ++t)
+                for (int t = 0; t < kCols; ++t)
                     if ((mask >> t) & 1u) sum[t] += hi[t] + lo[t];
             }
         }
-        put_sums<kTp>(to, row, all_tokens(p), sum);
+        put_sums<kCols>(to + t0 * kRows, row, all_tokens(p) >> t0, sum);
         return true;
     }
 
@@ -866,7 +889,7 @@ struct Finish {
 // Chosen experts of every token into shared memory, and the list of experts that any token chose, shared ones at its end.
 template <int kPerLane>
 __device__ __forceinline__ void choose_topk(const Params& p, Tail& st, int warp, int lane) {
-    for (int t = warp; t < p.T; t += kThreads / 32) {
+    for (int t = warp; t < p.T; t += int(blockDim.x >> 5)) {
         int* index = st.topk_index[t];
         float* weight = st.topk_weight[t];
         route::topk_of_token<kPerLane>(p.logits + size_t(t) * p.E, p.E, p.k, p.k, p.scoring, lane, index, weight);
@@ -904,7 +927,7 @@ __device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int 
 }
 
 template <bool kFp8, int kTp>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads(kTp), 1)
 moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ Params p) {
     using S = Shape<kFp8, kTp>;
     pdl_launch();
@@ -920,14 +943,14 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         }
         for (int i = 0; i < 4; ++i) {
             ptx::mbar_init(&st.tmem_full[i], kFp8 ? 2 : 1);  // the MMAs, and the scales
-            ptx::mbar_init(&st.tmem_empty[i], 4);
+            ptx::mbar_init(&st.tmem_empty[i], S::kDrainWarps);
         }
         for (int i = 0; i < kClaims; ++i) {
             ptx::mbar_init(&st.claim_full[i], 1);
-            ptx::mbar_init(&st.claim_empty[i], 6);  // tokens, MMA, draining warps
+            ptx::mbar_init(&st.claim_empty[i], 2 + S::kDrainWarps);  // tokens, MMA, draining warps
         }
         for (int i = 0; i < kJobs; ++i) {
-            ptx::mbar_init(&st.job_full[i], 4);
+            ptx::mbar_init(&st.job_full[i], S::kDrainWarps);
             ptx::mbar_init(&st.job_empty[i], 4);   // the finishing warps, or the counting thread for them
             ptx::mbar_init(&st.last_full[i], 1);
         }
@@ -939,7 +962,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         ptx::tmem_alloc(&st.tmem_base, S::kTmemCols);
         ptx::tmem_relinquish();
     }
-    for (int i = threadIdx.x; i < p.E; i += kThreads) st.mask[i] = 0;
+    for (int i = threadIdx.x; i < p.E; i += threads(kTp)) st.mask[i] = 0;
     if (threadIdx.x == 0) st.bad_tokens = 0;
     ptx::tc_fence_before();
     __syncthreads();
@@ -955,7 +978,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
 
     if (st.n_hit == 0) {  // no token has an expert
-        for (int i = blockIdx.x * kThreads + threadIdx.x; i < p.T * p.H; i += gridDim.x * kThreads)
+        for (int i = blockIdx.x * threads(kTp) + threadIdx.x; i < p.T * p.H; i += gridDim.x * threads(kTp))
             p.out[i] = __float2bfloat16_rn((st.bad_tokens >> (i / p.H)) & 1u ? __uint_as_float(0x7fffffffu) : 0.0f);
     } else if (warp == 0) {
         if (ptx::elect_one()) load_weights<kFp8, kTp>(p, map_b, map_b1, st, ring, claim);
@@ -968,11 +991,12 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
     } else if (warp == 3) {
         if (ptx::elect_one()) count_pieces(p, st);
         __syncwarp();
-    } else if (warp >= 8) {
+    } else if (warp >= 8 && warp < 12) {
         Finish<kFp8, kTp> f{p, st, warp - 8, lane, (warp - 8) * 32 + lane};
         f.run();
     } else if (warp >= 4) {
-        Drain<kFp8, kTp> d{p, st, tmem + (uint32_t((warp - 4) * 32) << 16), warp - 4, lane, (warp - 4) * 32 + lane};
+        const int quarter = warp & 3;  // of TMEM's lanes, that a warp may read
+        Drain<kFp8, kTp> d{p, st, tmem + (uint32_t(quarter * 32) << 16), warp - 4, lane, quarter * 32 + lane, warp >= 12 ? 16 : 0};
         d.run();
     }
     __syncthreads();
@@ -1051,7 +1075,7 @@ static int opt_in(K kern, int which) {
 template <bool kFp8, int kTp>
 static int launch_experts(const CUtensorMap& b, const CUtensorMap& b1, const Params& p, cudaStream_t stream) {
     DQ_RC(opt_in(moe_decode_experts_kernel<kFp8, kTp>, (kFp8 ? 3 : 0) + (kTp == 8 ? 0 : kTp == 16 ? 1 : 2)));
-    return launch_pdl(moe_decode_experts_kernel<kFp8, kTp>, dim3(p.blocks), kThreads, kSmemBytes, stream, b, b1, p);
+    return launch_pdl(moe_decode_experts_kernel<kFp8, kTp>, dim3(p.blocks), threads(kTp), kSmemBytes, stream, b, b1, p);
 }
 
 template <bool kF32, bool kFp8>
