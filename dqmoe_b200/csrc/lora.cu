@@ -330,41 +330,43 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 // ---------------------------------------------------------------- project
 
 constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warp 2 list of the adapters' products, warps 4..11 epilogue
-constexpr int kMaxTok = 224;                    // two accumulators of a tile leave 64 columns of TMEM for four products of 16 rows
-constexpr int kTmemCols = 512;
+constexpr int kMaxTok = 256;
+constexpr int kTmemCols = 512;                  // two accumulators
 constexpr int kRingBytes = 200 * 1024;
 constexpr int kMaxStages = 10;
 constexpr int kChunk = 16;                      // rows of x that are looked at together
-constexpr int kMaxSlots = 8;
-constexpr int kAtOnce = 5;                      // parts of a tile that are loaded at once
+constexpr int kProducts = 4;                    // steps of the mixed rows' products that are loaded at once
+constexpr int kMaxParts = 16;
 
 struct Params {
     const int* ids;
+    const uint16_t* lora_b;   // [L, N, R]
+    const uint16_t* z;        // [T, R]
     const float* z_scale;     // null unless fp16
     const float* bias;        // [N] or null
     uint16_t* y;
     int64_t ldy;
     int T, N, K, L, R;
-    int tok;                  // rows of x per tile, a multiple of 16
+    int tok;                  // rows of x per tile, a multiple of 16, on pairs of 32
     int stages;
-    int slots;                // accumulators of 16 columns for the products of mixed rows, for each half of the epilogue
     int n_tiles, tiles;       // tiles along N, and in all
     int kbs;
-    int whole;                // tiles that are not split: block b takes b, b + grid, ...; the others are cut into equal shares
-    int shares;               // of the others
-    int* counters;            // parts seen of each split tile
-    float* part;              // [shares][2] sums of a part of a tile, four rows of x together: [tok / 4][128][4]
+    int groups;               // blocks, or pairs of them
+    int whole;                // tiles that are not split: group g takes g, g + groups, ...
+    int parts;                // of each of the others, a group each
+    int* counters;            // parts seen of each split tile, on pairs of each half of it
+    float* part;              // [block] sums of a part of a tile, four rows of x together: [tok / 4][128][4]
     int* status;
 };
 
-// Products of a part of a tile. Direct: adapter, first chunk | chunks << 8, all of whose rows have it. Mixed: adapter, chunk | its rows << 16.
+// Products of a part of a tile. Direct: adapter, first chunk | chunks << 8, all of whose rows have it. Mixed, by the half of the epilogue that has
+// the chunk: adapter, chunk | its rows << 16.
 struct List {
-    int direct0, direct1, mixed0, mixed1;
-    uint2 direct[kMaxTok / kChunk], mixed[kMaxTok];
+    int direct0, direct1, mixed0[2], mixed1[2];
+    uint2 direct[kMaxTok / kChunk], mixed[2][kMaxTok / 2];
 };
 struct alignas(16) Tail {
     uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2];
-    uint64_t slot_full[2][kMaxSlots], slot_empty[2][kMaxSlots];  // by half of the epilogue
     uint64_t list_full[2], list_empty[2];
     uint64_t meet;            // the epilogue warps
     uint32_t tmem_base;
@@ -377,40 +379,32 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 
 struct Piece {
     int tile, kb0, kb1;
-    int part;                 // slot of its partial sums, -1 for a whole tile
     int index, of;            // which of how many parts of its tile
 };
-// The pieces of a block, in order: its whole tiles, then those of its share of the others.
+// The pieces of a group, in order: its whole tiles, then its part of one of the others.
 struct Pieces {
     const Params& p;
-    int whole, u, hi, lo, units;
-    __device__ __forceinline__ explicit Pieces(const Params& p_) : p(p_), whole(blockIdx.x), u(0), hi(0), lo(0), units((p_.tiles - p_.whole) * p_.kbs) {
-        if (int(blockIdx.x) < p.shares) {
-            lo = u = streamk::first_unit(blockIdx.x, p.shares, units);
-            hi = streamk::first_unit(blockIdx.x + 1, p.shares, units);
-        }
-    }
+    int group, tile;
+    __device__ __forceinline__ Pieces(const Params& p_, int group_) : p(p_), group(group_), tile(group_) {}
     __device__ __forceinline__ bool next(Piece* q) {
-        if (whole < p.whole) {
-            *q = Piece{whole, 0, p.kbs, -1, 0, 1};
-            whole += gridDim.x;
+        if (tile < p.whole) {
+            *q = Piece{tile, 0, p.kbs, 0, 1};
+            tile += p.groups;
             return true;
         }
-        if (u >= hi) return false;
-        const int tile = u / p.kbs, end = min(hi, (tile + 1) * p.kbs);
-        const int first = streamk::share_of(tile * p.kbs, p.shares, units), last = streamk::share_of((tile + 1) * p.kbs - 1, p.shares, units);
-        *q = Piece{p.whole + tile, u - tile * p.kbs, end - tile * p.kbs, first == last ? -1 : 2 * int(blockIdx.x) + (tile == lo / p.kbs ? 0 : 1),
-                   int(blockIdx.x) - first, last - first + 1};
-        u = end;
+        if (left() == 0) return false;
+        const int split = group / p.parts, index = group - split * p.parts;
+        *q = Piece{p.whole + split, index * p.kbs / p.parts, (index + 1) * p.kbs / p.parts, index, p.parts};
+        tile = 0x7fffffff;
         return true;
     }
-    __device__ __forceinline__ int left() const { return (whole < p.whole ? 1 : 0) + (u < hi ? 1 : 0); }  // 0: none
+    __device__ __forceinline__ int left() const { return tile < p.whole || (tile != 0x7fffffff && group < (p.tiles - p.whole) * p.parts) ? 1 : 0; }  // 0: none
 };
 
 // The adapters' products of a tile's rows, by one warp, and which of them belong to this part.
-template <bool kHalf>
+template <bool kHalf, bool kPair>
 __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane) {
-    int direct = 0, mixed = 0, last = -1, last_end = -1, last_first = 0;
+    int direct = 0, mixed0 = 0, mixed1 = 0, last = -1, last_end = -1, last_first = 0;
     const int rows = min(p.tok, p.T - t0), half = lane >> 4;
     int ids[kMaxTok / 32];
     uint32_t scaled_rows = 0;  // bit c: this lane's row of the c-th pair of chunks has a power of two
@@ -433,46 +427,55 @@ __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, cons
         if (with == 0) continue;
         const uint32_t scales = __ballot_sync(0xffffffffu, scaled);
         const uint32_t peers = __match_any_sync(0xffffffffu, 2 * id + half) >> (16 * half);  // of this half
-        bool mixes[2];
+        bool whole[2], mixes[2];  // whether a chunk has one adapter; whether it has any and is not a direct product
+        int a[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t here = 0xffffu << (16 * h);
-            mixes[h] = false;
-            if ((with & here) == 0) continue;
-            const int a = __shfl_sync(0xffffffffu, id, __ffs(with & here) - 1);
-            const uint32_t same = __ballot_sync(0xffffffffu, id == a) & here;
-            mixes[h] = same != (present & here) || (scales & here) != 0;
-            if (mixes[h]) continue;
-            if (a != last || c + h != last_end) {
-                last = a;
+            a[h] = __shfl_sync(0xffffffffu, id, (with & here) != 0 ? __ffs(with & here) - 1 : 0);
+            const uint32_t same = __ballot_sync(0xffffffffu, id == a[h]) & here;
+            whole[h] = (with & here) != 0 && same == (present & here) && (scales & here) == 0;
+        }
+        if constexpr (kPair) {  // both or neither: such products have 32 rows at least
+            const bool both = whole[0] && (whole[1] ? a[0] == a[1] : (present >> 16) == 0);
+            whole[0] = whole[1] = both;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            mixes[h] = (with & (0xffffu << (16 * h))) != 0 && !whole[h];
+            if (!whole[h]) continue;
+            if (a[kPair ? 0 : h] != last || c + h != last_end) {
+                last = a[kPair ? 0 : h];
                 last_first = c + h;
                 ++direct;
             }
             last_end = c + h + 1;
-            if (lane == 0) l.direct[direct - 1] = make_uint2(uint32_t(a), uint32_t(last_first | ((last_end - last_first) << 8)));
+            if (lane == 0) l.direct[direct - 1] = make_uint2(uint32_t(last), uint32_t(last_first | ((last_end - last_first) << 8)));
         }
-        // the two chunks' products in turn: the two halves of the epilogue work side by side
         const bool leads = id >= 0 && (lane & 15) == __ffs(peers) - 1 && (half ? mixes[1] : mixes[0]);
         const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
-        const int n0 = __popc(leaders & 0xffffu), n1 = __popc(leaders >> 16);
-        const int r = __popc((leaders >> (16 * half)) & ((1u << (lane & 15)) - 1u));
-        if (leads) l.mixed[mixed + r + (half ? min(r + 1, n0) : min(r, n1))] = make_uint2(uint32_t(id), uint32_t(c + half) | (peers << 16));
-        mixed += n0 + n1;
+        const int at = (half ? mixed1 : mixed0) + __popc((leaders >> (16 * half)) & ((1u << (lane & 15)) - 1u));
+        if (leads) l.mixed[half][at] = make_uint2(uint32_t(id), uint32_t(c + half) | (peers << 16));
+        mixed0 += __popc(leaders & 0xffffu);
+        mixed1 += __popc(leaders >> 16);
     }
     if (lane == 0) {
         l.direct0 = direct * q.index / q.of;
         l.direct1 = direct * (q.index + 1) / q.of;
-        l.mixed0 = mixed * q.index / q.of;
-        l.mixed1 = mixed * (q.index + 1) / q.of;
+        l.mixed0[0] = mixed0 * q.index / q.of;
+        l.mixed1[0] = mixed0 * (q.index + 1) / q.of;
+        l.mixed0[1] = mixed1 * q.index / q.of;
+        l.mixed1[1] = mixed1 * (q.index + 1) / q.of;
     }
 }
 
-template <bool kHalf>
+template <bool kHalf, bool kPair>
 struct Epilogue {
     const Params& p;
     Tail& st;
     uint32_t tmem;            // this warp's lanes
-    int warp, lane, row;      // warp 0..7, row = TMEM lane = row of W in the tile
+    int warp, lane, row;      // warp 0..7, row = TMEM lane = row of W among the block's 128 of the tile
+    int rank;                 // of the block in its pair
     uint32_t meetings = 0;
 
     __device__ __forceinline__ bool meet() {
@@ -490,110 +493,197 @@ struct Epilogue {
             if (t0 + j < p.T) y[j * p.ldy] = to_bits(v[j] + bias, kHalf);
     }
 
-    // The sums of a tile from its parts, in their order, some of them loaded at once.
-    __device__ __forceinline__ void add_parts(int slot0, int first, int last, int half, int cols, int t0, int n) {
+    // The same from the accumulators of m16n8k16 products, of the 32 rows of W from n0 on.
+    __device__ __forceinline__ void store_fragments(const float (&v)[kChunk], int t0, int n0) {
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            const int n = n0 + (i >> 3) * 16 + ((i >> 1) & 1) * 8 + (lane >> 2), t = t0 + ((i >> 2) & 1) * 8 + (lane & 3) * 2 + (i & 1);
+            if (n < p.N && t < p.T) p.y[int64_t(t) * p.ldy + n] = to_bits(v[i] + (p.bias != nullptr ? p.bias[n] : 0.0f), kHalf);
+        }
+    }
+
+    // The adapters' products of the mixed rows of a chunk, from place `e` of the list on: B's rows are the products' rows, z's rows their columns, of
+    // which each takes the columns that have its adapter. Operands straight from L2 into registers, where 16 bytes of a row are eight values that
+    // follow one another; which of them a product takes for its k is the same for both, and a sum does not mind. Steps are 32 of R.
+    __device__ __forceinline__ void products(const List& l, int half, int* e, int chunk, int t0, int n0, float (&v)[kChunk]) {
+        const int end = l.mixed1[half], rank_steps = (p.R + 31) / 32, k_lane = (lane & 3) * 8, g = lane >> 2;
+        int to = *e;
+        while (to < end && int(l.mixed[half][to].y & 0xff) == chunk) ++to;
+        int load = *e, load_k = 0, use = *e, use_k = 0;
+        float d[kChunk];
 #pragma unroll 1
-        for (int c = half; c * kChunk < cols; c += 2) {
-            const float* from = p.part + c * kChunk * kRows + row * 4;
-            const size_t stride = size_t(p.tok) * kRows;
-            float v[kChunk];
+        for (int left = (to - *e) * rank_steps; left > 0; left -= kProducts) {
+            uint4 b[kProducts][4], z[kProducts][2];
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
-#pragma unroll 1
-            for (int o0 = first; o0 <= last; o0 += kAtOnce) {
-                float4 f[kAtOnce][kChunk / 4];
+            for (int i = 0; i < kProducts; ++i) {
+                const uint2 q = i < left ? l.mixed[half][load] : make_uint2(0, 0);
+                const int k = load_k * 32 + k_lane;
+                const bool in = i < left && k < p.R;
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i) {
-                    const float* part = from + (o0 + i == first ? slot0 : 2 * (o0 + i)) * stride;
-#pragma unroll
-                    for (int j = 0; j < kChunk / 4; ++j)
-                        f[i][j] = o0 + i <= last && c * kChunk + 4 * j < cols ? streamk::ld_partial4(part + 4 * j * kRows) : make_float4(0, 0, 0, 0);
+                for (int j = 0; j < 4; ++j) {
+                    const int n = n0 + j * 8 + g;
+                    b[i][j] = in && n < p.N ? load16(p.lora_b + (size_t(q.x) * p.N + n) * p.R + k) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < kAtOnce; ++i)
-#pragma unroll
-                    for (int j = 0; j < kChunk / 4; ++j)
-                        v[4 * j] += f[i][j].x, v[4 * j + 1] += f[i][j].y, v[4 * j + 2] += f[i][j].z, v[4 * j + 3] += f[i][j].w;
+                for (int h = 0; h < 2; ++h) {
+                    const int t = t0 + h * 8 + g;
+                    z[i][h] = in && ((q.y >> (16 + 8 * h + g)) & 1u) ? load16(p.z + size_t(t) * p.R + k) : make_uint4(0, 0, 0, 0);
+                }
+                if (++load_k == rank_steps) load_k = 0, ++load;
             }
-            store(v, t0 + c * kChunk, n);
+#pragma unroll
+            for (int i = 0; i < kProducts; ++i) {
+                if (i >= left) break;
+                if (use_k == 0)
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) d[j] = 0.0f;
+                const uint32_t rows = l.mixed[half][use].y >> 16;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if ((rows >> (8 * h)) & 255u)
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            float* c = d + (2 * m + h) * 4;
+                            ptx::mma_16x8x16<kHalf>(c, b[i][2 * m].x, b[i][2 * m + 1].x, b[i][2 * m].y, b[i][2 * m + 1].y, z[i][h].x, z[i][h].y);
+                            ptx::mma_16x8x16<kHalf>(c, b[i][2 * m].z, b[i][2 * m + 1].z, b[i][2 * m].w, b[i][2 * m + 1].w, z[i][h].z, z[i][h].w);
+                        }
+                if (++use_k < rank_steps) continue;
+                use_k = 0, ++use;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    const int column = ((j >> 2) & 1) * 8 + (lane & 3) * 2 + (j & 1);
+                    if ((rows >> column) & 1u) v[j] = kHalf ? d[j] * p.z_scale[t0 + column] : d[j];
+                }
+            }
+        }
+        *e = to;
+    }
+    static __device__ __forceinline__ uint4 load16(const uint16_t* from) {  // past L1: written while this kernel was here already
+        uint4 v;
+        asm volatile("ld.relaxed.gpu.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from) : "memory");
+        return v;
+    }
+
+    // The sums of a tile from its parts, in their order: kParts parts of kChunks chunks of this half are loaded at once.
+    template <int kParts, int kChunks>
+    __device__ __forceinline__ void add_parts(const float* part, int parts, size_t stride, int half, int cols, int t0, int n) {
+#pragma unroll 1
+        for (int c = half; c * kChunk < cols; c += 2 * kChunks) {
+            const float* from = part + c * kChunk * kRows + row * 4;
+            float v[kChunks][kChunk];
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) v[i][j] = 0.0f;
+#pragma unroll 1
+            for (int o = 0; o < parts; o += kParts) {
+                float4 f[kParts][kChunks][kChunk / 4];
+#pragma unroll
+                for (int k = 0; k < kParts; ++k)
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                        for (int j = 0; j < kChunk / 4; ++j)
+                            f[k][i][j] = o + k < parts && (c + 2 * i) * kChunk + 4 * j < cols
+                                             ? streamk::ld_partial4(from + (o + k) * stride + (2 * i * kChunk + 4 * j) * kRows) : make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < kParts; ++k)
+#pragma unroll
+                    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+                        for (int j = 0; j < kChunk / 4; ++j)
+                            v[i][4 * j] += f[k][i][j].x, v[i][4 * j + 1] += f[k][i][j].y, v[i][4 * j + 2] += f[k][i][j].z, v[i][4 * j + 3] += f[k][i][j].w;
+            }
+#pragma unroll
+            for (int i = 0; i < kChunks; ++i)
+                if ((c + 2 * i) * kChunk < cols) store(v[i], t0 + (c + 2 * i) * kChunk, n);  // behind the tile begin the next one's rows
         }
     }
 
     __device__ __forceinline__ void run() {
         pdl_wait();  // shrink: the counters, z_scale
-        Pieces pieces(p);
+        const int group = int(blockIdx.x) >> (kPair ? 1 : 0);
+        Pieces pieces(p, group);
         Piece q;
         const int half = warp >> 2;
-        int slot_it = 0;
         for (int acc = 0; pieces.next(&q); ++acc) {
-            const int tt = q.tile / p.n_tiles, n = (q.tile - tt * p.n_tiles) * kRows + row, t0 = tt * p.tok;
+            const int tt = q.tile / p.n_tiles, n = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows + row, t0 = tt * p.tok;
             const int buf = acc & 1, parity = (acc >> 1) & 1;
-            if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
             if (!ptx::mbar_wait_warp(&st.list_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
-            ptx::tc_fence_after();
             const List& l = st.list[buf];
             // columns in use; the two halves of the epilogue take chunks in turn
-            const int cols = min(p.tok, p.T - t0), mixed1 = l.mixed1;
-            int e = l.mixed0;
+            const int cols = min(p.tok, p.T - t0), n0 = n - lane;
+            int e = l.mixed0[half];
+            bool full = false;
             for (int c = half; c * kChunk < cols; c += 2) {
-                float v[kChunk];
-                ptx::tmem_read<kChunk>(tmem + buf * p.tok + c * kChunk, v);
-                for (; e < mixed1 && int(l.mixed[e].y & 0xff) <= (c | 1); ++e) {  // this chunk's and its neighbour's, in turn
-                    if (int(l.mixed[e].y & 0xff) != c) continue;
-                    const int slot = slot_it % p.slots;
-                    if (!ptx::mbar_wait_warp(&st.slot_full[half][slot], (slot_it / p.slots) & 1, &st.abort_flag, kWaitLimit)) return;
+                float v[kChunk], d[kChunk];
+                const bool mixed = e < l.mixed1[half] && int(l.mixed[half][e].y & 0xff) == c;
+                if (mixed) {  // the first chunk's while the tensor core still sums
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) d[j] = 0.0f;
+                    products(l, half, &e, c, t0 + c * kChunk, n0, d);
+                }
+                if (!full) {
+                    if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
                     ptx::tc_fence_after();
-                    float d[kChunk];
-                    ptx::tmem_read<kChunk>(tmem + 2 * p.tok + (half * p.slots + slot) * kChunk, d);
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(&st.slot_empty[half][slot]);
-                    ++slot_it;
-                    const uint32_t rows = l.mixed[e].y >> 16;
-                    if constexpr (kHalf) {
-                        const float mine = (rows >> (lane & 15)) & 1u ? p.z_scale[t0 + c * kChunk + (lane & 15)] : 0.0f;
+                    full = true;
+                }
+                float* to = p.part + (size_t(blockIdx.x) * p.tok + c * kChunk) * kRows;
+                if (mixed) {
+                    ptx::tmem_read_fragments(tmem + buf * p.tok + c * kChunk, v);
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) {
-                            const float s = __shfl_sync(0xffffffffu, mine, j);
-                            if ((rows >> j) & 1u) v[j] = fmaf(d[j], s, v[j]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kChunk; ++j)
-                            if ((rows >> j) & 1u) v[j] += d[j];
+                    for (int j = 0; j < kChunk; ++j) v[j] += d[j];
+                    if (q.of == 1) {
+                        store_fragments(v, t0 + c * kChunk, n0);
+                        continue;
                     }
-                }
-                if (q.part < 0) {
-                    store(v, t0 + c * kChunk, n);
-                } else {
-                    float* to = p.part + (size_t(q.part) * p.tok + c * kChunk) * kRows + row * 4;
 #pragma unroll
-                    for (int j = 0; j < kChunk; j += 4)
-                        if (c * kChunk + j < cols) *reinterpret_cast<float4*>(to + j * kRows) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    for (int j = 0; j < kChunk; j += 2) {
+                        const int r = row - lane + (j >> 3) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2), t = ((j >> 2) & 1) * 8 + (lane & 3) * 2;
+                        if (c * kChunk + (t & ~3) < cols) *reinterpret_cast<float2*>(to + (t & ~3) * kRows + r * 4 + (t & 3)) = make_float2(v[j], v[j + 1]);
+                    }
+                    continue;
                 }
+                ptx::tmem_read<kChunk>(tmem + buf * p.tok + c * kChunk, v);
+                if (q.of == 1) {
+                    store(v, t0 + c * kChunk, n);
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < kChunk; j += 4)
+                    if (c * kChunk + j < cols) *reinterpret_cast<float4*>(to + j * kRows + row * 4) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             }
+            // also a half without a chunk waits, so that it does not run ahead of the tensor core
+            if (!full && !ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                ptx::mbar_arrive(&st.tmem_empty[buf]);
+                if constexpr (kPair) ptx::mbar_arrive_cluster(ptx::map_to_cta(&st.tmem_empty[buf], 0));
+                else ptx::mbar_arrive(&st.tmem_empty[buf]);
                 ptx::mbar_arrive(&st.list_empty[buf]);
             }
-            if (q.part < 0) continue;
+            if (q.of == 1) continue;
             // What the warps wrote, the counting thread has seen at `meet`, and its release and acquire at gpu scope hold for all of them: a fence in
             // each thread, before and after, took 1 and 3 to 6 us.
-            const int local = q.tile - p.whole, first = int(blockIdx.x) - q.index, last = first + q.of - 1;
+            const int first = kPair ? (group - q.index) * 2 + rank : group - q.index;
             if (!meet()) return;
-            if (warp == 0 && lane == 0) st.last_part = streamk::atomic_add_acq_rel_gpu(&p.counters[local], 1) == q.of - 1;
+            if (warp == 0 && lane == 0) {
+                int* counter = &p.counters[kPair ? (q.tile - p.whole) * 2 + rank : q.tile - p.whole];
+                st.last_part = streamk::atomic_add_acq_rel_gpu(counter, 1) == q.of - 1;
+            }
             if (!meet()) return;
             if (*const_cast<volatile int*>(&st.last_part) == 0) continue;
-            // only the first part may be its share's second tile
-            const int slot0 = 2 * first + (local == streamk::first_unit(first, p.shares, pieces.units) / p.kbs ? 0 : 1);
-            add_parts(slot0, first, last, half, cols, t0, n);
+            const size_t stride = size_t(kPair ? 2 : 1) * p.tok * kRows;
+            const float* from = p.part + size_t(first) * p.tok * kRows;
+            if (q.of == 2) add_parts<2, 2>(from, q.of, stride, half, cols, t0, n);
+            else add_parts<5, 1>(from, q.of, stride, half, cols, t0, n);
         }
     }
 };
 
-template <bool kHalf>
+// kPair: two blocks of a cluster have 128 rows of W each of a tile of 256 and half of its rows of x; the first one issues the MMAs for both and owns
+// the barriers of the stages.
+template <bool kHalf, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
 lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_z,
                     const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Params p) {
@@ -601,7 +691,9 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     extern __shared__ uint8_t smem_raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stage = kABytes + p.tok * kKBytes;
+    const int rank = kPair ? int(ptx::cluster_ctarank()) : 0, group = int(blockIdx.x) >> (kPair ? 1 : 0);
+    const int x_rows = kPair ? p.tok / 2 : p.tok;  // of this block
+    const int stage = kABytes + x_rows * kKBytes;
     Tail& st = *reinterpret_cast<Tail*>(ring + p.stages * stage);
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
@@ -610,64 +702,72 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&st.tmem_full[i], 1);
-            ptx::mbar_init(&st.tmem_empty[i], 8);
+            ptx::mbar_init(&st.tmem_empty[i], kPair ? 16 : 8);
             ptx::mbar_init(&st.list_full[i], 1);
-            ptx::mbar_init(&st.list_empty[i], 10);  // TMA thread, MMA thread, epilogue warps
-        }
-        for (int i = 0; i < 2 * kMaxSlots; ++i) {
-            ptx::mbar_init(&st.slot_full[0][i], 1);
-            ptx::mbar_init(&st.slot_empty[0][i], 4);
+            ptx::mbar_init(&st.list_empty[i], rank == 0 ? 10 : 9);  // TMA thread, the first block's MMA thread, epilogue warps
         }
         ptx::mbar_init(&st.meet, 8);
         st.abort_flag = 0;
         ptx::fence_barrier_init();
     }
+    if constexpr (kPair) ptx::cluster_sync();  // the other block's barriers exist before anything signals them
     if (warp == 1) {
-        ptx::tmem_alloc(&st.tmem_base, kTmemCols);
-        ptx::tmem_relinquish();
+        if constexpr (kPair) {
+            ptx::tmem_alloc_pair(&st.tmem_base, kTmemCols);
+            ptx::tmem_relinquish_pair();
+        } else {
+            ptx::tmem_alloc(&st.tmem_base, kTmemCols);
+            ptx::tmem_relinquish();
+        }
     }
     ptx::tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) ptx::cluster_sync();  // both hold their TMEM before the first MMA
     ptx::tc_fence_after();
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
 
     if (warp == 0) {
         if (ptx::elect_one()) {
-            Pieces pieces(p);
+            Pieces pieces(p, group);
             Piece q, held;
             int it = 0;
             bool ok = true, waited = false;
             auto next_stage = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
+            // the barrier of stage s, which expects `bytes` from this block, and on pairs as many from the other one
+            auto expect = [&](int s, uint32_t bytes) {
+                if (rank == 0) ptx::mbar_arrive_expect_tx(&st.full[s], kPair ? 2 * bytes : bytes);
+                return kPair ? ptx::map_to_cta(&st.full[s], 0) : ptx::smem_u32(&st.full[s]);
+            };
             auto sums = [&](const Piece& q) {  // x W^T
-                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows, t0 = tt * p.tok;
+                const int tt = q.tile / p.n_tiles, n0 = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows, t0 = tt * p.tok + rank * x_rows;
                 for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
                     if (!next_stage()) return false;
                     const int s = it % p.stages;
-                    ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(stage));
-                    ptx::tma_load_2d(ring + s * stage, &map_w, kb * kKElems, n0, &st.full[s]);
-                    ptx::tma_load_2d(ring + s * stage + kABytes, &map_x, kb * kKElems, t0, &st.full[s]);
+                    const uint32_t bar = expect(s, uint32_t(stage));
+                    ptx::tma_load_2d_any<kPair>(ring + s * stage, &map_w, kb * kKElems, n0, bar);
+                    ptx::tma_load_2d_any<kPair>(ring + s * stage + kABytes, &map_x, kb * kKElems, t0, bar);
                 }
                 return true;
             };
             auto products = [&](const Piece& q, int n) {  // z B^T
-                const int tt = q.tile / p.n_tiles, n0 = (q.tile - tt * p.n_tiles) * kRows, t0 = tt * p.tok;
+                const int tt = q.tile / p.n_tiles, n0 = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows, t0 = tt * p.tok;
                 if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit)) return false;
                 const List& l = st.list[n & 1];
-                const int direct = l.direct1 - l.direct0, all = direct + l.mixed1 - l.mixed0;
-                if (all > 0 && !waited) {
+                if (l.direct0 < l.direct1 && !waited) {
                     pdl_wait();  // shrink: z
                     waited = true;
                 }
-                for (int i = 0; i < all; ++i) {
-                    const uint2 e = i < direct ? l.direct[l.direct0 + i] : l.mixed[l.mixed0 + i - direct];
-                    const int c = int(e.y & 0xff), chunks = i < direct ? int(e.y >> 8) : 1;
+                for (int i = l.direct0; i < l.direct1; ++i) {
+                    const uint2 e = l.direct[i];
+                    const int c = int(e.y & 0xff), chunks = int(e.y >> 8);
                     for (int r0 = 0; r0 < p.R; r0 += kKElems, ++it) {
                         if (!next_stage()) return false;
                         const int s = it % p.stages;
-                        ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(kABytes + chunks * kChunk * kKBytes));
-                        ptx::tma_load_3d<false>(ring + s * stage, &map_b, r0, n0, int(e.x), ptx::smem_u32(&st.full[s]));
-                        for (int j = 0; j < chunks; ++j)
-                            ptx::tma_load_2d(ring + s * stage + kABytes + j * kChunk * kKBytes, &map_z, r0, t0 + (c + j) * kChunk, &st.full[s]);
+                        const int mine = kPair ? chunks / 2 : chunks;  // chunks of z that this block loads
+                        const uint32_t bar = expect(s, uint32_t(kABytes + mine * kChunk * kKBytes));
+                        ptx::tma_load_3d<kPair>(ring + s * stage, &map_b, r0, n0, int(e.x), bar);
+                        for (int j = 0; j < mine; ++j)
+                            ptx::tma_load_2d_any<kPair>(ring + s * stage + kABytes + j * kChunk * kKBytes, &map_z, r0, t0 + (c + rank * mine + j) * kChunk, bar);
                     }
                 }
                 ptx::mbar_arrive(&st.list_empty[n & 1]);
@@ -680,21 +780,33 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 if (n == 0 && pieces.left() == 0) ok = ok && products(q, 0);
             }
             if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
-                const long long begin = clock64();
-                for (int i = max(0, it - p.stages); i < it; ++i)
-                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - begin < kWaitLimit) {}
+                if constexpr (kPair) {  // whose barriers are the first block's, which may have got fewer than it expects
+                    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
+                } else {
+                    const long long begin = clock64();
+                    for (int i = max(0, it - p.stages); i < it; ++i)
+                        while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - begin < kWaitLimit) {}
+                }
             }
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (ptx::elect_one()) {
-            Pieces pieces(p);
+        if (rank == 0 && ptx::elect_one()) {
+            Pieces pieces(p, group);
             Piece q;
-            int it = 0, slot_it[2] = {0, 0};
+            int it = 0;
             bool ok = true;
+            auto commit = [&](uint64_t* bar) {  // all MMAs so far
+                if constexpr (kPair) {
+                    ptx::umma_commit_pair(ptx::map_to_cta(bar, 0));
+                    ptx::umma_commit_pair(ptx::map_to_cta(bar, 1));
+                } else {
+                    ptx::umma_commit(bar);
+                }
+            };
             // one stage into the accumulator at `d`, `cols` columns of the second operand
             auto block = [&](uint32_t d, int cols, int steps, bool more) {
-                const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kRows, uint32_t(cols));
+                const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kPair ? 2 * kRows : kRows, uint32_t(cols));
                 const int s = it % p.stages;
                 if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit)) return false;
                 ptx::tc_fence_after();
@@ -702,8 +814,11 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kABytes));
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (k < steps) ptx::umma<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
-                ptx::umma_commit(&st.empty[s]);
+                    if (k < steps) {
+                        if constexpr (kPair) ptx::umma_pair<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
+                        else ptx::umma<1>(d, ptx::smem_desc_advance(da, k * 32), ptx::smem_desc_advance(db, k * 32), idesc, more || k > 0);
+                    }
+                commit(&st.empty[s]);
                 ++it;
                 return true;
             };
@@ -721,16 +836,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     for (int r0 = 0; r0 < p.R; r0 += kKElems)
                         if (!block(tmem + (n & 1) * p.tok + (l.direct[e].y & 0xff) * kChunk, int(l.direct[e].y >> 8) * kChunk, min(4, (p.R - r0 + 15) / 16), true))
                             return false;
-                ptx::umma_commit(&st.tmem_full[n & 1]);
-                for (int e = l.mixed0; e < l.mixed1; ++e) {
-                    const bool odd = (l.mixed[e].y & 1u) != 0;  // the half of the epilogue that takes the chunk
-                    const int h = odd ? 1 : 0, at = odd ? slot_it[1]++ : slot_it[0]++, slot = at % p.slots;
-                    if (!ptx::mbar_wait(&st.slot_empty[h][slot], ((at / p.slots) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
-                    ptx::tc_fence_after();
-                    for (int r0 = 0; r0 < p.R; r0 += kKElems)
-                        if (!block(tmem + 2 * p.tok + (h * p.slots + slot) * kChunk, kChunk, min(4, (p.R - r0 + 15) / 16), r0 > 0)) return false;
-                    ptx::umma_commit(&st.slot_full[h][slot]);
-                }
+                commit(&st.tmem_full[n & 1]);
                 ptx::mbar_arrive(&st.list_empty[n & 1]);
                 return true;
             };
@@ -743,23 +849,34 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         __syncwarp();
     } else if (warp == 2) {
         if constexpr (kHalf) pdl_wait();  // shrink: z_scale
-        Pieces pieces(p);
+        Pieces pieces(p, group);
         Piece q;
         for (int n = 0; pieces.next(&q); ++n) {
             if (!ptx::mbar_wait_warp(&st.list_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
-            make_list<kHalf>(p, st.list[n & 1], q.tile / p.n_tiles * p.tok, q, lane);
+            List& l = st.list[n & 1];
+            make_list<kHalf, kPair>(p, l, q.tile / p.n_tiles * p.tok, q, lane);
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&st.list_full[n & 1]);
+            // The mixed rows' B towards L2 meanwhile: 128 rows of an adapter's follow one another in memory.
+            const int n0 = ((q.tile % p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows;
+            const uint32_t bytes = uint32_t(max(0, min(kRows, p.N - n0)) * p.R) * 2u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                for (int e = l.mixed0[h] + lane; bytes > 0 && e < l.mixed1[h]; e += 32)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.lora_b + (size_t(l.mixed[h][e].x) * p.N + n0) * p.R), "r"(bytes));
         }
     } else if (warp >= 4) {
-        Epilogue<kHalf> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane};
+        Epilogue<kHalf, kPair> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane, rank};
         ep.run();
     }
+    ptx::tc_fence_before();
     __syncthreads();
+    if constexpr (kPair) ptx::cluster_sync();  // the other block is through with this one's barriers and shared memory
     if (threadIdx.x == 0 && st.abort_flag != 0) *p.status = kStatusProject;
     if (warp == 1) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem, kTmemCols);
+        if constexpr (kPair) ptx::tmem_dealloc_pair(tmem, kTmemCols);
+        else ptx::tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -784,25 +901,50 @@ static int make_map_2d(CUtensorMap* map, const void* base, bool half, int64_t ro
 struct Layout {
     size_t counters, z, z_scale, part, total;
 };
-static Layout plan(Params* p, int T, int N, int K, int R) {
+// Tiles of x's rows, blocks or pairs, and parts, by an estimate in clock cycles, whose constants are fits to measurements (all forms, 1 to 8191
+// rows, N 2880 to 14336, K 2880 to 7168; the form chosen is within 4 % of the fastest): a K block of a tile takes its MMAs (two cycles a row)
+// or its bytes from L2; W and x come from HBM once, and of the two the shorter one costs a quarter of its time beside the longer; a tile's last sums
+// leave TMEM behind the last MMA; parts are written, counted and added. N = K = 4096, us per call without adapters: 1 row 1 part of a tile each
+// 22, 4 parts 12.8; 128 rows in one tile of 4 parts 18.3, in two of 2 parts 17.7; 512 rows in 4 tiles of 128 27.8, with what had one part
+// more or less in each block's share 41.5; 4096 rows on single blocks 110.8, on pairs 103.1.
+constexpr int kL2Bytes[2] = {60, 45};                // per cycle and SM, on single blocks and on pairs
+constexpr int kHbmBytes = 3300;                      // per cycle
+constexpr int kDrain = 12, kCount = 3000, kAdd = 12; // cycles a column; a tile in parts; a column of each part
+constexpr int kPairing = 1500;
+static bool plan_tiles(Params* p) {
+    const int sms = sm_count();
+    const int64_t hbm = (int64_t(p->N) + p->T) * p->K * 2 / kHbmBytes;
+    bool best_pair = false;
+    int64_t best = INT64_MAX;
+    const int fewest = ceil_div(p->T, kMaxTok);
+    for (int pair = 0; pair < 2; ++pair) {
+        const int unit = pair ? 32 : kChunk, groups = sms >> pair, n_tiles = ceil_div(p->N, kRows << pair);
+        for (int tt = fewest; tt < fewest + 8 && (tt == fewest || tt <= ceil_div(p->T, unit)); ++tt) {
+            const int tok = ceil_div(ceil_div(p->T, tt), unit) * unit;
+            const int tiles = n_tiles * ceil_div(p->T, tok), rest = tiles % groups;
+            const int load = (kABytes + (tok * kKBytes >> pair)) / kL2Bytes[pair], kb = tok * 2 > load ? tok * 2 : load;
+            const int most = rest == 0 ? 1 : (groups / rest < kMaxParts ? (groups / rest < p->kbs ? groups / rest : p->kbs) : kMaxParts);
+            for (int parts = 1; parts <= most; ++parts) {
+                const int64_t kbs = int64_t(tiles / groups) * p->kbs + (rest > 0 ? ceil_div(p->kbs, parts) : 0);
+                const int64_t tail = tok * kDrain + (parts > 1 ? kCount + parts * tok * kAdd : 0) + pair * kPairing, sum = kbs * kb;
+                const int64_t cost = (sum > hbm ? sum + hbm / 4 : hbm + sum / 4) + tail;
+                if (cost >= best) continue;
+                best = cost, best_pair = pair != 0;
+                p->tok = tok, p->n_tiles = n_tiles, p->tiles = tiles, p->groups = groups;
+                p->whole = parts > 1 ? tiles - rest : tiles, p->parts = parts;
+            }
+        }
+    }
+    return best_pair;
+}
+static Layout plan(Params* p, int T, int N, int K, int R, bool* pair) {
     T = T > 0 ? T : 1;  // an empty batch is asked about like a row
     p->T = T, p->N = N, p->K = K, p->R = R;
-    // rows spread evenly over the tiles they need
-    p->tok = (ceil_div(T, ceil_div(T, kMaxTok)) + kChunk - 1) / kChunk * kChunk;
-    const int stage = kABytes + p->tok * kKBytes;
-    p->stages = kRingBytes / stage < kMaxStages ? kRingBytes / stage : kMaxStages;
-    p->slots = (kTmemCols - 2 * p->tok) / (2 * kChunk) < kMaxSlots ? (kTmemCols - 2 * p->tok) / (2 * kChunk) : kMaxSlots;
-    p->n_tiles = ceil_div(N, kRows);
-    p->tiles = p->n_tiles * ceil_div(T, p->tok);
     p->kbs = ceil_div(K, kKElems);
-    const int sms = sm_count(), left = p->tiles % sms;
-    // a last round that is three quarters full is left as it is
-    p->whole = left * 4 >= sms * 3 ? p->tiles : p->tiles - left;
-    // The others in equal shares, one per SM; in as many equal parts of each tile as the SMs allow, where that leaves no more than one SM in
-    // seven without work: then no share has two pieces, and no tile more parts than it needs.
-    const int split = p->tiles - p->whole, each = split > 0 ? (sms / split < p->kbs ? sms / split : p->kbs) : 0;
-    const int64_t units = int64_t(split) * p->kbs;
-    p->shares = split * each * 7 >= sms * 6 ? split * each : units < sms ? int(units) : sms;
+    const int sms = sm_count();
+    *pair = plan_tiles(p);
+    const int stage = kABytes + (*pair ? p->tok / 2 : p->tok) * kKBytes;
+    p->stages = kRingBytes / stage < kMaxStages ? kRingBytes / stage : kMaxStages;
     Layout L{};
     size_t off = 0;
     auto add = [&](size_t bytes) {
@@ -811,11 +953,11 @@ static Layout plan(Params* p, int T, int N, int K, int R) {
         return at;
     };
     // for the most that a call of fewer rows splits, so that a workspace for the longest batch serves all
-    const int most = T < kMaxTok ? (T + kChunk - 1) / kChunk * kChunk : kMaxTok;
+    const int most = T < kMaxTok ? (T + 31) / 32 * 32 : kMaxTok;
     L.counters = add(size_t(sms) * sizeof(int));
     L.z = add(size_t(T) * R * 2);
     L.z_scale = add(size_t(T) * sizeof(float));
-    L.part = add(size_t(sms) * 2 * most * kRows * sizeof(float));
+    L.part = add(size_t(sms) * most * kRows * sizeof(float));
     L.total = off;
     return L;
 }
@@ -834,7 +976,7 @@ static int check_sizes(int64_t T, int N, int K, int L, int R) {
 template <class K>
 static int opt_in(K kern, int which, size_t bytes) {
     static std::mutex mu;
-    static size_t configured[3][64] = {};
+    static size_t configured[5][64] = {};
     int dev = 0;
     DQ_CUDA(cudaGetDevice(&dev));
     DQ_CHECK(dev >= 0 && dev < 64);
@@ -868,7 +1010,7 @@ static int launch_shrink(ShrinkParams p, const void* x, cudaStream_t stream) {
     CUtensorMap xs, a;
     DQ_RC(make_map_2d(&xs, x, p.half != 0, p.T, p.K, p.ldx, kShrinkTok));
     DQ_RC(make_map_2d(&a, p.lora_a, p.half != 0, int64_t(p.L) * p.R, p.K, p.K, p.R));
-    DQ_RC(opt_in(lora_shrink_tiles_kernel, 2, size_t(112) * 1024));
+    DQ_RC(opt_in(lora_shrink_tiles_kernel, 4, size_t(112) * 1024));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(tiles) * p.slots * split, 1, 1);
     cfg.blockDim = dim3(kShrinkThreads, 1, 1);
@@ -887,6 +1029,28 @@ static int launch_shrink(ShrinkParams p, const void* x, cudaStream_t stream) {
     return DQMOE_OK;
 }
 
+template <bool kHalf, bool kPair>
+static int launch_project(int groups, size_t smem, cudaStream_t stream, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& z, const CUtensorMap& b,
+                          const Params& p) {
+    DQ_RC(opt_in(lora_project_kernel<kHalf, kPair>, (kHalf ? 1 : 0) + (kPair ? 2 : 0), kSmemBytes));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(groups) << (kPair ? 1 : 0), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = kPair ? 2 : 1;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = kPair ? 2 : 1;
+    DQ_CUDA(cudaLaunchKernelEx(&cfg, lora_project_kernel<kHalf, kPair>, x, w, z, b, p));
+    return DQMOE_OK;
+}
+
 }  // namespace lora
 }  // namespace dq
 
@@ -897,7 +1061,8 @@ extern "C" {
 size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R) {
     if (lora::check_sizes(T, N, K, L, R) != DQMOE_OK) return 0;
     lora::Params p{};
-    return lora::plan(&p, T, N, K, R).total;
+    bool pair;
+    return lora::plan(&p, T, N, K, R, &pair).total;
 }
 
 int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lora_a, const void* lora_b, const int32_t* ids, const float* scale,
@@ -914,7 +1079,8 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     DQ_CHECK_FMT(ldy >= N, "ldy=%lld: at least N", (long long) ldy);
     DQ_CHECK_FMT(workspace != nullptr && is_aligned(workspace, 256), "workspace pointer %p is not aligned!", workspace);
     lora::Params p{};
-    const lora::Layout Y = lora::plan(&p, T, N, K, R);
+    bool pair;
+    const lora::Layout Y = lora::plan(&p, T, N, K, R, &pair);
     if (workspace_bytes != 0 && workspace_bytes < Y.total)
         return fail(DQMOE_ERR_WORKSPACE, __FILE__, __LINE__, "workspace_bytes >= dqmoe_lora_linear_workspace_bytes(...)",
                     "workspace has %zu bytes, the projection needs %zu", workspace_bytes, Y.total);
@@ -928,29 +1094,25 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     sp.ids = ids, sp.scale = scale;
     sp.z = reinterpret_cast<uint16_t*>(ws + Y.z), sp.z_scale = reinterpret_cast<float*>(ws + Y.z_scale);
     sp.counters = reinterpret_cast<int*>(ws + Y.counters);
-    sp.n_counters = p.tiles - p.whole;
+    sp.n_counters = (p.tiles - p.whole) << (pair ? 1 : 0);
     sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status;
 
     CUtensorMap xp, wm, zm, bm;
-    DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, p.tok));
+    DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, pair ? p.tok / 2 : p.tok));
     DQ_RC(lora::make_map_2d(&wm, w, half, N, K, K, lora::kRows));
     DQ_RC(lora::make_map_2d(&zm, sp.z, half, T, R, R, lora::kChunk));
     const cuuint64_t dim[3] = {cuuint64_t(R), cuuint64_t(N), cuuint64_t(L)}, stride[2] = {cuuint64_t(R) * 2, cuuint64_t(N) * R * 2};
     const cuuint32_t box[3] = {lora::kKElems, lora::kRows, 1};
     DQ_RC(lora::make_map(&bm, lora_b, half, 3, dim, stride, box));
     DQ_RC(lora::launch_shrink(sp, x, stream));
-    p.ids = ids, p.z_scale = half ? sp.z_scale : nullptr, p.bias = bias;
+    p.ids = ids, p.lora_b = static_cast<const uint16_t*>(lora_b), p.z = sp.z, p.z_scale = half ? sp.z_scale : nullptr, p.bias = bias;
     p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
     p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
-    const int sms = sm_count();
-    const int grid = p.whole > 0 ? (p.whole < sms ? (p.whole > p.shares ? p.whole : p.shares) : sms) : p.shares;
-    const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + p.tok * lora::kKBytes) + sizeof(lora::Tail);
-    if (half) {
-        DQ_RC(lora::opt_in(lora::lora_project_kernel<true>, 0, lora::kSmemBytes));
-        return launch_pdl(lora::lora_project_kernel<true>, dim3(grid), lora::kThreads, smem, stream, xp, wm, zm, bm, p);
-    }
-    DQ_RC(lora::opt_in(lora::lora_project_kernel<false>, 1, lora::kSmemBytes));
-    return launch_pdl(lora::lora_project_kernel<false>, dim3(grid), lora::kThreads, smem, stream, xp, wm, zm, bm, p);
+    const int split = (p.tiles - p.whole) * p.parts, busy = p.whole < p.groups ? (p.whole > split ? p.whole : split) : p.groups;
+    const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + (pair ? p.tok / 2 : p.tok) * lora::kKBytes) + sizeof(lora::Tail);
+    if (half)
+        return pair ? lora::launch_project<true, true>(busy, smem, stream, xp, wm, zm, bm, p) : lora::launch_project<true, false>(busy, smem, stream, xp, wm, zm, bm, p);
+    return pair ? lora::launch_project<false, true>(busy, smem, stream, xp, wm, zm, bm, p) : lora::launch_project<false, false>(busy, smem, stream, xp, wm, zm, bm, p);
 }
 
 }  // extern "C"

@@ -126,10 +126,6 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&w)[3]) {
         b -= bf16_hi(w[i]);
     }
 }
-__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // This warp's share of the logits of all tokens and eight experts, over chunks of 32 values of H. A thread loads 16 bytes of a row, eight values
 // that follow one another; which of them an MMA takes for its k is the same for x and the weights, and a sum does not mind.
 // Each value of x and each weight is read once per cluster. (With a warp per expert and fp32 FMAs each warp read all of x, and the kernel
@@ -172,8 +168,8 @@ __device__ __forceinline__ void partial_logits(const Params& p, int e0, int firs
         for (int m = 0; m < kM; ++m)
 #pragma unroll
             for (int i = (kF32 ? 2 : 0); i >= 0; --i) {
-                mma_16x8x16(acc[m], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, w[i][0], w[i][1]);
-                mma_16x8x16(acc[m], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, w[i][2], w[i][3]);
+                ptx::mma_16x8x16<false>(acc[m], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, w[i][0], w[i][1]);
+                ptx::mma_16x8x16<false>(acc[m], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, w[i][2], w[i][3]);
             }
     }
 #pragma unroll

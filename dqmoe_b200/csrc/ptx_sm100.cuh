@@ -526,7 +526,7 @@ __device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
 }
 template <int kCount>
 __device__ __forceinline__ void tmem_read2(uint32_t taddr_a, uint32_t taddr_b, float (&a)[kCount], float (&b)[kCount]) {
-    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
+    static_assert(kCount == 8 || kCount == 16, "");
     if constexpr (kCount == 8)
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
                      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
@@ -543,23 +543,27 @@ __device__ __forceinline__ void tmem_read2(uint32_t taddr_a, uint32_t taddr_b, f
                        "=&f"(b[0]), "=&f"(b[1]), "=&f"(b[2]), "=&f"(b[3]), "=&f"(b[4]), "=&f"(b[5]), "=&f"(b[6]), "=&f"(b[7]), "=&f"(b[8]),
                        "=&f"(b[9]), "=&f"(b[10]), "=&f"(b[11]), "=&f"(b[12]), "=&f"(b[13]), "=&f"(b[14]), "=&f"(b[15])
                      : "r"(taddr_a), "r"(taddr_b) : "memory");
-    else if constexpr (kCount == 32)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-                     "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
-                     "%31}, [%64];\n\t"
-                     "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-                     "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,"
-                     "%61,%62,%63}, [%65];\n\t"
-                     "tcgen05.wait::ld.sync.aligned;"
-                     : "=&f"(a[0]), "=&f"(a[1]), "=&f"(a[2]), "=&f"(a[3]), "=&f"(a[4]), "=&f"(a[5]), "=&f"(a[6]), "=&f"(a[7]), "=&f"(a[8]),
-                       "=&f"(a[9]), "=&f"(a[10]), "=&f"(a[11]), "=&f"(a[12]), "=&f"(a[13]), "=&f"(a[14]), "=&f"(a[15]), "=&f"(a[16]),
-                       "=&f"(a[17]), "=&f"(a[18]), "=&f"(a[19]), "=&f"(a[20]), "=&f"(a[21]), "=&f"(a[22]), "=&f"(a[23]), "=&f"(a[24]),
-                       "=&f"(a[25]), "=&f"(a[26]), "=&f"(a[27]), "=&f"(a[28]), "=&f"(a[29]), "=&f"(a[30]), "=&f"(a[31]),
-                       "=&f"(b[0]), "=&f"(b[1]), "=&f"(b[2]), "=&f"(b[3]), "=&f"(b[4]), "=&f"(b[5]), "=&f"(b[6]), "=&f"(b[7]), "=&f"(b[8]),
-                       "=&f"(b[9]), "=&f"(b[10]), "=&f"(b[11]), "=&f"(b[12]), "=&f"(b[13]), "=&f"(b[14]), "=&f"(b[15]), "=&f"(b[16]),
-                       "=&f"(b[17]), "=&f"(b[18]), "=&f"(b[19]), "=&f"(b[20]), "=&f"(b[21]), "=&f"(b[22]), "=&f"(b[23]), "=&f"(b[24]),
-                       "=&f"(b[25]), "=&f"(b[26]), "=&f"(b[27]), "=&f"(b[28]), "=&f"(b[29]), "=&f"(b[30]), "=&f"(b[31])
-                     : "r"(taddr_a), "r"(taddr_b) : "memory");
+}
+
+// 32 lanes x 16 columns as the accumulators of m16n8k16 products, with their wait: r[(2 m + h) * 4 + i] is row 16 m + lane / 4 + 8 (i / 2), column
+// 8 h + 2 (lane % 4) + i % 2.
+__device__ __forceinline__ void tmem_read_fragments(uint32_t taddr, float (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+                 "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
+                   "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15])
+                 : "r"(taddr), "r"(taddr + (16u << 16)) : "memory");
+}
+// c += a b for one warp: a 16 x 16, b 16 x 8, bf16 or fp16.
+template <bool kHalf>
+__device__ __forceinline__ void mma_16x8x16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // 16 lanes x 32 fp32 columns as matrix fragments (the lower or the upper half of the warp's lane quarter, by the lane field of

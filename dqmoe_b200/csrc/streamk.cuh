@@ -1,7 +1,5 @@
-// A list of tiles of equal length, cut into equal shares of their concatenated K steps ("units"): what the kernels with few output
-// tiles use to give every SM the same bytes (moe_decode.cu, lora.cu). A tile that several shares take part in is finished by the
-// block that completes its part last: each writes its partial sums, counts itself in, and the last one adds all parts in the order of
-// the shares, so the result does not depend on which block that was.
+// Tiles whose sums several blocks share (moe_decode.cu, lora.cu): each writes its partial sums, counts itself in, and the one that completes the
+// tile adds all parts in their order, so the result does not depend on which block that was.
 #pragma once
 
 #include <stdint.h>
@@ -10,11 +8,6 @@
 
 namespace dq {
 namespace streamk {
-
-// first unit of share g of `shares` over `units`; shares [first(g), first(g + 1))
-__device__ __forceinline__ int first_unit(int g, int shares, int units) { return int(int64_t(g) * units / shares); }
-// the share that unit u lies in: the largest g with first_unit(g) <= u
-__device__ __forceinline__ int share_of(int u, int shares, int units) { return int((int64_t(u + 1) * shares - 1) / units); }
 
 __device__ __forceinline__ int ld_acquire_gpu(const int* p) {
     int v;
