@@ -72,8 +72,7 @@ struct ShrinkParams {
 };
 
 // A row's z in the operands' type, by a warp whose lanes hold four values each (lane * 4 < R).
-__device__ __forceinline__ void put_z(const ShrinkParams& p, int64_t t, int id, float4 v, int lane) {
-    const float scale = p.scale != nullptr ? p.scale[id] : 1.0f;
+__device__ __forceinline__ void put_z(const ShrinkParams& p, int64_t t, float scale, float4 v, int lane) {
     v.x *= scale, v.y *= scale, v.z *= scale, v.w *= scale;
     if (p.half) {
         const float most = warp_max(lane * 4 < p.R ? fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) : 0.0f);
@@ -140,7 +139,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) lora_shrink_rows_kernel(const 
     __syncthreads();
     if (warp > 0) return;
     if (gridDim.y == 1) {
-        put_z(p, t, id, lane * 4 < p.R ? *reinterpret_cast<const float4*>(s_z + lane * 4) : make_float4(0, 0, 0, 0), lane);
+        put_z(p, t, p.scale != nullptr ? p.scale[id] : 1.0f, lane * 4 < p.R ? *reinterpret_cast<const float4*>(s_z + lane * 4) : make_float4(0, 0, 0, 0), lane);
     } else if (lane < ranks - first) {  // bf16: no power of two
         const float scale = p.scale != nullptr ? p.scale[id] : 1.0f;
         p.z[int64_t(t) * p.R + first + lane] = to_bits(s_z[first + lane] * scale, false);
@@ -152,8 +151,9 @@ struct alignas(16) ShrinkTail {
     uint32_t tmem_base;
     int abort_flag;
     int distinct;                               // adapters of the tile
-    int id[kShrinkTok];                         // -1 where there is none
-    int place[kShrinkTok];                      // place of a row's adapter among the tile's
+    alignas(16) int id[kShrinkTok];             // -1 where there is none
+    float scale[kShrinkTok];
+    alignas(16) int place[kShrinkTok];          // place of a row's adapter among the tile's
     int adapter[kShrinkTok];                    // the tile's adapters in the order of their first rows
     uint32_t firsts[2];
 };
@@ -214,8 +214,11 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     int first = kShrinkTok;  // this row's adapter appears first in row `first`
     if (threadIdx.x < kShrinkTok) {
         const int mine = st.id[threadIdx.x];
-        for (int t = kShrinkTok - 1; t >= 0; --t)
-            if (st.id[t] == mine) first = t;
+#pragma unroll
+        for (int t = kShrinkTok - 4; t >= 0; t -= 4) {
+            const int4 ids = *reinterpret_cast<const int4*>(st.id + t);
+            first = ids.x == mine ? t : ids.y == mine ? t + 1 : ids.z == mine ? t + 2 : ids.w == mine ? t + 3 : first;
+        }
         const uint32_t firsts = __ballot_sync(0xffffffffu, mine >= 0 && first == int(threadIdx.x));
         if (lane == 0) st.firsts[warp] = firsts;
     }
@@ -281,6 +284,9 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             }
         }
         __syncwarp();
+    } else if (warp == 2 || warp == 3) {
+        const int t = threadIdx.x - 2 * 32, id = st.id[t];
+        st.scale[t] = p.scale != nullptr && id >= 0 ? p.scale[id] : 1.0f;
     } else if (warp >= 4 && kb0 < kb1) {
         const int row = (warp - 4) * 32 + lane, mine = row / p.R, r = row - mine * p.R;
         int acc = 0;
@@ -290,11 +296,17 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             const int rows = min(kShrinkTok, p.T - tile * kShrinkTok);
 #pragma unroll 1
             for (int c = 0; c < rows; c += 16) {
+                int place[16];  // all of them before the first sum is put down, which might be one of them for all the compiler knows
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int4 four = *reinterpret_cast<const int4*>(st.place + c + i);
+                    place[i] = four.x, place[i + 1] = four.y, place[i + 2] = four.z, place[i + 3] = four.w;
+                }
                 float v[16];
                 ptx::tmem_read<16>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (mine < cap && st.place[c + i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
+                    if (mine < cap && place[i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
             }
             ptx::tc_fence_before();
             __syncwarp();
@@ -313,15 +325,17 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     for (int t = warp * split + rank; t < kShrinkTok; t += split * (kShrinkThreads / 32)) {
         const int place = st.place[t];
         if (place < 0 || (place / cap) % p.slots != slot) continue;
-        float4 sum = make_float4(0, 0, 0, 0);
-        if (lane * 4 < p.R)
-            for (int c = 0; c < split; ++c) {
-                float4 v;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+        float4 v[kMaxSplit], sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c) {
+            v[c] = make_float4(0, 0, 0, 0);
+            if (c < split && lane * 4 < p.R)
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[c].x), "=f"(v[c].y), "=f"(v[c].z), "=f"(v[c].w)
                              : "r"(ptx::map_to_cta(part + t * p.R + lane * 4, c)) : "memory");
-                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-            }
-        put_z(p, int64_t(tile) * kShrinkTok + t, st.id[t], sum, lane);
+        }
+#pragma unroll
+        for (int c = 0; c < kMaxSplit; ++c) sum.x += v[c].x, sum.y += v[c].y, sum.z += v[c].z, sum.w += v[c].w;
+        put_z(p, int64_t(tile) * kShrinkTok + t, st.scale[t], sum, lane);
     }
     __syncthreads();
     ptx::cluster_sync();  // the others read this block's shared memory until here
@@ -401,6 +415,12 @@ struct Pieces {
     __device__ __forceinline__ int left() const { return tile < p.whole || (tile != 0x7fffffff && group < (p.tiles - p.whole) * p.parts) ? 1 : 0; }  // 0: none
 };
 
+__device__ __forceinline__ float load_f32(const float* from) {  // past L1: written while this kernel was here already
+    float v;
+    asm volatile("ld.relaxed.gpu.global.f32 %0, [%1];" : "=f"(v) : "l"(from) : "memory");
+    return v;
+}
+
 // The adapters' products of a tile's rows, by one warp, and which of them belong to this part.
 template <bool kHalf, bool kPair>
 __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane) {
@@ -411,9 +431,12 @@ __device__ __forceinline__ void make_list(const Params& p, List& l, int t0, cons
 #pragma unroll
     for (int c = 0; c < kMaxTok / 32; ++c) ids[c] = c * 32 + lane < rows ? ld_relaxed_gpu(p.ids + t0 + c * 32 + lane) : -2;  // bf16: before this kernel's wait, so past L1
     if constexpr (kHalf) {
+        float scale[kMaxTok / 32];  // all loads at once; rows without an adapter have none
+#pragma unroll
+        for (int c = 0; c < kMaxTok / 32; ++c) scale[c] = c * 32 + lane < rows ? load_f32(p.z_scale + t0 + c * 32 + lane) : 1.0f;
 #pragma unroll
         for (int c = 0; c < kMaxTok / 32; ++c)
-            if (c * 32 + lane < rows && ids[c] >= 0 && ids[c] < p.L && p.z_scale[t0 + c * 32 + lane] != 1.0f) scaled_rows |= 1u << c;
+            if (ids[c] >= 0 && ids[c] < p.L && scale[c] != 1.0f) scaled_rows |= 1u << c;
     }
 #pragma unroll
     for (int pair = 0; pair < kMaxTok / 32; ++pair) {  // two chunks at a time, half a warp each
@@ -502,17 +525,26 @@ struct Epilogue {
         }
     }
 
-    // The adapters' products of the mixed rows of a chunk, from place `e` of the list on: B's rows are the products' rows, z's rows their columns, of
+    // The adapters' products of the mixed rows of a chunk, from place `e` of the list on, and the place behind them: B's rows are the products' rows, z's rows their columns, of
     // which each takes the columns that have its adapter. Operands straight from L2 into registers, where 16 bytes of a row are eight values that
     // follow one another; which of them a product takes for its k is the same for both, and a sum does not mind. Steps are 32 of R.
-    __device__ __forceinline__ void products(const List& l, int half, int* e, int chunk, int t0, int n0, float (&v)[kChunk]) {
+    __device__ __forceinline__ int products(const List& l, int half, int e, int chunk, int t0, int n0, float (&v)[kChunk]) {
         const int end = l.mixed1[half], rank_steps = (p.R + 31) / 32, k_lane = (lane & 3) * 8, g = lane >> 2;
-        int to = *e;
+        int to = e;
         while (to < end && int(l.mixed[half][to].y & 0xff) == chunk) ++to;
-        int load = *e, load_k = 0, use = *e, use_k = 0;
-        float d[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
+        int load = e, load_k = 0, use = e, use_k = 0;
+        float d[kChunk], scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // of this lane's columns
+        if constexpr (kHalf) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = t0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1);
+                if (t < p.T) scale[j] = load_f32(p.z_scale + t);
+            }
+        }
 #pragma unroll 1
-        for (int left = (to - *e) * rank_steps; left > 0; left -= kProducts) {
+        for (int left = (to - e) * rank_steps; left > 0; left -= kProducts) {
             uint4 b[kProducts][4], z[kProducts][2];
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
@@ -552,11 +584,11 @@ struct Epilogue {
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     const int column = ((j >> 2) & 1) * 8 + (lane & 3) * 2 + (j & 1);
-                    if ((rows >> column) & 1u) v[j] = kHalf ? d[j] * p.z_scale[t0 + column] : d[j];
+                    if ((rows >> column) & 1u) v[j] = kHalf ? d[j] * scale[((j >> 2) & 1) * 2 + (j & 1)] : d[j];
                 }
             }
         }
-        *e = to;
+        return to;
     }
     static __device__ __forceinline__ uint4 load16(const uint16_t* from) {  // past L1: written while this kernel was here already
         uint4 v;
@@ -613,48 +645,56 @@ struct Epilogue {
             const List& l = st.list[buf];
             // columns in use; the two halves of the epilogue take chunks in turn
             const int cols = min(p.tok, p.T - t0), n0 = n - lane;
+            // A block's only piece: the mixed products while the tensor core still sums, into the accumulators that nobody needs. Else, and then, the sums.
+            const bool ahead = pieces.left() == 0 && acc == 0;
+            const uint32_t sums = tmem + buf * p.tok, others = tmem + (buf ^ 1) * p.tok;
+            uint32_t mixed_chunks = 0;
             int e = l.mixed0[half];
-            bool full = false;
-            for (int c = half; c * kChunk < cols; c += 2) {
-                float v[kChunk], d[kChunk];
-                const bool mixed = e < l.mixed1[half] && int(l.mixed[half][e].y & 0xff) == c;
-                if (mixed) {  // the first chunk's while the tensor core still sums
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) d[j] = 0.0f;
-                    products(l, half, &e, c, t0 + c * kChunk, n0, d);
-                }
-                if (!full) {
+#pragma unroll 1
+            for (int pass = ahead ? 0 : 1; pass < 2; ++pass) {
+                if (pass == 1) {
                     if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
                     ptx::tc_fence_after();
-                    full = true;
                 }
-                float* to = p.part + (size_t(blockIdx.x) * p.tok + c * kChunk) * kRows;
-                if (mixed) {
-                    ptx::tmem_read_fragments(tmem + buf * p.tok + c * kChunk, v);
+#pragma unroll 1
+                for (int c = half; c * kChunk < cols; c += 2) {
+                    float v[kChunk], d[kChunk];
+                    const bool now = e < l.mixed1[half] && int(l.mixed[half][e].y & 0xff) == c;
+                    if (now) e = products(l, half, e, c, t0 + c * kChunk, n0, d);
+                    if (pass == 0) {
+                        if (now) {
+                            ptx::tmem_write_fragments(others + c * kChunk, d);
+                            mixed_chunks |= 1u << c;
+                        }
+                        continue;
+                    }
+                    float* to = p.part + (size_t(blockIdx.x) * p.tok + c * kChunk) * kRows;
+                    if (now || ((mixed_chunks >> c) & 1u) != 0) {
+                        if (!now) ptx::tmem_read_fragments(others + c * kChunk, d);
+                        ptx::tmem_read_fragments(sums + c * kChunk, v);
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) v[j] += d[j];
+                        for (int j = 0; j < kChunk; ++j) v[j] += d[j];
+                        if (q.of == 1) {
+                            store_fragments(v, t0 + c * kChunk, n0);
+                            continue;
+                        }
+#pragma unroll
+                        for (int j = 0; j < kChunk; j += 2) {
+                            const int r = row - lane + (j >> 3) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2), t = ((j >> 2) & 1) * 8 + (lane & 3) * 2;
+                            if (c * kChunk + (t & ~3) < cols) *reinterpret_cast<float2*>(to + (t & ~3) * kRows + r * 4 + (t & 3)) = make_float2(v[j], v[j + 1]);
+                        }
+                        continue;
+                    }
+                    ptx::tmem_read<kChunk>(sums + c * kChunk, v);
                     if (q.of == 1) {
-                        store_fragments(v, t0 + c * kChunk, n0);
+                        store(v, t0 + c * kChunk, n);
                         continue;
                     }
 #pragma unroll
-                    for (int j = 0; j < kChunk; j += 2) {
-                        const int r = row - lane + (j >> 3) * 16 + ((j >> 1) & 1) * 8 + (lane >> 2), t = ((j >> 2) & 1) * 8 + (lane & 3) * 2;
-                        if (c * kChunk + (t & ~3) < cols) *reinterpret_cast<float2*>(to + (t & ~3) * kRows + r * 4 + (t & 3)) = make_float2(v[j], v[j + 1]);
-                    }
-                    continue;
+                    for (int j = 0; j < kChunk; j += 4)
+                        if (c * kChunk + j < cols) *reinterpret_cast<float4*>(to + j * kRows + row * 4) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                 }
-                ptx::tmem_read<kChunk>(tmem + buf * p.tok + c * kChunk, v);
-                if (q.of == 1) {
-                    store(v, t0 + c * kChunk, n);
-                    continue;
-                }
-#pragma unroll
-                for (int j = 0; j < kChunk; j += 4)
-                    if (c * kChunk + j < cols) *reinterpret_cast<float4*>(to + j * kRows + row * 4) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
             }
-            // also a half without a chunk waits, so that it does not run ahead of the tensor core
-            if (!full && !ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
             ptx::tc_fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -909,7 +949,7 @@ struct Layout {
 // more or less in each block's share 41.5; 4096 rows on single blocks 110.8, on pairs 103.1.
 constexpr int kL2Bytes[2] = {60, 45};                // per cycle and SM, on single blocks and on pairs
 constexpr int kHbmBytes = 3300;                      // per cycle
-constexpr int kDrain = 12, kCount = 3000, kAdd = 12; // cycles a column; a tile in parts; a column of each part
+constexpr int kDrain = 12, kCount = 3000, kAdd = 8;  // cycles a column; a tile in parts; a column of each part
 constexpr int kPairing = 1500;
 static bool plan_tiles(Params* p) {
     const int sms = sm_count();
@@ -996,8 +1036,9 @@ static int launch_shrink(ShrinkParams p, const void* x, cudaStream_t stream) {
         return p.half ? launch_pdl(lora_shrink_rows_kernel<true>, grid, kRowWarps * 32, 0, stream, p)
                       : launch_pdl(lora_shrink_rows_kernel<false>, grid, kRowWarps * 32, 0, stream, p);
     }
-    // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached.
-    const int tiles = ceil_div(p.T, kShrinkTok), room = 2 * sm_count(), kbs = ceil_div(p.K, kKElems);
+    // A tile's K is cut over a cluster, and its groups of adapters over several, as long as two blocks per SM are not reached, less an eighth, as
+    // clusters of eight do not fill every part of the chip (288 blocks: the last clusters began after 9 us).
+    const int tiles = ceil_div(p.T, kShrinkTok), room = 2 * sm_count() * 7 / 8, kbs = ceil_div(p.K, kKElems);
     int split = kMaxSplit;
     while (split > 1 && (tiles * split > room || split > kbs)) split /= 2;
     p.cap = kRows / 2 / p.R > 1 ? kRows / 2 / p.R : 1;

@@ -555,6 +555,14 @@ __device__ __forceinline__ void tmem_read_fragments(uint32_t taddr, float (&r)[1
                    "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15])
                  : "r"(taddr), "r"(taddr + (16u << 16)) : "memory");
 }
+// The same way back, complete when it returns.
+__device__ __forceinline__ void tmem_write_fragments(uint32_t taddr, const float (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%2,%3,%4,%5,%6,%7,%8,%9};\n\t"
+                 "tcgen05.st.sync.aligned.16x256b.x2.b32 [%1], {%10,%11,%12,%13,%14,%15,%16,%17};\n\t"
+                 "tcgen05.wait::st.sync.aligned;"
+                 ::"r"(taddr), "r"(taddr + (16u << 16)), "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]),
+                 "f"(r[8]), "f"(r[9]), "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]) : "memory");
+}
 // c += a b for one warp: a 16 x 16, b 16 x 8, bf16 or fp16.
 template <bool kHalf>
 __device__ __forceinline__ void mma_16x8x16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
