@@ -422,22 +422,11 @@ __device__ __forceinline__ float load_f32(const float* from) {  // past L1: writ
 }
 
 // The adapters' products of a tile's rows, by one warp, and which of them belong to this part.
-template <bool kHalf, bool kPair>
-__device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane) {
+// scaled_rows: bit c where this lane's row of the c-th pair of chunks has a power of two.
+template <bool kPair>
+__device__ __forceinline__ void make_list(const Params& p, List& l, int t0, const Piece& q, int lane, const int (&ids)[kMaxTok / 32], uint32_t scaled_rows) {
     int direct = 0, mixed0 = 0, mixed1 = 0, last = -1, last_end = -1, last_first = 0;
     const int rows = min(p.tok, p.T - t0), half = lane >> 4;
-    int ids[kMaxTok / 32];
-    uint32_t scaled_rows = 0;  // bit c: this lane's row of the c-th pair of chunks has a power of two
-#pragma unroll
-    for (int c = 0; c < kMaxTok / 32; ++c) ids[c] = c * 32 + lane < rows ? ld_relaxed_gpu(p.ids + t0 + c * 32 + lane) : -2;  // bf16: before this kernel's wait, so past L1
-    if constexpr (kHalf) {
-        float scale[kMaxTok / 32];  // all loads at once; rows without an adapter have none
-#pragma unroll
-        for (int c = 0; c < kMaxTok / 32; ++c) scale[c] = c * 32 + lane < rows ? load_f32(p.z_scale + t0 + c * 32 + lane) : 1.0f;
-#pragma unroll
-        for (int c = 0; c < kMaxTok / 32; ++c)
-            if (ids[c] >= 0 && ids[c] < p.L && scale[c] != 1.0f) scaled_rows |= 1u << c;
-    }
 #pragma unroll
     for (int pair = 0; pair < kMaxTok / 32; ++pair) {  // two chunks at a time, half a warp each
         const int c = 2 * pair;
@@ -543,24 +532,27 @@ struct Epilogue {
                 if (t < p.T) scale[j] = load_f32(p.z_scale + t);
             }
         }
+        // what does not depend on the step, before the loop: it is bound by its instructions as much as by its loads
+        const size_t adapter = size_t(p.N) * p.R;
+        const uint16_t *b_lane = p.lora_b + size_t(n0 + g) * p.R + k_lane, *z_lane = p.z + size_t(t0 + g) * p.R + k_lane;
+        const int down = 8 * p.R, inside = (p.N - n0 - g + 7) >> 3;  // to the next row of B of this lane; how many of the four there are
+        bool mine[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine[j] = j < inside;
 #pragma unroll 1
         for (int left = (to - e) * rank_steps; left > 0; left -= kProducts) {
             uint4 b[kProducts][4], z[kProducts][2];
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
                 const uint2 q = i < left ? l.mixed[half][load] : make_uint2(0, 0);
-                const int k = load_k * 32 + k_lane;
-                const bool in = i < left && k < p.R;
+                const int k = load_k * 32;
+                const bool in = i < left && k + k_lane < p.R;
+                const uint16_t *from = b_lane + q.x * adapter + k, *z_from = z_lane + k;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int n = n0 + j * 8 + g;
-                    b[i][j] = in && n < p.N ? load16(p.lora_b + (size_t(q.x) * p.N + n) * p.R + k) : make_uint4(0, 0, 0, 0);
-                }
+                for (int j = 0; j < 4; ++j) b[i][j] = in && mine[j] ? load16(from + j * down) : make_uint4(0, 0, 0, 0);
+                const uint32_t columns = q.y >> (16 + g);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int t = t0 + h * 8 + g;
-                    z[i][h] = in && ((q.y >> (16 + 8 * h + g)) & 1u) ? load16(p.z + size_t(t) * p.R + k) : make_uint4(0, 0, 0, 0);
-                }
+                for (int h = 0; h < 2; ++h) z[i][h] = in && ((columns >> (8 * h)) & 1u) ? load16(z_from + h * down) : make_uint4(0, 0, 0, 0);
                 if (++load_k == rank_steps) load_k = 0, ++load;
             }
 #pragma unroll
@@ -888,22 +880,41 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         }
         __syncwarp();
     } else if (warp == 2) {
-        if constexpr (kHalf) pdl_wait();  // shrink: z_scale
         Pieces pieces(p, group);
         Piece q;
         for (int n = 0; pieces.next(&q); ++n) {
             if (!ptx::mbar_wait_warp(&st.list_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
             List& l = st.list[n & 1];
-            make_list<kHalf, kPair>(p, l, q.tile / p.n_tiles * p.tok, q, lane);
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&st.list_full[n & 1]);
-            // The mixed rows' B towards L2 meanwhile: 128 rows of an adapter's follow one another in memory.
-            const int n0 = ((q.tile % p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows;
-            const uint32_t bytes = uint32_t(max(0, min(kRows, p.N - n0)) * p.R) * 2u;
+            const int tt = q.tile / p.n_tiles, t0 = tt * p.tok, rows = min(p.tok, p.T - t0);
+            int ids[kMaxTok / 32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                for (int e = l.mixed0[h] + lane; bytes > 0 && e < l.mixed1[h]; e += 32)
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.lora_b + (size_t(l.mixed[h][e].x) * p.N + n0) * p.R), "r"(bytes));
+            for (int c = 0; c < kMaxTok / 32; ++c) ids[c] = c * 32 + lane < rows ? ld_relaxed_gpu(p.ids + t0 + c * 32 + lane) : -2;  // before this kernel's wait, so past L1
+            uint32_t scaled_rows = 0;
+            // fp16: before shrink is over as if no row had a power of two, which is made good where one has
+#pragma unroll 1
+            for (bool known = !kHalf;;) {
+                make_list<kPair>(p, l, t0, q, lane, ids, scaled_rows);
+                __syncwarp();
+                if (scaled_rows == 0) {  // the mixed rows' B towards L2 meanwhile: 128 rows of an adapter's follow one another in memory
+                    const int n0 = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows;
+                    const uint32_t bytes = uint32_t(max(0, min(kRows, p.N - n0)) * p.R) * 2u;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        for (int e = l.mixed0[h] + lane; bytes > 0 && e < l.mixed1[h]; e += 32)
+                            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.lora_b + (size_t(l.mixed[h][e].x) * p.N + n0) * p.R), "r"(bytes));
+                }
+                if (known) break;
+                known = true;
+                if (n == 0) pdl_wait();  // shrink: z_scale
+                float scale[kMaxTok / 32];  // all loads at once; rows without an adapter have none
+#pragma unroll
+                for (int c = 0; c < kMaxTok / 32; ++c) scale[c] = c * 32 + lane < rows ? load_f32(p.z_scale + t0 + c * 32 + lane) : 1.0f;
+#pragma unroll
+                for (int c = 0; c < kMaxTok / 32; ++c)
+                    if (ids[c] >= 0 && ids[c] < p.L && scale[c] != 1.0f) scaled_rows |= 1u << c;
+                if (!__any_sync(0xffffffffu, scaled_rows != 0)) break;
+            }
+            if (lane == 0) ptx::mbar_arrive(&st.list_full[n & 1]);
         }
     } else if (warp >= 4) {
         Epilogue<kHalf, kPair> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane, rank};
