@@ -343,13 +343,13 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 
 // ---------------------------------------------------------------- project
 
-constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warp 2 list of the adapters' products, warps 4..11 epilogue
+constexpr int kThreads = 384;                   // warp 0 TMA, warp 1 MMA, warp 2 list of the adapters' products, warp 3 B of mixed rows, warps 4..11 epilogue
 constexpr int kMaxTok = 256;
 constexpr int kTmemCols = 512;                  // two accumulators
-constexpr int kRingBytes = 200 * 1024;
+constexpr int kRingBytes = 216 * 1024;          // stages, and B of mixed rows
 constexpr int kMaxStages = 10;
 constexpr int kChunk = 16;                      // rows of x that are looked at together
-constexpr int kProducts = 4;                    // steps of the mixed rows' products that are loaded at once
+constexpr int kMaxSlots = 8;                    // adapters' B on their way to each half of the epilogue
 constexpr int kMaxParts = 16;
 
 struct Params {
@@ -363,6 +363,7 @@ struct Params {
     int T, N, K, L, R;
     int tok;                  // rows of x per tile, a multiple of 16, on pairs of 32
     int stages;
+    int slots;                // for B of mixed rows, of each half of the epilogue
     int n_tiles, tiles;       // tiles along N, and in all
     int kbs;
     int groups;               // blocks, or pairs of them
@@ -382,6 +383,7 @@ struct List {
 struct alignas(16) Tail {
     uint64_t full[kMaxStages], empty[kMaxStages], tmem_full[2], tmem_empty[2];
     uint64_t list_full[2], list_empty[2];
+    uint64_t b_full[2][kMaxSlots], b_empty[2][kMaxSlots];  // by half of the epilogue
     uint64_t meet;            // the epilogue warps
     uint32_t tmem_base;
     int abort_flag;
@@ -488,6 +490,8 @@ struct Epilogue {
     uint32_t tmem;            // this warp's lanes
     int warp, lane, row;      // warp 0..7, row = TMEM lane = row of W among the block's 128 of the tile
     int rank;                 // of the block in its pair
+    const uint8_t* b_ring;
+    int b_it = 0;             // B's of this half so far
     uint32_t meetings = 0;
 
     __device__ __forceinline__ bool meet() {
@@ -514,17 +518,20 @@ struct Epilogue {
         }
     }
 
-    // The adapters' products of the mixed rows of a chunk, from place `e` of the list on, and the place behind them: B's rows are the products' rows, z's rows their columns, of
-    // which each takes the columns that have its adapter. Operands straight from L2 into registers, where 16 bytes of a row are eight values that
-    // follow one another; which of them a product takes for its k is the same for both, and a sum does not mind. Steps are 32 of R.
-    __device__ __forceinline__ int products(const List& l, int half, int e, int chunk, int t0, int n0, float (&v)[kChunk]) {
-        const int end = l.mixed1[half], rank_steps = (p.R + 31) / 32, k_lane = (lane & 3) * 8, g = lane >> 2;
-        int to = e;
-        while (to < end && int(l.mixed[half][to].y & 0xff) == chunk) ++to;
+    // The adapters' products of the mixed rows of a chunk, from place `e` of the list on: B's rows are the products' rows, z's rows their columns, of
+    // which each takes the columns that have its adapter. 16 bytes of a row are eight values that follow one another; which of them a product takes
+    // for its k is the same for both, and a sum does not mind. Returns the place behind them, -1 where a wait has run out.
+    __device__ __forceinline__ int products(const List& l, int half, int e, int chunk, int t0, float (&v)[kChunk]) {
+        const int k_lane = (lane & 3) * 8, g = lane >> 2;
+        uint4 z[kMaxRank / 32][2];
+        float scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // of this lane's columns
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
-        int load = e, load_k = 0, use = e, use_k = 0;
-        float d[kChunk], scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // of this lane's columns
+        for (int k = 0; k < kMaxRank / 32; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int t = t0 + h * 8 + g;  // a row without an adapter, whose z is nothing, has a column that nobody takes
+                z[k][h] = k * 32 + k_lane < p.R && t < p.T ? load16(p.z + size_t(t) * p.R + k * 32 + k_lane) : make_uint4(0, 0, 0, 0);
+            }
         if constexpr (kHalf) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -532,55 +539,46 @@ struct Epilogue {
                 if (t < p.T) scale[j] = load_f32(p.z_scale + t);
             }
         }
-        // what does not depend on the step, before the loop: it is bound by its instructions as much as by its loads
-        const size_t adapter = size_t(p.N) * p.R;
-        const uint16_t *b_lane = p.lora_b + size_t(n0 + g) * p.R + k_lane, *z_lane = p.z + size_t(t0 + g) * p.R + k_lane;
-        const int down = 8 * p.R, inside = (p.N - n0 - g + 7) >> 3;  // to the next row of B of this lane; how many of the four there are
-        bool mine[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mine[j] = j < inside;
+        for (int j = 0; j < kChunk; ++j) v[j] = 0.0f;
+        const int end = l.mixed1[half], slot_bytes = kRows * p.R * 2;
 #pragma unroll 1
-        for (int left = (to - e) * rank_steps; left > 0; left -= kProducts) {
-            uint4 b[kProducts][4], z[kProducts][2];
+        for (; e < end; ++e, ++b_it) {
+            const uint32_t entry = l.mixed[half][e].y, rows = entry >> 16;
+            if (int(entry & 0xff) != chunk) break;
+            const int slot = b_it % p.slots;
+            if (!ptx::mbar_wait_warp(&st.b_full[half][slot], (b_it / p.slots) & 1, &st.abort_flag, kWaitLimit)) return -1;
+            const uint8_t* from = b_ring + (half * p.slots + slot) * slot_bytes + ((row - lane + g) * p.R + k_lane) * 2;
+            float d[kChunk];
 #pragma unroll
-            for (int i = 0; i < kProducts; ++i) {
-                const uint2 q = i < left ? l.mixed[half][load] : make_uint2(0, 0);
-                const int k = load_k * 32;
-                const bool in = i < left && k + k_lane < p.R;
-                const uint16_t *from = b_lane + q.x * adapter + k, *z_from = z_lane + k;
+            for (int j = 0; j < kChunk; ++j) d[j] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) b[i][j] = in && mine[j] ? load16(from + j * down) : make_uint4(0, 0, 0, 0);
-                const uint32_t columns = q.y >> (16 + g);
+            for (int k = 0; k < kMaxRank / 32; ++k) {
+                if (k * 32 >= p.R) break;
+                const bool in = k * 32 + k_lane < p.R;
+                uint4 b[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) z[i][h] = in && ((columns >> (8 * h)) & 1u) ? load16(z_from + h * down) : make_uint4(0, 0, 0, 0);
-                if (++load_k == rank_steps) load_k = 0, ++load;
-            }
-#pragma unroll
-            for (int i = 0; i < kProducts; ++i) {
-                if (i >= left) break;
-                if (use_k == 0)
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) d[j] = 0.0f;
-                const uint32_t rows = l.mixed[half][use].y >> 16;
+                for (int j = 0; j < 4; ++j) b[j] = in ? *reinterpret_cast<const uint4*>(from + (j * 8 * p.R + k * 32) * 2) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    if ((rows >> (8 * h)) & 255u)
+                    if ((rows >> (8 * h)) & 255u) {
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             float* c = d + (2 * m + h) * 4;
-                            ptx::mma_16x8x16<kHalf>(c, b[i][2 * m].x, b[i][2 * m + 1].x, b[i][2 * m].y, b[i][2 * m + 1].y, z[i][h].x, z[i][h].y);
-                            ptx::mma_16x8x16<kHalf>(c, b[i][2 * m].z, b[i][2 * m + 1].z, b[i][2 * m].w, b[i][2 * m + 1].w, z[i][h].z, z[i][h].w);
+                            ptx::mma_16x8x16<kHalf>(c, b[2 * m].x, b[2 * m + 1].x, b[2 * m].y, b[2 * m + 1].y, z[k][h].x, z[k][h].y);
+                            ptx::mma_16x8x16<kHalf>(c, b[2 * m].z, b[2 * m + 1].z, b[2 * m].w, b[2 * m + 1].w, z[k][h].z, z[k][h].w);
                         }
-                if (++use_k < rank_steps) continue;
-                use_k = 0, ++use;
+                    }
+            }
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.b_empty[half][slot]);
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) {
-                    const int column = ((j >> 2) & 1) * 8 + (lane & 3) * 2 + (j & 1);
-                    if ((rows >> column) & 1u) v[j] = kHalf ? d[j] * scale[((j >> 2) & 1) * 2 + (j & 1)] : d[j];
-                }
+            for (int j = 0; j < kChunk; ++j) {
+                const int column = ((j >> 2) & 1) * 8 + (lane & 3) * 2 + (j & 1);
+                if ((rows >> column) & 1u) v[j] = kHalf ? d[j] * scale[((j >> 2) & 1) * 2 + (j & 1)] : d[j];
             }
         }
-        return to;
+        return e;
     }
     static __device__ __forceinline__ uint4 load16(const uint16_t* from) {  // past L1: written while this kernel was here already
         uint4 v;
@@ -652,7 +650,7 @@ struct Epilogue {
                 for (int c = half; c * kChunk < cols; c += 2) {
                     float v[kChunk], d[kChunk];
                     const bool now = e < l.mixed1[half] && int(l.mixed[half][e].y & 0xff) == c;
-                    if (now) e = products(l, half, e, c, t0 + c * kChunk, n0, d);
+                    if (now && (e = products(l, half, e, c, t0 + c * kChunk, d)) < 0) return;
                     if (pass == 0) {
                         if (now) {
                             ptx::tmem_write_fragments(others + c * kChunk, d);
@@ -726,17 +724,24 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
     const int rank = kPair ? int(ptx::cluster_ctarank()) : 0, group = int(blockIdx.x) >> (kPair ? 1 : 0);
     const int x_rows = kPair ? p.tok / 2 : p.tok;  // of this block
     const int stage = kABytes + x_rows * kKBytes;
-    Tail& st = *reinterpret_cast<Tail*>(ring + p.stages * stage);
+    uint8_t* b_ring = ring + p.stages * stage;     // [half of the epilogue][slot]: 128 rows of an adapter's B, as in memory
+    const int slot_bytes = kRows * p.R * 2;
+    Tail& st = *reinterpret_cast<Tail*>(b_ring + 2 * p.slots * slot_bytes);
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) {
             ptx::mbar_init(&st.full[i], 1);
             ptx::mbar_init(&st.empty[i], 1);
         }
+        for (int i = 0; i < p.slots; ++i)
+            for (int h = 0; h < 2; ++h) {
+                ptx::mbar_init(&st.b_full[h][i], 1);
+                ptx::mbar_init(&st.b_empty[h][i], 4);
+            }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&st.tmem_full[i], 1);
             ptx::mbar_init(&st.tmem_empty[i], kPair ? 16 : 8);
             ptx::mbar_init(&st.list_full[i], 1);
-            ptx::mbar_init(&st.list_empty[i], rank == 0 ? 10 : 9);  // TMA thread, the first block's MMA thread, epilogue warps
+            ptx::mbar_init(&st.list_empty[i], rank == 0 ? 11 : 10);  // TMA thread, B's thread, epilogue warps, the first block's MMA thread
         }
         ptx::mbar_init(&st.meet, 8);
         st.abort_flag = 0;
@@ -914,10 +919,51 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     if (ids[c] >= 0 && ids[c] < p.L && scale[c] != 1.0f) scaled_rows |= 1u << c;
                 if (!__any_sync(0xffffffffu, scaled_rows != 0)) break;
             }
-            if (lane == 0) ptx::mbar_arrive(&st.list_full[n & 1]);
+            if (lane == 0) {
+                if (((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows >= p.N) l.mixed1[0] = l.mixed0[0], l.mixed1[1] = l.mixed0[1];  // no rows of W
+                ptx::mbar_arrive(&st.list_full[n & 1]);
+            }
         }
+    } else if (warp == 3) {
+        // B of the mixed rows' products: 128 rows of an adapter's follow one another in memory. A lane for each slot of each half: one thread's
+        // 300 cycles a copy would set the pace.
+        Pieces pieces(p, group);
+        Piece q;
+        const int h = lane >> 4, slot = lane & 15;
+        int before = 0, uses = 0;  // products of this half in earlier pieces; of this slot
+        bool ok = true;
+        for (int n = 0; ok && pieces.next(&q); ++n) {
+            if (!(ok = ptx::mbar_wait_warp(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+            const List& l = st.list[n & 1];
+            const int n0 = ((q.tile % p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows;
+            const uint32_t bytes = uint32_t(max(0, min(kRows, p.N - n0)) * p.R) * 2u;
+            const int first = l.mixed0[h], end = l.mixed1[h];
+            int e = slot < p.slots ? first + (slot + p.slots - before % p.slots) % p.slots : end;  // this slot's first
+            const long long begin = clock64();
+            while (__any_sync(0xffffffffu, e < end)) {
+                if (e < end && ptx::mbar_test_wait(&st.b_empty[h][slot], (uses & 1) ^ 1)) {
+                    ptx::mbar_arrive_expect_tx(&st.b_full[h][slot], bytes);
+                    ptx::bulk_load(b_ring + (h * p.slots + slot) * slot_bytes, p.lora_b + (size_t(l.mixed[h][e].x) * p.N + n0) * p.R, bytes, &st.b_full[h][slot]);
+                    ++uses;
+                    e += p.slots;
+                }
+                if (clock64() - begin > kWaitLimit) *const_cast<volatile int*>(&st.abort_flag) = 1;
+                if (__any_sync(0xffffffffu, *const_cast<volatile int*>(&st.abort_flag) != 0)) {
+                    ok = false;
+                    break;
+                }
+            }
+            before += end - first;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&st.list_empty[n & 1]);
+        }
+        if (*const_cast<volatile int*>(&st.abort_flag) != 0 && uses > 0) {  // nobody leaves with copies in flight
+            const long long begin = clock64();
+            while (!ptx::mbar_try_wait(&st.b_full[h][slot], (uses - 1) & 1) && clock64() - begin < kWaitLimit) {}
+        }
+        __syncwarp();
     } else if (warp >= 4) {
-        Epilogue<kHalf, kPair> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane, rank};
+        Epilogue<kHalf, kPair> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane, rank, b_ring};
         ep.run();
     }
     ptx::tc_fence_before();
@@ -962,6 +1008,7 @@ constexpr int kL2Bytes[2] = {60, 45};                // per cycle and SM, on sin
 constexpr int kHbmBytes = 3300;                      // per cycle
 constexpr int kDrain = 12, kCount = 3000, kAdd = 8;  // cycles a column; a tile in parts; a column of each part
 constexpr int kPairing = 1500;
+constexpr int kMixedRows = 512, kMixedBytes = 64 * 1024, kFewMixedBytes = 24 * 1024;
 static bool plan_tiles(Params* p) {
     const int sms = sm_count();
     const int64_t hbm = (int64_t(p->N) + p->T) * p->K * 2 / kHbmBytes;
@@ -995,7 +1042,11 @@ static Layout plan(Params* p, int T, int N, int K, int R, bool* pair) {
     const int sms = sm_count();
     *pair = plan_tiles(p);
     const int stage = kABytes + (*pair ? p->tok / 2 : p->tok) * kKBytes;
-    p->stages = kRingBytes / stage < kMaxStages ? kRingBytes / stage : kMaxStages;
+    // Few rows may each have an adapter of their own, whose B's come one after the other; of many some chunks where two requests meet
+    const int slot = kRows * R * 2, room = (T <= kMixedRows ? kMixedBytes : kFewMixedBytes) / (2 * slot);
+    p->slots = room < 1 ? 1 : room < kMaxSlots ? room : kMaxSlots;
+    const int left = kRingBytes - 2 * p->slots * slot;
+    p->stages = left / stage < kMaxStages ? left / stage : kMaxStages;
     Layout L{};
     size_t off = 0;
     auto add = [&](size_t bytes) {
@@ -1161,7 +1212,7 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
     p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
     const int split = (p.tiles - p.whole) * p.parts, busy = p.whole < p.groups ? (p.whole > split ? p.whole : split) : p.groups;
-    const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + (pair ? p.tok / 2 : p.tok) * lora::kKBytes) + sizeof(lora::Tail);
+    const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + (pair ? p.tok / 2 : p.tok) * lora::kKBytes) + size_t(2) * p.slots * lora::kRows * R * 2 + sizeof(lora::Tail);
     if (half)
         return pair ? lora::launch_project<true, true>(busy, smem, stream, xp, wm, zm, bm, p) : lora::launch_project<true, false>(busy, smem, stream, xp, wm, zm, bm, p);
     return pair ? lora::launch_project<false, true>(busy, smem, stream, xp, wm, zm, bm, p) : lora::launch_project<false, false>(busy, smem, stream, xp, wm, zm, bm, p);
