@@ -82,6 +82,18 @@ def test_against_64_bits(dtype, T, N, K, L, R, ids):
     assert torch.equal(ops.lora_linear(**a), out[:T])  # whichever block finishes a tile
 
 
+PAIRS = [  # large enough for pairs of blocks: whole tiles in one round and in two, split ones, a last tile of one block, ragged rows
+    (1214, 3096, 1280, 5, 16, 400), (2089, 3336, 1024, 9, 32, 37), (2413, 2312, 2048, 6, 64, 300), (2661, 1720, 2048, 40, 128, "random"),
+    (2989, 2480, 1024, 64, 8, 1), (1221, 3280, 1280, 3, 24, "none"),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T,N,K,L,R,ids", PAIRS)
+def test_large_batches_against_64_bits(dtype, T, N, K, L, R, ids):
+    test_against_64_bits(dtype, T, N, K, L, R, ids)
+
+
 @pytest.mark.parametrize("T", [5, 90, 400])
 def test_rows_that_lie_apart(T):
     """x as a slice of a wider matrix, y into one: what stands beside it stays."""
@@ -125,6 +137,41 @@ def test_inner_values_beyond_fp16(run):
     check(ops.lora_linear(**a), a, "fp16")
 
 
+@pytest.mark.parametrize("run", [512, 3])
+def test_inner_values_beyond_fp16_in_large_batches(run):
+    a = make(31, 1221, 3280, 1280, 2, 8, "fp16", run)
+    a["lora_a"].mul_(3e4)
+    a["lora_b"].mul_(1e-4)
+    a["scale"].fill_(4.0)
+    a["lora_a"][1].mul_(1e-4)  # one adapter stays in range: chunks with and without powers of two
+    check(ops.lora_linear(**a), a, "fp16")
+
+
+def test_large_batches_do_not_see_other_adapters():
+    a = make(33, 1214, 3096, 1280, 8, 16, "bf16", 150)
+    a["ids"][::97] = -1
+    clean = ops.lora_linear(**a)
+    bad = int(a["ids"][1])
+    a["lora_b"][bad, :, 3] = float("inf")
+    a["lora_a"][bad] = float("nan")
+    out = ops.lora_linear(**a)
+    hit = a["ids"] == bad
+    assert torch.equal(out[~hit], clean[~hit]) and out[hit].isnan().all() and ops.device_status() == 0
+
+
+def test_one_workspace_for_all_batches():
+    """A workspace for the longest batch serves all, one call after the other without waiting."""
+    T, N, K, L, R = 1300, 1536, 512, 12, 32
+    ws = torch.full((ops.lora_linear_workspace_bytes(T, N, K, L, R),), 0xff, dtype=torch.uint8, device="cuda")
+    a = make(35, T, N, K, L, R, ids=5)
+    got = []
+    for t in (1300, 1, 17, 640, 64, 255, 257, 1300, 31, 900):
+        part = {**a, "x": a["x"][:t], "ids": a["ids"][:t]}
+        got.append((part, ops.lora_linear(**part, workspace=ws)))
+    for part, out in got:
+        check(out, part)
+
+
 def test_captured_and_replayed():
     a = make(11, 48, 1024, 768, 16, 16)
     ws = torch.empty(ops.lora_linear_workspace_bytes(48, 1024, 768, 16, 16), dtype=torch.uint8, device="cuda")
@@ -156,6 +203,23 @@ def test_streams_at_once():
     streams = [torch.cuda.Stream() for _ in calls]
     got = [[] for _ in calls]
     for _ in range(5):
+        for i, (a, s) in enumerate(zip(calls, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.lora_linear(**a))
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+
+
+def test_large_batches_at_once():
+    """Pairs of blocks of two calls and a decode batch between them compete for the SMs."""
+    calls = [make(41 + i, *s) for i, s in enumerate([(1214, 3096, 1280, 5, 16), (40, 2048, 1024, 16, 16), (2413, 2312, 2048, 6, 64)])]
+    want = [ops.lora_linear(**a) for a in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(6):
         for i, (a, s) in enumerate(zip(calls, streams)):
             with torch.cuda.stream(s):
                 got[i].append(ops.lora_linear(**a))
