@@ -4,20 +4,29 @@
 //   shrink    z[t] = scale_a x[t] A_a^T, [T, R] in the operands' type
 //   project   y = x W^T + z B_a^T, summed in fp32
 //
-// What bounds it: few rows the weights W and the adapters in use from HBM, many rows the tensor cores. project runs with W on the
-// tensor core's first operand (M = 128 rows of W) and up to 224 rows of x on the second, so that a decode batch computes few columns too
-// many. Tiles that do not fill the chip are cut along K into equal shares per SM (streamk.cuh).
+// What bounds it: with few rows the weights W and the adapters in use from HBM, and a chain of latencies (shrink, the last sums, the sums over
+// parts); with hundreds the way from L2 to the SMs, some 60 bytes a cycle and SM (a K block of a tile of 128 x 256 takes 820 cycles to
+// arrive, its MMAs 512); with thousands the tensor cores at the clock that the power limit leaves. project runs with W on the tensor core's first
+// operand (M = 128 rows of W) and up to 256 rows of x on the second, so that a decode batch computes few columns too many; large batches take
+// pairs of blocks, each with half of the rows of x for both. Tiles that do not fill the chip are cut along K into equal parts (plan_tiles).
 //
-// The adapters' part is MMAs, too: B_a on the first operand, rows of z on the second, 16 rows (the least N) at a time. Where 16 rows have
-// one adapter - prefill, where a request's rows stand together - the product goes on top of x W^T, for all such rows that follow one
-// another at once. Where they have several, each adapter's product gets 16 accumulator columns of its own, and the epilogue adds the columns
-// whose rows have that adapter: masks on a mixed product would let one adapter's infinities reach the rows of another. (The first form of
-// this kernel added z B^T in the epilogue's threads, each with its row of B: bound by L1, whose lines hold one row of B each, and on the
-// last block of a tile alone. 64 rows of 64 adapters, K 4096, N 6144, R 16: 70 us; 333 rows of 40 requests, 2880 x 2880, R 64: 489 us.)
-// The list of these products is made from the ids by a warp of each block, and divided among the parts of a tile like its K.
+// The adapters' part has two forms, by chunk of 16 rows. Where a chunk has one adapter - prefill, where a request's rows stand together - B_a is
+// the first operand and z the second of MMAs on top of x W^T, for all such chunks that follow one another at once. Where it has several,
+// the epilogue's warps multiply m16n8k16 fragments, each adapter by itself, and take the columns whose rows have that adapter: masks on a mixed
+// product would let one adapter's infinities reach the rows of another. A block whose tile is its only one does that while the tensor core
+// still sums. The list of these products is made from the ids by a warp of each block, and divided among the parts of a tile like its K.
+// Forms of the second kind, us per call, for 64 rows of 64 adapters (K 4096, N 6144, R 16), and 333 fp16 rows of 40 requests (2880 x 2880, R 64):
+//   rows of B in threads, z B^T by FMAs                                                                      70, 489
+//   B and 16 rows of z through the stages into accumulators of their own, whose columns the epilogue picks   28, 38: 460 cycles of the
+//                                                                               one thread that issues the copies for each product
+//   fragments straight from L2, behind the sums / while the tensor core sums                                 24, 37 / 20, 31
+//   B through shared memory in slots of their own                                                            20, 28.5
 //
-// project starts while shrink runs: it reads only x and W until a tile's K is through. That is sound because shrink lets it start
+// project starts while shrink runs: it reads only x, W, ids and B until a tile's K is through. That is sound because shrink lets it start
 // behind its own wait for the kernels before, which wrote those. No counterpart in the reference.
+//
+// us per call: one row, 4096 x 4096, R 16 10.4 (3.2 TB/s; floor 5.2); 64 rows as above 20.0 (3.5 TB/s; floor 10.8); 333 as above 28.5 (floor 6.4);
+// 4096 rows of 6 requests, 4096 x 4096, R 32 113 (1.22 PFLOP/s); 8191 rows of 24, K 7168, N 4096, R 16 348 (1.39 PFLOP/s).
 #include <mutex>
 
 #include "common.cuh"
