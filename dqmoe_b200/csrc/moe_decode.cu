@@ -849,10 +849,11 @@ struct Finish {
         const int h = q.tile * kRows + row;
         float* group_sums = p.group2 + size_t(q.tile) * kGroups * S::kPart2;
         auto put_out = [&](int t0, const float (&sum)[8]) {
-            if (h < p.H)
+            if (h < p.H) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (t0 + i < p.T) p.out[size_t(t0 + i) * p.H + h] = __float2bfloat16_rn((bad >> (t0 + i)) & 1u ? __uint_as_float(0x7fffffffu) : sum[i]);
+            }
         };
 #pragma unroll 1
         for (int t0 = 0; t0 < p.T; t0 += 8) {

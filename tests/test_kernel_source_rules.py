@@ -165,3 +165,44 @@ def test_kernels_before_an_early_gemm_start_it_after_their_own_wait():
     mx = braces(mx, mx.index("__global__"))
     assert re.findall(r"if \((!?p\.early)\) pdl_launch\(\)", mx) == ["!p.early", "p.early"] and mx.count("pdl_launch()") == 2
     assert len(re.findall(r"pdl_wait\(\);\s*if \(p\.early\) pdl_launch\(\)", mx)) == 1
+
+
+def test_a_pragma_is_no_branch():
+    """`if constexpr (false)` with a pragma between it and its loop made nvcc drop what follows the loop as well."""
+    for name in sorted(os.listdir(CSRC)):
+        assert not re.search(r"\b(if|else)\b[^\n;{]*\n#pragma", source(name)), name
+
+
+def test_operators_for_few_rows_wait_by_whole_warps():
+    """Roles of moe_decode and lora_linear that a whole warp plays: see test_roles_of_a_whole_warp_wait_together."""
+    decode, lora = source("moe_decode.cu"), source("lora.cu")
+    for text, role in ((decode, "struct Drain {"), (decode, "struct Finish {"), (lora, "struct Epilogue {")):
+        body = braces(text, text.index(role))
+        assert "mbar_wait_warp(" in body and not re.search(r"\bmbar_wait\(", body), role
+    multiply = braces(decode, decode.index("void multiply("))
+    assert "mbar_wait_warp(" in multiply and "next_piece<true>" in multiply and not re.search(r"\bmbar_wait\(", multiply)
+    kernel = braces(lora, lora.index("lora_project_kernel("))
+    for role in ("else if (warp == 2) {", "else if (warp == 3) {"):
+        body = braces(kernel, kernel.index(role))
+        assert "mbar_wait_warp(" in body and not re.search(r"\bmbar_wait\(", body), role
+
+
+def test_tmem_loads_and_their_wait_are_one_statement():
+    """The registers of a tcgen05.ld are written at some time until its wait: moe_decode and lora_linear have them as results of both together."""
+    helpers = source("ptx_sm100.cuh")
+    for name in ("tmem_read", "tmem_read2", "tmem_read_fragments"):
+        body = braces(helpers, helpers.index(f"void {name}("))
+        assert body.count("asm volatile(") == body.count("tcgen05.wait::ld") > 0, name
+    for name in ("moe_decode.cu", "lora.cu"):
+        assert not re.search(r"tmem_ld|tmem_wait_ld", source(name)), name
+
+
+def test_lora_reads_what_shrink_writes_past_l1():
+    """project is resident while shrink still writes z and z_scale, and reads the ids before its own wait."""
+    text = source("lora.cu")
+    project = text[text.index("struct Params {"):text.index("static int make_map(")]
+    reads = re.findall(r"p\.(?:z|z_scale|ids)\b(?! =)[^;]*;", project)
+    assert reads
+    for m in re.finditer(r"p\.(z|z_scale|ids) ?[+\[]", project):
+        before = project[max(0, m.start() - 20):m.start()]
+        assert "[" not in m.group(0) and re.search(r"(load16|load_f32|ld_relaxed_gpu)\($", before), project[m.start() - 60:m.end() + 20]
