@@ -975,10 +975,10 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
     if (threadIdx.x == 32 * 3) ptx::prefetch_tensormap(&map_b1);
     pdl_wait();
     int claim = 0;
-    if (threadIdx.x == 0) claim = atomicAdd(&p.counters[0], 1);
-    claim = __shfl_sync(0xffffffffu, claim, 0);
+    if (threadIdx.x == 0) claim = atomicAdd(&p.counters[0], 1);  // looked at behind the choice, which does not need it
     choose(p, st, warp, lane);
     __syncthreads();
+    if (warp == 0) claim = __shfl_sync(0xffffffffu, claim, 0);
     const uint32_t tmem = *const_cast<volatile uint32_t*>(&st.tmem_base);
 
     if (st.n_hit == 0) {  // no token has an expert
