@@ -1013,6 +1013,8 @@ struct Layout {
 // leave TMEM behind the last MMA; parts are written, counted and added. N = K = 4096, us per call without adapters: 1 row 1 part of a tile each
 // 22, 4 parts 12.8; 128 rows in one tile of 4 parts 18.3, in two of 2 parts 17.7; 512 rows in 4 tiles of 128 27.8, with what had one part
 // more or less in each block's share 41.5; 4096 rows on single blocks 110.8, on pairs 103.1.
+// Parts add through L2. As clusters that send their sums through distributed shared memory one row took 12.4 instead of 10.5 (4 parts), 64 rows of
+// 64 adapters (N 6144, R 16; 3 parts) 22.6 / 20.0: clusters start late and do not fill the chip (of three blocks 45 fit).
 constexpr int kL2Bytes[2] = {60, 45};                // per cycle and SM, on single blocks and on pairs
 constexpr int kHbmBytes = 3300;                      // per cycle
 constexpr int kDrain = 12, kCount = 3000, kAdd = 8;  // cycles a column; a tile in parts; a column of each part

@@ -216,7 +216,8 @@ int dqmoe_moe_block_shared(const void* x_bf16, const float* logits, const void* 
  * dqmoe_moe_block, which quantises both operands, the results differ by that quantisation. T <= 32, E + n_shared <= 1024, k <= 32, H and I
  * multiples of 16, operands aligned to 16 bytes. A token whose weights are not numbers (no logit above -inf) gets NaN, and so does
  * one whose x holds an infinity or a NaN in the FP8 modes; it changes no other token's result. The status codes of
- * dqmoe_device_status are 301 and 302. A call has its workspace for itself until it is over. No counterpart in the reference.
+ * dqmoe_device_status are 301 and 302. A call has its workspace for itself until it is over; out and the workspace overlap no operand. No
+ * counterpart in the reference.
  */
 size_t dqmoe_moe_decode_workspace_bytes(int T, int H, int I, int E, int k, int n_shared, int quant_mode);
 int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, const void* b, const float* b_scale,
@@ -498,8 +499,9 @@ int dqmoe_grouped_gemm_nvfp4(const void* a, const uint8_t* a_sf, const float* a_
  * A row whose id is outside [0, L) has no adapter. Adapters of a lower rank are padded with zeros to R, a multiple of 8 up to 128; K is a
  * multiple of 8; x, w, lora_a, lora_b are aligned to 16 bytes. The ids may come in any order; rows of one request that stand together
  * are faster. Sums are fp32, scale[a] * (x A_a^T) and the result are rounded to the operands' type (fp16: with a power of two per row
- * where the former leaves its range). No row's result depends on another row's adapter. Any T from 0 on. dqmoe_device_status gives 311 or 312 where a wait ran out. A call has its workspace for itself until it is over. No counterpart in
- * the reference.
+ * where the former leaves its range). No row's result depends on another row's adapter. Any T from 0 on. The status codes of
+ * dqmoe_device_status are 311 and 312. A call has its workspace for itself until it is over; y and the workspace overlap no operand. No
+ * counterpart in the reference.
  */
 size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R);
 int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lora_a, const void* lora_b, const int32_t* ids,

@@ -172,6 +172,34 @@ def test_one_workspace_for_all_batches():
         check(out, part)
 
 
+@pytest.mark.parametrize("T,N,K,L,R,ids", [(1, 4096, 4096, 8, 16, 1), (48, 2048, 1024, 16, 128, 1), (333, 2880, 512, 32, 64, 9), (1214, 3096, 1280, 5, 16, 400)])
+def test_the_workspace_is_all_that_it_needs(T, N, K, L, R, ids):
+    need = ops.lora_linear_workspace_bytes(T, N, K, L, R)
+    ws = torch.full((need + (1 << 20),), 0xa5, dtype=torch.uint8, device="cuda")
+    a = make(51, T, N, K, L, R, ids=ids)
+    check(ops.lora_linear(**a, workspace=ws[:need]), a)
+    assert (ws[need:] == 0xa5).all()
+
+
+def test_adapters_far_apart():
+    """Adapters whose B begins behind 2^31 elements."""
+    T, N, K, L, R = 40, 28672, 64, 600, 128
+    assert (L - 1) * N * R > 1 << 31
+    b = torch.empty(L, N, R, dtype=torch.bfloat16, device="cuda")
+    a = make(53, T, N, K, 3, R, ids=13)  # as three adapters ...
+    b[0], b[1], b[L - 1] = a["lora_b"][0], a["lora_b"][1], a["lora_b"][2]
+    far_a = torch.zeros(L, R, K, dtype=torch.bfloat16, device="cuda")
+    far_a[0], far_a[1], far_a[L - 1] = a["lora_a"][0], a["lora_a"][1], a["lora_a"][2]
+    far_scale = torch.ones(L, device="cuda")
+    far_scale[[0, 1, L - 1]] = a["scale"]
+    for ids in (a["ids"], torch.arange(T, dtype=torch.int32, device="cuda") % 3):  # direct products and mixed ones
+        near = {**a, "ids": ids}
+        far = {**near, "ids": torch.where(ids == 2, L - 1, ids).int(), "lora_a": far_a, "lora_b": b, "scale": far_scale}
+        out = ops.lora_linear(**far)
+        check(out, near)
+        assert torch.equal(out, ops.lora_linear(**near))
+
+
 def test_captured_and_replayed():
     a = make(11, 48, 1024, 768, 16, 16)
     ws = torch.empty(ops.lora_linear_workspace_bytes(48, 1024, 768, 16, 16), dtype=torch.uint8, device="cuda")

@@ -186,6 +186,18 @@ def test_small_and_large_values_of_a_group(mode):
     assert out.isfinite().all()
 
 
+@pytest.mark.parametrize("mode", list(MODES))
+@pytest.mark.parametrize("T,H,I,E,k,shared", [(1, 1024, 2048, 8, 2, 0), (5, 528, 272, 6, 3, 1), (16, 2048, 768, 24, 4, 0), (32, 1024, 512, 40, 8, 2)])
+def test_the_workspace_is_all_that_it_needs(mode, T, H, I, E, k, shared):
+    need = ops.moe_decode_workspace_bytes(T, H, I, E, k, shared, MODES[mode])
+    ws = torch.full((need + (1 << 20),), 0xa5, dtype=torch.uint8, device="cuda")
+    ws[:need] = 0xff  # NaN, as floats
+    a = make(61 + T, mode, T, H, I, E, k, shared)
+    out = ops.moe_decode(**a, workspace=ws[:need])
+    check(out, *reference(a))
+    assert (ws[need:] == 0xa5).all()
+
+
 def test_captured_and_replayed_on_another_stream():
     a = make(19, "block", 8, 1024, 512, 16, 4, shared=1)
     ws = torch.empty(ops.moe_decode_workspace_bytes(8, 1024, 512, 16, 4, 1, 1024), dtype=torch.uint8, device="cuda")
