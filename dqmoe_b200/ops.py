@@ -53,8 +53,8 @@ def _raw_stream(index: int) -> int:
 
 def _call(index: int, fn, *args) -> None:
     """fn(*args, current stream) with device `index` current. Entering torch.cuda.device and building a Stream object cost 4 us of a call that
-    takes the GPU 15, so neither is done where the device is current already."""
-    if torch.cuda.current_device() == index:
+    takes the GPU 10, so neither is done where the device is current already."""
+    if torch._C._cuda_getDevice() == index:  # CUDA is up: the operands are there
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -215,17 +215,20 @@ def moe_decode(x: torch.Tensor, w_router: torch.Tensor, b: torch.Tensor, b_scale
     T, H, E, I = _moe_decode_sizes(x, w_router, b, b_scale, b1, b1_scale, quant_mode, n_shared, dev)
     lib = _lib.load()
     if workspace is None:
-        workspace = torch.empty(max(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode), 256), dtype=torch.uint8, device=dev)
+        nbytes = max(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode), 256)
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
     if out is None:
-        out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_like(x)
     elif out.shape != (T, H) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is contiguous bf16 [T, H] on x's device")
     fp8 = quant_mode != QUANT_NONE
     _call(dev.index, lib.dqmoe_moe_decode, x.data_ptr(), w_router.data_ptr(), DT_FLOAT if w_router.dtype is torch.float32 else DT_BF16,
           b.data_ptr(), b_scale.data_ptr() if fp8 else None, b1.data_ptr(), b1_scale.data_ptr() if fp8 else None, out.data_ptr(),
-          workspace.data_ptr(), workspace.numel() * workspace.element_size(), T, H, I, E, k, n_shared, mode, quant_mode)
+          workspace.data_ptr(), nbytes, T, H, I, E, k, n_shared, mode, quant_mode)
     return out
 
 
@@ -615,23 +618,28 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
     dev, dtype = x.device, x.dtype
     T, K, N, L, R = _lora_sizes(x, w, lora_a, lora_b, ids, scale, bias, dev)
     if out is None:
-        out = torch.empty((T, N), dtype=dtype, device=dev)
+        out = x.new_empty((T, N))
+        ldy = N
     elif out.shape != (T, N) or out.dtype is not dtype or out.device != dev or not _rows_apart(out):
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is [T, N] of x's type, on its device, its rows apart and its columns together")
+    else:
+        ldy = N if out.is_contiguous() else out.stride(0)
     lib = _lib.load()
     if workspace is None:
-        workspace = torch.empty(max(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R), 256), dtype=torch.uint8, device=dev)
+        nbytes = max(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R), 256)
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
-    _call(dev.index, lib.dqmoe_lora_linear, x.data_ptr(), x.stride(0) if T > 1 else (K + 7) // 8 * 8, w.data_ptr(), lora_a.data_ptr(),
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    _call(dev.index, lib.dqmoe_lora_linear, x.data_ptr(), K if x.is_contiguous() else x.stride(0), w.data_ptr(), lora_a.data_ptr(),
           lora_b.data_ptr(), ids.data_ptr(), None if scale is None else scale.data_ptr(), None if bias is None else bias.data_ptr(),
-          out.data_ptr(), out.stride(0) if T > 1 else N, workspace.data_ptr(), workspace.numel() * workspace.element_size(), T, N, K, L, R,
-          DT_HALF if dtype is torch.float16 else DT_BF16)
+          out.data_ptr(), ldy, workspace.data_ptr(), nbytes, T, N, K, L, R, DT_HALF if dtype is torch.float16 else DT_BF16)
     return out
 
 
 def _rows_apart(t: torch.Tensor) -> bool:
-    return (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
+    return t.is_contiguous() or ((t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]))
 
 
 def _lora_sizes(x, w, lora_a, lora_b, ids, scale, bias, dev):
