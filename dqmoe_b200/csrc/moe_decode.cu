@@ -293,7 +293,7 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 // of equal parts, which saves the second level of sums, unless that costs more units than it stands for.
 // Parts without / with regard to what counting them costs, us per call: H 1024, I 2048, 8 experts in block FP8, 5 tokens 26.1 / 23.2, 32 tokens
 // 57 / 40. The same for longer tiles or parts lengthens the wait for the slowest block: 16 tokens of 128 experts (H 2048, I 768) 91 / 112,
-// one token of 32 experts (H 7168, I 2048) 77.5 / 80.9.
+// one token of 32 experts (H 7168, I 2048) 77.5 / 80.9; in fc2 alone from six units a block on, 4 tokens of the 128 experts 44.4 / 48.5.
 constexpr int kShortUnits = 16;
 constexpr int kCountUnits = 6;  // a counter, the sums and their hand-over take some 4 us, a unit 0.6
 __device__ __forceinline__ void plan_pieces(const Params& p, Tail& st, int n_hit, int lane) {
@@ -314,7 +314,8 @@ __device__ __forceinline__ void plan_pieces(const Params& p, Tail& st, int n_hit
     if (shrinking == 0) knee = float(units);
     int equal = max(1, min(kMaxParts - kMaxShrinking, int(knee / least)));
     const int few = min(kGroup, units), few_cost = few > 0 ? (p.tiles2 * few + p.blocks - 1) / p.blocks * ((units + few - 1) / few) : 0;
-    if (few_cost <= kShortUnits && float(few_cost) <= float(p.tiles2) / float(p.blocks) * float(units) + float(kCountUnits)) {
+    const float even = float(p.tiles2) / float(p.blocks) * float(units);  // units of a block
+    if (even <= float(kCountUnits) && float(few_cost) <= even + float(kCountUnits)) {
         shrinking = 0;
         knee = float(units);
         equal = max(1, few);
