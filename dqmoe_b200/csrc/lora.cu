@@ -1008,17 +1008,17 @@ struct Layout {
     size_t counters, z, z_scale, part, total;
 };
 // Tiles of x's rows, blocks or pairs, and parts, by an estimate in clock cycles, whose constants are fits to measurements (all forms, 1 to 8191
-// rows, N 2880 to 14336, K 2880 to 7168; the form chosen is within 4 % of the fastest): a K block of a tile takes its MMAs (two cycles a row)
-// or its bytes from L2; W and x come from HBM once, and of the two the shorter one costs a quarter of its time beside the longer; a tile's last sums
+// rows, N 2880 to 14336, K 2880 to 7168; the form chosen is within 5 % of the fastest): a K block of a tile takes its MMAs (two cycles a row)
+// or its bytes from L2; W and x come from HBM once, and of the two the shorter one costs half of its time beside the longer; a tile's last sums
 // leave TMEM behind the last MMA; parts are written, counted and added. N = K = 4096, us per call without adapters: 1 row 1 part of a tile each
 // 22, 4 parts 12.8; 128 rows in one tile of 4 parts 18.3, in two of 2 parts 17.7; 512 rows in 4 tiles of 128 27.8, with what had one part
 // more or less in each block's share 41.5; 4096 rows on single blocks 110.8, on pairs 103.1.
 // Parts add through L2. As clusters that send their sums through distributed shared memory one row took 12.4 instead of 10.5 (4 parts), 64 rows of
 // 64 adapters (N 6144, R 16; 3 parts) 22.6 / 20.0: clusters start late and do not fill the chip (of three blocks 45 fit).
-constexpr int kL2Bytes[2] = {60, 45};                // per cycle and SM, on single blocks and on pairs
+constexpr int kL2Bytes[2] = {60, 47};                // per cycle and SM, on single blocks and on pairs
 constexpr int kHbmBytes = 3300;                      // per cycle
-constexpr int kDrain = 12, kCount = 3000, kAdd = 8;  // cycles a column; a tile in parts; a column of each part
-constexpr int kPairing = 1500;
+constexpr int kDrain = 12, kAdd = 8;                 // cycles a column; a column of each part
+constexpr int kPairing[2] = {0, 700}, kCount[2] = {3000, 5500};  // a launch; a tile in parts
 constexpr int kMixedRows = 512, kMixedBytes = 64 * 1024, kFewMixedBytes = 24 * 1024;
 static bool plan_tiles(Params* p) {
     const int sms = sm_count();
@@ -1035,8 +1035,8 @@ static bool plan_tiles(Params* p) {
             const int most = rest == 0 ? 1 : (groups / rest < kMaxParts ? (groups / rest < p->kbs ? groups / rest : p->kbs) : kMaxParts);
             for (int parts = 1; parts <= most; ++parts) {
                 const int64_t kbs = int64_t(tiles / groups) * p->kbs + (rest > 0 ? ceil_div(p->kbs, parts) : 0);
-                const int64_t tail = tok * kDrain + (parts > 1 ? kCount + parts * tok * kAdd : 0) + pair * kPairing, sum = kbs * kb;
-                const int64_t cost = (sum > hbm ? sum + hbm / 4 : hbm + sum / 4) + tail;
+                const int64_t tail = tok * kDrain + (parts > 1 ? kCount[pair] + parts * tok * kAdd : 0) + kPairing[pair], sum = kbs * kb;
+                const int64_t cost = (sum > hbm ? sum + hbm / 2 : hbm + sum / 2) + tail;
                 if (cost >= best) continue;
                 best = cost, best_pair = pair != 0;
                 p->tok = tok, p->n_tiles = n_tiles, p->tiles = tiles, p->groups = groups;

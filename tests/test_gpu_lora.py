@@ -85,6 +85,7 @@ def test_against_64_bits(dtype, T, N, K, L, R, ids):
 PAIRS = [  # large enough for pairs of blocks: whole tiles in one round and in two, split ones, a last tile of one block, ragged rows
     (1214, 3096, 1280, 5, 16, 400), (2089, 3336, 1024, 9, 32, 37), (2413, 2312, 2048, 6, 64, 300), (2661, 1720, 2048, 40, 128, "random"),
     (2989, 2480, 1024, 64, 8, 1), (1221, 3280, 1280, 3, 24, "none"),
+    (1282, 3384, 2400, 6, 16, 300), (3899, 1200, 2048, 20, 64, 61), (2916, 656, 4096, 8, 40, "random"),
 ]
 
 
