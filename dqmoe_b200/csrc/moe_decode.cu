@@ -33,6 +33,7 @@
 // fc2's first MMA (8), and behind the last (5): nearly all of the smallest case.
 //
 // No counterpart in the reference, whose runner (csrc/moe_kernels.h:770-892) takes routed rows and five launches.
+#include <cmath>
 #include <mutex>
 
 #include "common.cuh"
@@ -85,6 +86,7 @@ struct Params {
     int kb1, pairs2;          // K blocks of fc1; pairs of K blocks of fc2
     int tiles1, tiles2;       // tiles of 128 rows of I and H
     int blocks;
+    float share, per_share, shrink_rate, even;  // of fc2's parts, see plan_parts2
     int max_hit;              // experts hit at most
     int n_counters;
     size_t rec1, rec2;        // bytes of a unit's second operand with its scales
@@ -268,7 +270,7 @@ struct alignas(16) Tail {
     int abort_flag;
     int n_hit;
     int whole1, split1, pieces1;               // fc1 tiles in one piece; parts of each of the others; pieces of fc1
-    int parts2, pieces2;                       // parts of an fc2 tile; pieces of both
+    int parts2;                                // of an fc2 tile
     int bound2[kMaxParts + 1];                 // first unit of each part of an fc2 tile
     uint32_t bad_tokens;                       // tokens without a number among their weights
     int last;
@@ -283,7 +285,7 @@ struct alignas(16) Tail {
 constexpr size_t kSmemBytes = 1024 + size_t(kRingBytes) + sizeof(Tail);
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 
-// Pieces of the work, from the experts that are hit; by one warp.
+// Pieces of the work, from the experts that are hit, fc1's and fc2's by a warp each. Approximate logarithms and quotients do: all blocks get the same.
 // fc1: whole tiles, but the last ones, one per block, in parts of some eight units, three pieces per block at least, so that fc1's end is not
 // waited for long. Few short tiles: in as many parts as make the longest block's share shortest, where counting and adding parts stands for
 // kCountUnits units.
@@ -296,44 +298,47 @@ static_assert(kSmemBytes <= 227 * 1024, "shared memory of one block");
 // one token of 32 experts (H 7168, I 2048) 77.5 / 80.9; in fc2 alone from six units a block on, 4 tokens of the 128 experts 44.4 / 48.5.
 constexpr int kShortUnits = 16;
 constexpr int kCountUnits = 6;  // a counter, the sums and their hand-over take some 4 us, a unit 0.6
-__device__ __forceinline__ void plan_pieces(const Params& p, Tail& st, int n_hit, int lane) {
+__device__ __forceinline__ void plan_pieces1(const Params& p, Tail& st, int n_hit, int lane) {
     const int tiles1 = n_hit * p.tiles1, cut = min(tiles1, p.blocks);
     const int most = max(1, min(kMaxSplit1, p.kb1 / 2));
-    int split = max(1, min(max(p.kb1 / 8, (3 * p.blocks + tiles1 - 1) / max(tiles1, 1)), most));
+    int split = max(1, min(max(p.kb1 / 8, int(__fdividef(float(3 * p.blocks), float(max(tiles1, 1))) + 0.999f)), most));
     if (tiles1 <= p.blocks && p.kb1 <= kShortUnits) {
         const int mine = lane + 1;  // a lane for each number of parts
         const int cost = mine <= most ? (tiles1 * mine + p.blocks - 1) / p.blocks * ((p.kb1 + mine - 1) / mine) + (mine > 1 ? kCountUnits : 0) : 0x7fffff;
         split = int(__reduce_min_sync(0xffffffffu, unsigned(cost) * 32u + lane) & 31u) + 1;
     }
-    const int units = n_hit * p.pairs2;
-    const float share = fminf(0.5f, float(p.tiles2) / float(2 * p.blocks));  // of what is left, per part
-    const float least = fmaxf(1.0f, fminf(4.0f, float(units) * share));
-    float knee = fminf(float(units), least / share);
-    int shrinking = 0;
-    if (knee < float(units)) shrinking = min(kMaxShrinking, int(log2f(float(units) / knee) / -log2f(1.0f - share)));
-    if (shrinking == 0) knee = float(units);
-    int equal = max(1, min(kMaxParts - kMaxShrinking, int(knee / least)));
-    const int few = min(kGroup, units), few_cost = few > 0 ? (p.tiles2 * few + p.blocks - 1) / p.blocks * ((units + few - 1) / few) : 0;
-    const float even = float(p.tiles2) / float(p.blocks) * float(units);  // units of a block
-    if (even <= float(kCountUnits) && float(few_cost) <= even + float(kCountUnits)) {
-        shrinking = 0;
-        knee = float(units);
-        equal = max(1, few);
-    }
-    const float step = shrinking > 0 ? log2f(knee / float(units)) / float(shrinking) : 0.0f;
-    for (int q = lane; q < shrinking + equal; q += 32)
-        st.bound2[q] = int(0.001f +  // against a whole number that came out a little less
-                           (q < shrinking ? float(units) * (1.0f - exp2f(step * float(q))) : float(units) - knee * (1.0f - float(q - shrinking) / float(equal))));
     if (lane == 0) {
         st.n_hit = n_hit;
         st.whole1 = tiles1 - cut;
         st.split1 = split;
         st.pieces1 = tiles1 - cut + cut * split;
-        st.bound2[shrinking + equal] = units;
-        st.parts2 = units > 0 ? shrinking + equal : 0;
-        st.pieces2 = st.pieces1 + st.parts2 * p.tiles2;
     }
 }
+__device__ __forceinline__ void plan_parts2(const Params& p, Tail& st, int n_hit, int lane) {
+    const int units = n_hit * p.pairs2;
+    const float all = float(units), log_all = __log2f(all);
+    const float least = fmaxf(1.0f, fminf(4.0f, all * p.share));
+    float knee = fminf(all, least * p.per_share), log_knee = __log2f(knee);
+    int shrinking = knee < all ? min(kMaxShrinking, int((log_all - log_knee) * p.shrink_rate)) : 0;
+    if (shrinking == 0) knee = all;
+    int equal = max(1, min(kMaxParts - kMaxShrinking, int(__fdividef(knee, least))));
+    const int few = min(kGroup, units), few_cost = few > 0 ? (p.tiles2 * few + p.blocks - 1) / p.blocks * ((units + few - 1) / few) : 0;
+    const float even = p.even * all;  // units of a block
+    if (even <= float(kCountUnits) && float(few_cost) <= even + float(kCountUnits)) {
+        shrinking = 0;
+        knee = all;
+        equal = max(1, few);
+    }
+    const float step = shrinking > 0 ? __fdividef(log_knee - log_all, float(shrinking)) : 0.0f, each = __fdividef(knee, float(equal));
+    for (int q = lane; q < shrinking + equal; q += 32)
+        st.bound2[q] = q == 0 ? 0 : int(0.001f +  // against a whole number that came out a little less
+                           (q < shrinking ? all * (1.0f - exp2f(step * float(q))) : all - each * float(shrinking + equal - q)));
+    if (lane == 0) {
+        st.bound2[shrinking + equal] = units;
+        st.parts2 = units > 0 ? shrinking + equal : 0;
+    }
+}
+__device__ __forceinline__ int all_pieces(const Params& p, const Tail& st) { return st.pieces1 + st.parts2 * p.tiles2; }
 
 struct Piece {
     int phase;       // 0 fc1, 1 fc2, 2 no more, 3 a wait has run out
@@ -342,7 +347,7 @@ struct Piece {
 };
 __device__ __forceinline__ Piece piece_at(const Params& p, const Tail& st, int c) {
     Piece q;
-    if (c >= st.pieces2) return Piece{2, 0, 0, 0, 0};
+    if (c >= all_pieces(p, st)) return Piece{2, 0, 0, 0, 0};
     if (c < st.pieces1) {
         q.phase = 0;
         const int cut = c - st.whole1;
@@ -417,7 +422,7 @@ __device__ __forceinline__ void load_weights(const Params& p, const CUtensorMap&
     bool ok = true;
     for (int n = 0; ok; ++n) {
         const int slot = n % kClaims;
-        const int next = claim < st.pieces2 ? atomicAdd(&p.counters[0], 1) : claim;  // known by the time it is needed
+        const int next = claim < all_pieces(p, st) ? atomicAdd(&p.counters[0], 1) : claim;  // known by the time it is needed
         if (!(ok = ptx::mbar_wait(&st.claim_empty[slot], ((n / kClaims) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
         *const_cast<volatile int*>(&st.claim[slot]) = claim;
         ptx::mbar_arrive(&st.claim_full[slot]);
@@ -911,23 +916,27 @@ __device__ __forceinline__ void choose(const Params& p, Tail& st, int warp, int 
     else if (p.E <= 256) choose_topk<8>(p, st, warp, lane);
     else choose_topk<32>(p, st, warp, lane);
     __syncthreads();
-    if (warp == 0) {
+    if (warp < 2) {  // each for its part of the plan: one after the other they took 2 us
         int count = 0;
         for (int e0 = 0; e0 < p.E; e0 += 32) {
             const uint32_t m = e0 + lane < p.E ? st.mask[e0 + lane] : 0u;
             const uint32_t hits = __ballot_sync(0xffffffffu, m != 0);
-            const int at = count + __popc(hits & ((1u << lane) - 1u));
-            if (m != 0) {
+            if (warp == 0 && m != 0) {
+                const int at = count + __popc(hits & ((1u << lane) - 1u));
                 st.hit[at] = uint16_t(e0 + lane);
                 st.hit_mask[at] = m;
             }
             count += __popc(hits);
         }
-        for (int i = lane; i < p.n_shared; i += 32) {
-            st.hit[count + i] = uint16_t(p.E + i);
-            st.hit_mask[count + i] = all_tokens(p);
+        if (warp == 0) {
+            for (int i = lane; i < p.n_shared; i += 32) {
+                st.hit[count + i] = uint16_t(p.E + i);
+                st.hit_mask[count + i] = all_tokens(p);
+            }
+            plan_pieces1(p, st, count + p.n_shared, lane);
+        } else {
+            plan_parts2(p, st, count + p.n_shared, lane);
         }
-        plan_pieces(p, st, count + p.n_shared, lane);
     }
 }
 
@@ -1028,6 +1037,10 @@ static Layout plan(Params* p, bool fp8) {
     p->rec1 = size_t(fc1_cols(fp8, tp)) * kKBytes + (fp8 ? size_t(tp) * sizeof(float) : 0);
     p->rec2 = size_t(2) * fc2_cols(tp) * kKBytes + (fp8 ? size_t(2) * tp * sizeof(float) : 0);
     p->blocks = sm_count();
+    p->even = float(p->tiles2) / float(p->blocks);
+    p->share = p->even < 1.0f ? 0.5f * p->even : 0.5f;  // of what is left, per part
+    p->per_share = 1.0f / p->share;
+    p->shrink_rate = -1.0f / log2f(1.0f - p->share);
     p->n_counters = 4 + p->max_hit + p->max_hit * p->tiles1 + p->tiles2 * (kGroups + 1);
     Layout L{};
     size_t off = 0;
