@@ -499,7 +499,7 @@ int dqmoe_grouped_gemm_nvfp4(const void* a, const uint8_t* a_sf, const float* a_
  * A row whose id is outside [0, L) has no adapter. Adapters of a lower rank are padded with zeros to R, a multiple of 8 up to 128; K is a
  * multiple of 8; x, w, lora_a, lora_b are aligned to 16 bytes. The ids may come in any order; rows of one request that stand together
  * are faster. Sums are fp32, scale[a] * (x A_a^T) and the result are rounded to the operands' type (fp16: with a power of two per row
- * where the former leaves its range). No row's result depends on another row's adapter. Any T from 0 on. The status codes of
+ * where the row's largest value of the former is above 2^15 or below R 2^-14, so that rows of any magnitude keep the type's precision). No row's result depends on another row's adapter. Any T from 0 on. The status codes of
  * dqmoe_device_status are 311 and 312. A call has its workspace for itself until it is over; y and the workspace overlap no operand. No
  * counterpart in the reference.
  */
