@@ -51,7 +51,9 @@ __device__ __forceinline__ void topk_of_token(const float* row, int E, int k, in
         }
     }
     const float m = __shfl_sync(0xffffffffu, value, 0);
-    const float score = scoring == DQMOE_SCORE_SIGMOID ? 1.0f / (1.0f + expf(-value)) : expf(value - m);
+    // sigmoid(v) = e^v / (1 + e^v). expf(-v) overflows from v = -88.8 down, where this is 0: a loss below 2^-24 of the largest chosen score as long as
+    // that one's m is -72 or more. Below, 1 + e^v is 1 in fp32, and e^(v - m) the same ratios.
+    const float score = scoring == DQMOE_SCORE_SIGMOID && !(m < -72.0f) ? 1.0f / (1.0f + expf(-value)) : expf(value - m);
     float denom = 0.0f;
     for (int j = 0; j < k; ++j) denom += __shfl_sync(0xffffffffu, score, j);
     if (lane < k) {
