@@ -267,11 +267,6 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                         ptx::tma_load_2d(a + i * p.R * kKBytes, &map_a, kb * kKElems, st.adapter[g * cap + i] * p.R, &st.full[s]);
                 }
             }
-            if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
-                const long long t0 = clock64();
-                for (int i = max(0, it - p.stages); i < it; ++i)
-                    while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - t0 < kWaitLimit) {}
-            }
         }
         __syncwarp();
     } else if (warp == 1 && kb0 < kb1) {
@@ -326,6 +321,7 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             if (lane == 0) ptx::mbar_arrive(&st.tmem_empty[acc & 1]);
         }
     }
+    ptx::settle_after_abort(&st.abort_flag);
     __syncthreads();
     if (threadIdx.x == 0 && st.abort_flag != 0) *p.status = kStatusShrink;
     if (warp == 1) {
@@ -829,15 +825,6 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 else ok = ok && (n > 1 || products(held, 0)) && products(q, n);
                 if (n == 0 && pieces.left() == 0) ok = ok && products(q, 0);
             }
-            if (*const_cast<volatile int*>(&st.abort_flag) != 0) {  // nobody leaves with copies in flight
-                if constexpr (kPair) {  // whose barriers are the first block's, which may have got fewer than it expects
-                    for (int i = 0; i < 2000; ++i) __nanosleep(1000);
-                } else {
-                    const long long begin = clock64();
-                    for (int i = max(0, it - p.stages); i < it; ++i)
-                        while (!ptx::mbar_try_wait(&st.full[i % p.stages], (i / p.stages) & 1) && clock64() - begin < kWaitLimit) {}
-                }
-            }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -970,15 +957,12 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&st.list_empty[n & 1]);
         }
-        if (*const_cast<volatile int*>(&st.abort_flag) != 0 && uses > 0) {  // nobody leaves with copies in flight
-            const long long begin = clock64();
-            while (!ptx::mbar_try_wait(&st.b_full[h][slot], (uses - 1) & 1) && clock64() - begin < kWaitLimit) {}
-        }
         __syncwarp();
     } else if (warp >= 4) {
         Epilogue<kHalf, kPair> ep{p, st, tmem + (uint32_t((warp & 3) * 32) << 16), warp - 4, lane, (warp & 3) * 32 + lane, rank, b_ring};
         ep.run();
     }
+    ptx::settle_after_abort(&st.abort_flag);
     ptx::tc_fence_before();
     __syncthreads();
     if constexpr (kPair) ptx::cluster_sync();  // the other block is through with this one's barriers and shared memory

@@ -406,15 +406,6 @@ struct Shape {
     static constexpr size_t kPart1 = size_t(2) * kTp * kRows, kPart2 = size_t(kTp) * kRows;  // floats
 };
 
-// A stage is filled by two threads; nobody may leave with copies in flight. Where all went well the other roles have waited for each.
-template <int kStages>
-__device__ __forceinline__ void drain_copies(Tail& st, int it) {
-    if (*const_cast<volatile int*>(&st.abort_flag) == 0) return;
-    const long long t0 = clock64();
-    for (int i = max(0, it - kStages); i < it; ++i)
-        while (!ptx::mbar_try_wait(&st.full[i % kStages], (i / kStages) & 1) && clock64() - t0 < kWaitLimit) {}
-}
-
 template <bool kFp8, int kTp>
 __device__ __forceinline__ void load_weights(const Params& p, const CUtensorMap& map_b, const CUtensorMap& map_b1, Tail& st, uint8_t* ring, int claim) {
     using S = Shape<kFp8, kTp>;
@@ -446,7 +437,6 @@ __device__ __forceinline__ void load_weights(const Params& p, const CUtensorMap&
         }
         claim = next;
     }
-    drain_copies<S::kStages>(st, it);
 }
 
 template <bool kFp8, int kTp>
@@ -486,7 +476,6 @@ __device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* 
             ptx::bulk_load(b, p.aq + size_t(u) * p.rec2, uint32_t(p.rec2), &st.full[s]);  // [expert][pair], as the units
         }
     }
-    drain_copies<S::kStages>(st, it);
 }
 
 // The MMAs of every unit, issued by one thread; by the whole warp because it also takes the scales of a unit's tokens out of its stage (FP8), to stand
@@ -1013,6 +1002,7 @@ moe_decode_experts_kernel(const __grid_constant__ CUtensorMap map_b, const __gri
         Drain<kFp8, kTp> d{p, st, tmem + (uint32_t(quarter * 32) << 16), warp - 4, lane, quarter * 32 + lane, warp >= 12 ? 16 : 0};
         d.run();
     }
+    ptx::settle_after_abort(&st.abort_flag);
     __syncthreads();
     if (threadIdx.x == 0 && st.abort_flag != 0 && *const_cast<volatile int*>(p.status) == 0) *p.status = kStatusRing;
     if (warp == 1) {

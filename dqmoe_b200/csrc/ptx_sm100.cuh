@@ -103,6 +103,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, v
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
 }
 
+// For every thread, behind its role and before the block's last barrier: where a wait gave up, nobody may leave while copies or MMAs are under
+// way, of whichever role (one that had nothing to wait for any more may have returned long before, with its copies in flight). They take
+// microseconds; 4 million cycles are two milliseconds.
+__device__ __forceinline__ void settle_after_abort(const volatile int* abort_flag) {
+    if (*abort_flag == 0) return;
+    for (const long long t0 = clock64(); clock64() - t0 < 4000000;) __nanosleep(1000);
+}
+
 // ---------------------------------------------------------------- small asynchronous copies
 
 // 4-byte global -> shared copy (non-bulk), completion tracked per thread.

@@ -206,3 +206,19 @@ def test_lora_reads_what_shrink_writes_past_l1():
     for m in re.finditer(r"p\.(z|z_scale|ids) ?[+\[]", project):
         before = project[max(0, m.start() - 20):m.start()]
         assert "[" not in m.group(0) and re.search(r"(load16|load_f32|ld_relaxed_gpu)\($", before), project[m.start() - 60:m.end() + 20]
+
+
+def test_nobody_leaves_while_copies_or_mmas_are_under_way():
+    """A role that gives up may find the others gone: the thread that issues the copies returns with the last of them in flight where nothing is
+    left to wait for, and the MMA thread with its MMAs. So behind the roles every thread looks at the flag, before the barrier that frees
+    the block's TMEM, and in a cluster before the one behind which the other block's signals find nobody."""
+    for name, kernels in (("moe_decode.cu", ["moe_decode_experts_kernel("]), ("lora.cu", ["lora_shrink_tiles_kernel(", "lora_project_kernel("])):
+        text = source(name)
+        for kernel in kernels:
+            body = braces(text, text.index(kernel))
+            assert body.count("settle_after_abort(&st.abort_flag);") == 1, kernel
+            at = body.index("settle_after_abort(")
+            depth = body[:at].count("{") - body[:at].count("}")
+            assert depth == 1, kernel  # no branch keeps a thread from it
+            assert "mbar_wait" not in body[at:] and "tmem_dealloc" not in body[:at] and body.index("__syncthreads()", at) < body.index("tmem_dealloc", at), kernel
+            assert body.rindex("warp == ", 0, at) > 0
