@@ -24,6 +24,7 @@ SIGNATURES = {
     "dqmoe_last_error": (ctypes.c_char_p, []),
     "dqmoe_abi_version": (_c_int, []),
     "dqmoe_device_status": (_c_int, [ctypes.POINTER(_c_int)]),
+    "dqmoe_set_wait_limit": (_c_int, [_c_i64]),
     "dqmoe_moe_workspace_bytes": (_c_size, [_c_int] * 6),
     "dqmoe_moe_forward": (_c_int, [_ptr] * 9 + [_c_size] + [_c_int] * 7 + [_ptr]),
     "dqmoe_moe_workspace_ptr": (_ptr, [_ptr] + [_c_int] * 7),

@@ -1,6 +1,7 @@
 // Error reporting, device status word and device properties for the C ABI.
 #include "common.cuh"
 
+#include <atomic>
 #include <mutex>
 #include <vector>
 
@@ -38,6 +39,8 @@ std::mutex g_mu;
 int* g_status_host[kMaxDevices] = {nullptr};
 int* g_status_dev[kMaxDevices] = {nullptr};
 int g_sm_count[kMaxDevices] = {0};
+constexpr long long kDefaultWaitLimit = 1000000000LL;  // ~0.5 s
+std::atomic<long long> g_wait_limit{kDefaultWaitLimit};
 }  // namespace
 
 static bool ensure_status(int dev) {
@@ -86,6 +89,8 @@ int sm_count() {
     return g_sm_count[dev];
 }
 
+long long wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
+
 }  // namespace dq
 
 extern "C" {
@@ -101,6 +106,12 @@ int dqmoe_device_status(int* code) {
     DQ_CUDA(cudaDeviceSynchronize());
     *code = *h;
     *h = 0;
+    return DQMOE_OK;
+}
+
+int dqmoe_set_wait_limit(int64_t cycles) {
+    DQ_CHECK(cycles >= 0);
+    dq::g_wait_limit.store(cycles == 0 ? dq::kDefaultWaitLimit : static_cast<long long>(cycles), std::memory_order_relaxed);
     return DQMOE_OK;
 }
 

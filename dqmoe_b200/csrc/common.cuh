@@ -59,6 +59,9 @@ volatile int* host_status_word();
 
 int sm_count();
 
+// Clock cycles that a wait inside moe_decode and lora_linear may take before it gives up (dqmoe_set_wait_limit).
+long long wait_limit();
+
 namespace decode {
 constexpr int kAmaxParts = 4096;  // floats the layer workspace holds for the per-block amax values of the decode path's fc1
 }

@@ -42,7 +42,6 @@ constexpr int kKElems = 64;
 constexpr int kRows = 128;                      // rows of W, or of stacked A, of an MMA
 constexpr int kABytes = kRows * kKBytes;        // 16 KiB
 constexpr int kMaxRank = 128;
-constexpr long long kWaitLimit = 1000000000LL;  // clock cycles before a wait gives up (~0.5 s)
 constexpr int kStatusShrink = 311, kStatusProject = 312;
 
 // ---------------------------------------------------------------- shrink
@@ -78,6 +77,7 @@ struct ShrinkParams {
     int stages;             // stages of the ring,
     int slots;              // clusters that share a tile's groups of adapters
     int* status;
+    long long wait_limit;   // clock cycles before a wait gives up
 };
 
 // A row's z in the operands' type, by a warp whose lanes hold four values each (lane * 4 < R).
@@ -259,7 +259,7 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                 const int n = min(cap, st.distinct - g * cap);
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = it % p.stages;
-                    if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+                    if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / p.stages) & 1) ^ 1, &st.abort_flag, p.wait_limit))) break;
                     uint8_t* a = ring + s * stage + kShrinkXBytes;
                     ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(n * p.R + kShrinkTok) * kKBytes);
                     ptx::tma_load_2d(ring + s * stage, &map_x, kb * kKElems, tile * kShrinkTok, &st.full[s]);
@@ -275,10 +275,10 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             int it = 0, acc = 0;
             bool ok = true;
             for (int g = slot; ok && g < groups; g += p.slots, ++acc) {
-                if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+                if (!ptx::mbar_wait(&st.tmem_empty[acc & 1], ((acc >> 1) & 1) ^ 1, &st.abort_flag, p.wait_limit)) break;
                 for (int kb = kb0; kb < kb1; ++kb, ++it) {
                     const int s = it % p.stages;
-                    if (!(ok = ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit))) break;
+                    if (!(ok = ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, p.wait_limit))) break;
                     ptx::tc_fence_after();
                     const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kShrinkXBytes));
                     const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
@@ -299,7 +299,7 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
         const int row = (warp - 4) * 32 + lane, mine = row / p.R, r = row - mine * p.R;
         int acc = 0;
         for (int g = slot; g < groups; g += p.slots, ++acc) {
-            if (!ptx::mbar_wait_warp(&st.tmem_full[acc & 1], (acc >> 1) & 1, &st.abort_flag, kWaitLimit)) break;
+            if (!ptx::mbar_wait_warp(&st.tmem_full[acc & 1], (acc >> 1) & 1, &st.abort_flag, p.wait_limit)) break;
             ptx::tc_fence_after();
             const int rows = min(kShrinkTok, p.T - tile * kShrinkTok);
 #pragma unroll 1
@@ -381,6 +381,7 @@ struct Params {
     int* counters;            // parts seen of each split tile, on pairs of each half of it
     float* part;              // [block] sums of a part of a tile, four rows of x together: [tok / 4][128][4]
     int* status;
+    long long wait_limit;     // clock cycles before a wait gives up
 };
 
 // Products of a part of a tile. Direct: adapter, first chunk | chunks << 8, all of whose rows have it. Mixed, by the half of the epilogue that has
@@ -506,7 +507,7 @@ struct Epilogue {
     __device__ __forceinline__ bool meet() {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&st.meet);
-        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
+        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, p.wait_limit);
     }
 
     __device__ __forceinline__ void store(float (&v)[kChunk], int t0, int n) {
@@ -556,7 +557,7 @@ struct Epilogue {
             const uint32_t entry = l.mixed[half][e].y, rows = entry >> 16;
             if (int(entry & 0xff) != chunk) break;
             const int slot = b_it % p.slots;
-            if (!ptx::mbar_wait_warp(&st.b_full[half][slot], (b_it / p.slots) & 1, &st.abort_flag, kWaitLimit)) return -1;
+            if (!ptx::mbar_wait_warp(&st.b_full[half][slot], (b_it / p.slots) & 1, &st.abort_flag, p.wait_limit)) return -1;
             const uint8_t* from = b_ring + (half * p.slots + slot) * slot_bytes + ((row - lane + g) * p.R + k_lane) * 2;
             float d[kChunk];
 #pragma unroll
@@ -640,7 +641,7 @@ struct Epilogue {
         for (int acc = 0; pieces.next(&q); ++acc) {
             const int tt = q.tile / p.n_tiles, n = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows + row, t0 = tt * p.tok;
             const int buf = acc & 1, parity = (acc >> 1) & 1;
-            if (!ptx::mbar_wait_warp(&st.list_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
+            if (!ptx::mbar_wait_warp(&st.list_full[buf], parity, &st.abort_flag, p.wait_limit)) return;
             const List& l = st.list[buf];
             // columns in use; the two halves of the epilogue take chunks in turn
             const int cols = min(p.tok, p.T - t0), n0 = n - lane;
@@ -652,7 +653,7 @@ struct Epilogue {
 #pragma unroll 1
             for (int pass = ahead ? 0 : 1; pass < 2; ++pass) {
                 if (pass == 1) {
-                    if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, kWaitLimit)) return;
+                    if (!ptx::mbar_wait_warp(&st.tmem_full[buf], parity, &st.abort_flag, p.wait_limit)) return;
                     ptx::tc_fence_after();
                 }
 #pragma unroll 1
@@ -778,7 +779,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             Piece q, held;
             int it = 0;
             bool ok = true, waited = false;
-            auto next_stage = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, kWaitLimit); };
+            auto next_stage = [&]() { return ptx::mbar_wait(&st.empty[it % p.stages], ((it / p.stages) & 1) ^ 1, &st.abort_flag, p.wait_limit); };
             // the barrier of stage s, which expects `bytes` from this block, and on pairs as many from the other one
             auto expect = [&](int s, uint32_t bytes) {
                 if (rank == 0) ptx::mbar_arrive_expect_tx(&st.full[s], kPair ? 2 * bytes : bytes);
@@ -797,7 +798,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             };
             auto products = [&](const Piece& q, int n) {  // z B^T
                 const int tt = q.tile / p.n_tiles, n0 = ((q.tile - tt * p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows, t0 = tt * p.tok;
-                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit)) return false;
+                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, p.wait_limit)) return false;
                 const List& l = st.list[n & 1];
                 if (l.direct0 < l.direct1 && !waited) {
                     pdl_wait();  // shrink: z
@@ -845,7 +846,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
             auto block = [&](uint32_t d, int cols, int steps, bool more) {
                 const uint32_t idesc = ptx::make_idesc(kHalf ? 0 : 1, kPair ? 2 * kRows : kRows, uint32_t(cols));
                 const int s = it % p.stages;
-                if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, kWaitLimit)) return false;
+                if (!ptx::mbar_wait(&st.full[s], (it / p.stages) & 1, &st.abort_flag, p.wait_limit)) return false;
                 ptx::tc_fence_after();
                 const uint64_t da = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage));
                 const uint64_t db = ptx::smem_desc_sw128(ptx::smem_u32(ring + s * stage + kABytes));
@@ -860,14 +861,14 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                 return true;
             };
             auto sums = [&](const Piece& q, int n) {
-                if (!ptx::mbar_wait(&st.tmem_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return false;
+                if (!ptx::mbar_wait(&st.tmem_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, p.wait_limit)) return false;
                 ptx::tc_fence_after();
                 for (int kb = q.kb0; kb < q.kb1; ++kb)
                     if (!block(tmem + (n & 1) * p.tok, p.tok, 4, kb > q.kb0)) return false;
                 return true;
             };
             auto products = [&](int n) {
-                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit)) return false;
+                if (!ptx::mbar_wait(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, p.wait_limit)) return false;
                 const List& l = st.list[n & 1];
                 for (int e = l.direct0; e < l.direct1; ++e)
                     for (int r0 = 0; r0 < p.R; r0 += kKElems)
@@ -888,7 +889,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         Pieces pieces(p, group);
         Piece q;
         for (int n = 0; pieces.next(&q); ++n) {
-            if (!ptx::mbar_wait_warp(&st.list_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, kWaitLimit)) break;
+            if (!ptx::mbar_wait_warp(&st.list_empty[n & 1], ((n >> 1) & 1) ^ 1, &st.abort_flag, p.wait_limit)) break;
             List& l = st.list[n & 1];
             const int tt = q.tile / p.n_tiles, t0 = tt * p.tok, rows = min(p.tok, p.T - t0);
             int ids[kMaxTok / 32];
@@ -933,7 +934,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
         int before = 0, uses = 0;  // products of this half in earlier pieces; of this slot
         bool ok = true;
         for (int n = 0; ok && pieces.next(&q); ++n) {
-            if (!(ok = ptx::mbar_wait_warp(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, kWaitLimit))) break;
+            if (!(ok = ptx::mbar_wait_warp(&st.list_full[n & 1], (n >> 1) & 1, &st.abort_flag, p.wait_limit))) break;
             const List& l = st.list[n & 1];
             const int n0 = ((q.tile % p.n_tiles) * (kPair ? 2 : 1) + rank) * kRows;
             const uint32_t bytes = uint32_t(max(0, min(kRows, p.N - n0)) * p.R) * 2u;
@@ -947,7 +948,7 @@ lora_project_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     ++uses;
                     e += p.slots;
                 }
-                if (clock64() - begin > kWaitLimit) *const_cast<volatile int*>(&st.abort_flag) = 1;
+                if (clock64() - begin > p.wait_limit) *const_cast<volatile int*>(&st.abort_flag) = 1;
                 if (__any_sync(0xffffffffu, *const_cast<volatile int*>(&st.abort_flag) != 0)) {
                     ok = false;
                     break;
@@ -1197,7 +1198,7 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     sp.z = reinterpret_cast<uint16_t*>(ws + Y.z), sp.z_scale = reinterpret_cast<float*>(ws + Y.z_scale);
     sp.counters = reinterpret_cast<int*>(ws + Y.counters);
     sp.n_counters = (p.tiles - p.whole) << (pair ? 1 : 0);
-    sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status;
+    sp.T = T, sp.K = K, sp.L = L, sp.R = R, sp.half = half, sp.status = status, sp.wait_limit = wait_limit();
 
     CUtensorMap xp, wm, zm, bm;
     DQ_RC(lora::make_map_2d(&xp, x, half, T, K, ldx, pair ? p.tok / 2 : p.tok));
@@ -1209,7 +1210,7 @@ int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lor
     DQ_RC(lora::launch_shrink(sp, x, stream));
     p.ids = ids, p.lora_b = static_cast<const uint16_t*>(lora_b), p.z = sp.z, p.z_scale = half ? sp.z_scale : nullptr, p.bias = bias;
     p.y = static_cast<uint16_t*>(y), p.ldy = ldy, p.L = L;
-    p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status;
+    p.counters = sp.counters, p.part = reinterpret_cast<float*>(ws + Y.part), p.status = status, p.wait_limit = sp.wait_limit;
     const int split = (p.tiles - p.whole) * p.parts, busy = p.whole < p.groups ? (p.whole > split ? p.whole : split) : p.groups;
     const size_t smem = 1024 + size_t(p.stages) * (lora::kABytes + (pair ? p.tok / 2 : p.tok) * lora::kKBytes) + size_t(2) * p.slots * lora::kRows * R * 2 + sizeof(lora::Tail);
     if (half)

@@ -63,7 +63,6 @@ constexpr int kGroups = (kMaxParts + kGroup - 1) / kGroup;
 constexpr int kMaxStages = 6;
 constexpr int kScaleBytes = 1024;             // room behind a stage's second operand for its scales
 constexpr int kClaims = 4, kJobs = 4;
-constexpr long long kWaitLimit = 1000000000LL;  // clock cycles before a wait gives up (~0.5 s)
 constexpr int kStatusRing = 301, kStatusPhase = 302;
 constexpr int kSplit = 8;                     // blocks of a route cluster: slices of H
 constexpr int kRouteThreads = 256;
@@ -100,6 +99,7 @@ struct Params {
     float* part2;             // [tile][part]
     float* group2;            // [tile][group]
     int* status;
+    long long wait_limit;     // clock cycles before a wait gives up
 };
 
 // byte `byte` of row `row` of an operand tile with 128-byte rows, as the 128-byte swizzle places it
@@ -380,8 +380,8 @@ __device__ __forceinline__ float* place1(const Params& p, const Tail& st, const 
 template <bool kWarp>
 __device__ __forceinline__ Piece next_piece(const Params& p, Tail& st, int it, int lane, int* code = nullptr) {
     const int slot = it % kClaims, parity = (it / kClaims) & 1;
-    const bool ok = kWarp ? ptx::mbar_wait_warp(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit)
-                          : ptx::mbar_wait(&st.claim_full[slot], parity, &st.abort_flag, kWaitLimit);
+    const bool ok = kWarp ? ptx::mbar_wait_warp(&st.claim_full[slot], parity, &st.abort_flag, p.wait_limit)
+                          : ptx::mbar_wait(&st.claim_full[slot], parity, &st.abort_flag, p.wait_limit);
     if (!ok) return Piece{3, 0, 0, 0, 0};
     const int c = *const_cast<volatile int*>(&st.claim[slot]);
     if constexpr (kWarp) __syncwarp();
@@ -414,14 +414,14 @@ __device__ __forceinline__ void load_weights(const Params& p, const CUtensorMap&
     for (int n = 0; ok; ++n) {
         const int slot = n % kClaims;
         const int next = claim < all_pieces(p, st) ? atomicAdd(&p.counters[0], 1) : claim;  // known by the time it is needed
-        if (!(ok = ptx::mbar_wait(&st.claim_empty[slot], ((n / kClaims) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+        if (!(ok = ptx::mbar_wait(&st.claim_empty[slot], ((n / kClaims) & 1) ^ 1, &st.abort_flag, p.wait_limit))) break;
         *const_cast<volatile int*>(&st.claim[slot]) = claim;
         ptx::mbar_arrive(&st.claim_full[slot]);
         const Piece q = piece_at(p, st, claim);
         if (q.phase == 2) break;
         for (int u = q.lo; u < q.hi; ++u, ++it) {
             const int s = it % S::kStages;
-            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, p.wait_limit))) break;
             uint8_t* a = ring + s * S::kStage;
             ptx::mbar_arrive_expect_tx(&st.full[s], kABytes);
             if (q.phase == 0) {
@@ -449,7 +449,7 @@ __device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* 
         if (q.phase >= 2) break;
         for (int u = q.lo; u < q.hi; ++u, ++it) {
             const int s = it % S::kStages;
-            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, kWaitLimit))) break;
+            if (!(ok = ptx::mbar_wait(&st.empty[s], ((it / S::kStages) & 1) ^ 1, &st.abort_flag, p.wait_limit))) break;
             uint8_t* b = ring + s * S::kStage + kABytes;
             if (q.phase == 0) {
                 ptx::mbar_arrive_expect_tx(&st.full[s], uint32_t(p.rec1));
@@ -461,7 +461,7 @@ __device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* 
                 const long long t0 = clock64();
                 while (streamk::ld_acquire_gpu(&p.counters[4 + j]) < p.tiles1) {
                     if (*const_cast<volatile int*>(&st.abort_flag) != 0) ok = false;
-                    if (clock64() - t0 > kWaitLimit) {
+                    if (clock64() - t0 > p.wait_limit) {
                         *const_cast<volatile int*>(&st.abort_flag) = 1;
                         *p.status = kStatusPhase;
                         ok = false;
@@ -493,8 +493,8 @@ __device__ __forceinline__ void multiply(const Params& p, Tail& st, uint8_t* rin
         bool fresh = true;  // the next unit begins an accumulator buffer
         for (int u = q.lo; u < q.hi; ++u, ++it) {
             const int slot = it % S::kStages, buf = buf_it % S::kBufs;
-            if (fresh && !ptx::mbar_wait_warp(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
-            if (!ptx::mbar_wait_warp(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, kWaitLimit)) return;
+            if (fresh && !ptx::mbar_wait_warp(&st.tmem_empty[buf], ((buf_it / S::kBufs) & 1) ^ 1, &st.abort_flag, p.wait_limit)) return;
+            if (!ptx::mbar_wait_warp(&st.full[slot], (it / S::kStages) & 1, &st.abort_flag, p.wait_limit)) return;
             ptx::tc_fence_after();
             const bool done = kFp8 || u + 1 == q.hi || (q.phase == 1 && (u + 1) % p.pairs2 == 0);
             if (ptx::elect_one()) {
@@ -574,7 +574,7 @@ struct Drain {
 
     __device__ __forceinline__ bool acquire() {
         const int buf = buf_it % S::kBufs;
-        if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (buf_it / S::kBufs) & 1, &st.abort_flag, kWaitLimit)) return false;
+        if (!ptx::mbar_wait_warp(&st.tmem_full[buf], (buf_it / S::kBufs) & 1, &st.abort_flag, p.wait_limit)) return false;
         ptx::tc_fence_after();
         return true;
     }
@@ -690,7 +690,7 @@ struct Drain {
             const Piece q = next_piece<true>(p, st, n, lane, &code);
             // the finishing warps are through with what used this note, and this place for a tile in one part, before
             const int slot = n % kJobs;
-            if (q.phase == 3 || !ptx::mbar_wait_warp(&st.job_empty[slot], ((n / kJobs) & 1) ^ 1, &st.abort_flag, kWaitLimit)) return;
+            if (q.phase == 3 || !ptx::mbar_wait_warp(&st.job_empty[slot], ((n / kJobs) & 1) ^ 1, &st.abort_flag, p.wait_limit)) return;
             if (q.phase == 0) {
                 if (!fc1(q, place1<S::kPart1>(p, st, q, slot))) return;
             } else if (q.phase == 1) {
@@ -710,7 +710,7 @@ __device__ __forceinline__ void count_pieces(const Params& p, Tail& st) {
     int passed = 0;
     for (int n = 0;; ++n) {
         const int slot = n % kJobs;
-        if (!ptx::mbar_wait(&st.job_full[slot], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
+        if (!ptx::mbar_wait(&st.job_full[slot], (n / kJobs) & 1, &st.abort_flag, p.wait_limit)) return;
         const int code = *const_cast<volatile int*>(&st.job[slot]);
         const Piece q = piece_at(p, st, code);
         bool last = true;
@@ -747,7 +747,7 @@ struct Finish {
     __device__ __forceinline__ bool meet() {
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&st.meet);
-        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, kWaitLimit);
+        return ptx::mbar_wait_warp(&st.meet, meetings++ & 1, &st.abort_flag, p.wait_limit);
     }
 
     // Weight of token t for the expert e (routed ids only), by all lanes together.
@@ -874,7 +874,7 @@ struct Finish {
 
     __device__ __forceinline__ void run() {
         for (int n = 0;; ++n) {
-            if (!ptx::mbar_wait_warp(&st.last_full[n % kJobs], (n / kJobs) & 1, &st.abort_flag, kWaitLimit)) return;
+            if (!ptx::mbar_wait_warp(&st.last_full[n % kJobs], (n / kJobs) & 1, &st.abort_flag, p.wait_limit)) return;
             const int note = *const_cast<volatile int*>(&st.last_job[n % kJobs]), slot = note % kJobs;
             const Piece q = piece_at(p, st, note / kJobs);
             if (q.phase == 2) return;
@@ -1159,6 +1159,7 @@ int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, 
     p.group2 = reinterpret_cast<float*>(ws + L.group2);
     p.status = device_status_word();
     if (p.status == nullptr) return DQMOE_ERR_CUDA;
+    p.wait_limit = wait_limit();
     const int esz = fp8 ? 1 : 2;
     CUtensorMap map_b, map_b1;
     DQ_RC(gemm::make_map(&map_b, b, esz, uint64_t(E + n_shared) * 2 * I, uint64_t(H), moe_decode::kRows));

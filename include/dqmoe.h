@@ -82,6 +82,10 @@ int dqmoe_abi_version(void);
  * process (csrc/util.h:61-80).
  */
 int dqmoe_device_status(int* code);
+/* Clock cycles that a wait inside dqmoe_moe_decode and dqmoe_lora_linear may take before it gives up (process-wide, applies to launches made
+ * afterwards, and in a captured graph as it was at the capture); 0 restores the default of about half a second. A call that gave up leaves its output
+ * unspecified and the next one unharmed. */
+int dqmoe_set_wait_limit(int64_t cycles);
 
 /* ------------------------------------------------------------------ layer */
 
@@ -499,9 +503,9 @@ int dqmoe_grouped_gemm_nvfp4(const void* a, const uint8_t* a_sf, const float* a_
  * A row whose id is outside [0, L) has no adapter. Adapters of a lower rank are padded with zeros to R, a multiple of 8 up to 128; K is a
  * multiple of 8; x, w, lora_a, lora_b are aligned to 16 bytes. The ids may come in any order; rows of one request that stand together
  * are faster. Sums are fp32, scale[a] * (x A_a^T) and the result are rounded to the operands' type (fp16: with a power of two per row
- * where the row's largest value of the former is above 2^15 or below R 2^-14, so that rows of any magnitude keep the type's precision). No row's result depends on another row's adapter. Any T from 0 on. The status codes of
- * dqmoe_device_status are 311 and 312. A call has its workspace for itself until it is over; y and the workspace overlap no operand. No
- * counterpart in the reference.
+ * where the row's largest value of the former is above 2^15 or below R 2^-14, so that rows of any magnitude keep the type's precision). No
+ * row's result depends on another row's adapter. Any T from 0 on. The status codes of dqmoe_device_status are 311 and 312. A call has its
+ * workspace for itself until it is over; y and the workspace overlap no operand. No counterpart in the reference.
  */
 size_t dqmoe_lora_linear_workspace_bytes(int T, int N, int K, int L, int R);
 int dqmoe_lora_linear(const void* x, int64_t ldx, const void* w, const void* lora_a, const void* lora_b, const int32_t* ids,

@@ -53,3 +53,9 @@ def test_no_cpu_path():
     x = torch.zeros(2, 256, dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.moe_decode(x, x, x, None, x, None, 1)
+
+
+def test_wait_limit_is_checked():
+    lib = _lib.load()
+    assert lib.dqmoe_set_wait_limit(-1) == 1 and "cycles >= 0" in lib.dqmoe_last_error().decode()
+    assert lib.dqmoe_set_wait_limit(5) == 0 and lib.dqmoe_set_wait_limit(0) == 0
