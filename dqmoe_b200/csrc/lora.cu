@@ -311,7 +311,7 @@ lora_shrink_tiles_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
                     place[i] = four.x, place[i + 1] = four.y, place[i + 2] = four.z, place[i + 3] = four.w;
                 }
                 float v[16];
-                ptx::tmem_read<16>(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
+                ptx::tmem_read(tmem + (uint32_t((warp - 4) * 32) << 16) + (acc & 1) * kShrinkTok + c, v);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (mine < cap && place[i] == g * cap + mine) part[(c + i) * p.R + r] = v[i];
@@ -685,7 +685,7 @@ struct Epilogue {
                         }
                         continue;
                     }
-                    ptx::tmem_read<kChunk>(sums + c * kChunk, v);
+                    ptx::tmem_read(sums + c * kChunk, v);
                     if (q.of == 1) {
                         store(v, t0 + c * kChunk, n);
                         continue;

@@ -89,7 +89,7 @@ struct Params {
     int max_hit;              // experts hit at most
     int n_counters;
     size_t rec1, rec2;        // bytes of a unit's second operand with its scales
-    int* counters;            // claims; 3 unused; finished fc1 tiles of each expert; parts seen of each fc1 tile, of each group of parts
+    int* counters;            // claims; finished fc1 tiles of each expert; parts seen of each fc1 tile, of each group of parts
                               // of an fc2 tile, groups seen of each fc2 tile
     float* logits;            // [T, E]
     uint8_t* xq;              // [kb1] records: [fc1_cols][128 B] swizzled, scales [token_rows]
@@ -459,7 +459,7 @@ __device__ __forceinline__ void load_tokens(const Params& p, Tail& st, uint8_t* 
             const int j = u / p.pairs2;
             if (j != ready) {
                 const long long t0 = clock64();
-                while (streamk::ld_acquire_gpu(&p.counters[4 + j]) < p.tiles1) {
+                while (streamk::ld_acquire_gpu(&p.counters[1 + j]) < p.tiles1) {
                     if (*const_cast<volatile int*>(&st.abort_flag) != 0) ok = false;
                     if (clock64() - t0 > p.wait_limit) {
                         *const_cast<volatile int*>(&st.abort_flag) = 1;
@@ -715,10 +715,10 @@ __device__ __forceinline__ void count_pieces(const Params& p, Tail& st) {
         const Piece q = piece_at(p, st, code);
         bool last = true;
         if (q.phase == 0 && q.part >= 0 && st.split1 > 1) {
-            last = streamk::atomic_add_acq_rel_gpu(&p.counters[4 + p.max_hit + q.tile], 1) == st.split1 - 1;
+            last = streamk::atomic_add_acq_rel_gpu(&p.counters[1 + p.max_hit + q.tile], 1) == st.split1 - 1;
         } else if (q.phase == 1) {
             const int group = q.part / kGroup, in_group = min(kGroup, st.parts2 - group * kGroup);
-            int* counters = p.counters + 4 + p.max_hit + p.max_hit * p.tiles1;
+            int* counters = p.counters + 1 + p.max_hit + p.max_hit * p.tiles1;
             if (in_group > 1) last = streamk::atomic_add_acq_rel_gpu(&counters[q.tile * kGroups + group], 1) == in_group - 1;
         }
         if (last) {  // at most kJobs of them are under way, each with its slot of `job`
@@ -834,7 +834,7 @@ struct Finish {
         }
         asm volatile("fence.proxy.async;" ::: "memory");  // to the bulk copies of other blocks
         if (!meet()) return false;
-        if (warp == 0 && lane == 0) streamk::red_add_release_gpu(&p.counters[4 + j], 1);
+        if (warp == 0 && lane == 0) streamk::red_add_release_gpu(&p.counters[1 + j], 1);
         return true;
     }
 
@@ -860,7 +860,7 @@ struct Finish {
         if (groups == 1) return true;
         if (!meet()) return false;
         if (warp == 0 && lane == 0)
-            st.last = streamk::atomic_add_acq_rel_gpu(p.counters + 4 + p.max_hit + p.max_hit * p.tiles1 + p.tiles2 * kGroups + q.tile, 1) == groups - 1;
+            st.last = streamk::atomic_add_acq_rel_gpu(p.counters + 1 + p.max_hit + p.max_hit * p.tiles1 + p.tiles2 * kGroups + q.tile, 1) == groups - 1;
         if (!meet()) return false;
         if (*const_cast<volatile int*>(&st.last) == 0) return true;  // read by all before they meet for the next job's
 #pragma unroll 1
@@ -1031,7 +1031,7 @@ static Layout plan(Params* p, bool fp8) {
     p->share = p->even < 1.0f ? 0.5f * p->even : 0.5f;  // of what is left, per part
     p->per_share = 1.0f / p->share;
     p->shrink_rate = -1.0f / log2f(1.0f - p->share);
-    p->n_counters = 4 + p->max_hit + p->max_hit * p->tiles1 + p->tiles2 * (kGroups + 1);
+    p->n_counters = 1 + p->max_hit + p->max_hit * p->tiles1 + p->tiles2 * (kGroups + 1);
     Layout L{};
     size_t off = 0;
     auto add = [&](size_t bytes) {

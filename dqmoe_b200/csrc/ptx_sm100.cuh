@@ -504,34 +504,17 @@ __device__ __forceinline__ void tmem_wait_ld2(uint32_t (&a)[32], uint32_t (&b)[3
                  : "memory");
 }
 
-// 32 lanes x kCount consecutive fp32 columns, as floats: thread i of the warp receives the columns of lane i. The loads and their wait are one
+// 32 lanes x 16 consecutive fp32 columns, as floats: thread i of the warp receives the columns of lane i. The loads and their wait are one
 // statement. The hardware writes the registers at some time until the wait: had the compiler them as results before it, it could move or
 // spill them, and give the registers to something else, while they are still to be written.
-template <int kCount>
-__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[kCount]) {
-    static_assert(kCount == 8 || kCount == 16 || kCount == 32, "");
-    if constexpr (kCount == 8)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
-                     "tcgen05.wait::ld.sync.aligned;"
-                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7])
-                     : "r"(taddr) : "memory");
-    else if constexpr (kCount == 16)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-                     "tcgen05.wait::ld.sync.aligned;"
-                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
-                       "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15])
-                     : "r"(taddr) : "memory");
-    else if constexpr (kCount == 32)
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-                     "%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
-                     "%31}, [%32];\n\t"
-                     "tcgen05.wait::ld.sync.aligned;"
-                     : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
-                       "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15]), "=&f"(r[16]),
-                       "=&f"(r[17]), "=&f"(r[18]), "=&f"(r[19]), "=&f"(r[20]), "=&f"(r[21]), "=&f"(r[22]), "=&f"(r[23]), "=&f"(r[24]),
-                       "=&f"(r[25]), "=&f"(r[26]), "=&f"(r[27]), "=&f"(r[28]), "=&f"(r[29]), "=&f"(r[30]), "=&f"(r[31])
-                     : "r"(taddr) : "memory");
+__device__ __forceinline__ void tmem_read(uint32_t taddr, float (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=&f"(r[0]), "=&f"(r[1]), "=&f"(r[2]), "=&f"(r[3]), "=&f"(r[4]), "=&f"(r[5]), "=&f"(r[6]), "=&f"(r[7]), "=&f"(r[8]),
+                   "=&f"(r[9]), "=&f"(r[10]), "=&f"(r[11]), "=&f"(r[12]), "=&f"(r[13]), "=&f"(r[14]), "=&f"(r[15])
+                 : "r"(taddr) : "memory");
 }
+// The same of two places.
 template <int kCount>
 __device__ __forceinline__ void tmem_read2(uint32_t taddr_a, uint32_t taddr_b, float (&a)[kCount], float (&b)[kCount]) {
     static_assert(kCount == 8 || kCount == 16, "");
