@@ -63,6 +63,17 @@ def _call(index: int, fn, *args) -> None:
         _lib.check(rc)
 
 
+def _new_workspace(like: torch.Tensor, workspace_bytes, *sizes) -> torch.Tensor:
+    """What workspace_bytes(*sizes) asks for with the device of `like` current, whose SMs it counts; 256 bytes where it refuses, as the call will."""
+    index = like.device.index
+    if torch._C._cuda_getDevice() == index:
+        nbytes = workspace_bytes(*sizes)
+    else:
+        with torch.cuda.device(index):
+            nbytes = workspace_bytes(*sizes)
+    return like.new_empty(nbytes or 256, dtype=torch.uint8)
+
+
 def device_status() -> int:
     """Synchronise the current device and return (then clear) the kernels' sticky status word."""
     code = ctypes.c_int(0)
@@ -198,7 +209,7 @@ def moe_block(x: torch.Tensor, logits: torch.Tensor, b, b_scale, b1, b1_scale, k
 
 
 def moe_decode_workspace_bytes(T: int, H: int, I: int, E: int, k: int, n_shared: int = 0, quant_mode: int = QUANT_FP8_BLOCK) -> int:
-    """Bytes of workspace for moe_decode; 0 where the sizes are not ones it takes."""
+    """Bytes of workspace for moe_decode on the current device; 0 where the sizes are not ones it takes."""
     return int(_lib.load().dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, int(quant_mode)))
 
 
@@ -215,12 +226,10 @@ def moe_decode(x: torch.Tensor, w_router: torch.Tensor, b: torch.Tensor, b_scale
     T, H, E, I = _moe_decode_sizes(x, w_router, b, b_scale, b1, b1_scale, quant_mode, n_shared, dev)
     lib = _lib.load()
     if workspace is None:
-        nbytes = max(lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode), 256)
-        workspace = x.new_empty(nbytes, dtype=torch.uint8)
+        workspace = _new_workspace(x, lib.dqmoe_moe_decode_workspace_bytes, T, H, I, E, k, n_shared, quant_mode)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
-    else:
-        nbytes = workspace.numel() * workspace.element_size()
+    nbytes = workspace.numel() * workspace.element_size()
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != (T, H) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous():
@@ -604,7 +613,7 @@ def requant_from_amax(act: torch.Tensor, amax: torch.Tensor, per_row: bool, n_ro
 # ---------------------------------------------------------------------- projections with adapters
 
 def lora_linear_workspace_bytes(T: int, N: int, K: int, L: int, R: int) -> int:
-    """Bytes of workspace for lora_linear; 0 where the sizes are not ones it takes."""
+    """Bytes of workspace for lora_linear on the current device; 0 where the sizes are not ones it takes."""
     return int(_lib.load().dqmoe_lora_linear_workspace_bytes(T, N, K, L, R))
 
 
@@ -626,12 +635,10 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         ldy = N if out.is_contiguous() else out.stride(0)
     lib = _lib.load()
     if workspace is None:
-        nbytes = max(lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R), 256)
-        workspace = x.new_empty(nbytes, dtype=torch.uint8)
+        workspace = _new_workspace(x, lib.dqmoe_lora_linear_workspace_bytes, T, N, K, L, R)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
-    else:
-        nbytes = workspace.numel() * workspace.element_size()
+    nbytes = workspace.numel() * workspace.element_size()
     _call(dev.index, lib.dqmoe_lora_linear, x.data_ptr(), K if x.is_contiguous() else x.stride(0), w.data_ptr(), lora_a.data_ptr(),
           lora_b.data_ptr(), ids.data_ptr(), None if scale is None else scale.data_ptr(), None if bias is None else bias.data_ptr(),
           out.data_ptr(), ldy, workspace.data_ptr(), nbytes, T, N, K, L, R, DT_HALF if dtype is torch.float16 else DT_BF16)
