@@ -51,27 +51,10 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _call(index: int, fn, *args) -> None:
-    """fn(*args, current stream) with device `index` current. Entering torch.cuda.device and building a Stream object cost 4 us of a call that
-    takes the GPU 10, so neither is done where the device is current already."""
-    if torch._C._cuda_getDevice() == index:  # CUDA is up: the operands are there
-        rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
-    if rc != 0:
-        _lib.check(rc)
-
-
-def _new_workspace(like: torch.Tensor, workspace_bytes, *sizes) -> torch.Tensor:
-    """What workspace_bytes(*sizes) asks for with the device of `like` current, whose SMs it counts; 256 bytes where it refuses, as the call will."""
-    index = like.device.index
-    if torch._C._cuda_getDevice() == index:
-        nbytes = workspace_bytes(*sizes)
-    else:
-        with torch.cuda.device(index):
-            nbytes = workspace_bytes(*sizes)
-    return like.new_empty(nbytes or 256, dtype=torch.uint8)
+def _elsewhere(x: torch.Tensor) -> bool:
+    """Whether x is on another GPU than the current one. Entering torch.cuda.device and building a Stream object cost 4 us of a call that takes the
+    GPU 10, so the calls below enter it only then, and take the stream's address."""
+    return x.is_cuda and torch._C._cuda_getDevice() != x.device.index
 
 
 def device_status() -> int:
@@ -221,23 +204,30 @@ def moe_decode(x: torch.Tensor, w_router: torch.Tensor, b: torch.Tensor, b_scale
     x [T, H] bf16, w_router [E, H] bf16 or fp32, experts' weights bf16 (quant_mode 0) or e4m3 with that mode's scales
     (256 / 512 / 1024). The activations are not quantised. The last n_shared experts of b / b1 are shared ones that every token
     passes through with weight 1. Returns out [T, H] bf16."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return moe_decode(x, w_router, b, b_scale, b1, b1_scale, k, scoring, quant_mode, n_shared, workspace, out)
     quant_mode = int(quant_mode)
     dev, mode = x.device, _SCORES[scoring]
     T, H, E, I = _moe_decode_sizes(x, w_router, b, b_scale, b1, b1_scale, quant_mode, n_shared, dev)
     lib = _lib.load()
     if workspace is None:
-        workspace = _new_workspace(x, lib.dqmoe_moe_decode_workspace_bytes, T, H, I, E, k, n_shared, quant_mode)
+        nbytes = lib.dqmoe_moe_decode_workspace_bytes(T, H, I, E, k, n_shared, quant_mode) or 256  # 0: the call will refuse
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
-    nbytes = workspace.numel() * workspace.element_size()
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != (T, H) or out.dtype != torch.bfloat16 or out.device != dev or not out.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: out is contiguous bf16 [T, H] on x's device")
     fp8 = quant_mode != QUANT_NONE
-    _call(dev.index, lib.dqmoe_moe_decode, x.data_ptr(), w_router.data_ptr(), DT_FLOAT if w_router.dtype is torch.float32 else DT_BF16,
-          b.data_ptr(), b_scale.data_ptr() if fp8 else None, b1.data_ptr(), b1_scale.data_ptr() if fp8 else None, out.data_ptr(),
-          workspace.data_ptr(), nbytes, T, H, I, E, k, n_shared, mode, quant_mode)
+    rc = lib.dqmoe_moe_decode(x.data_ptr(), w_router.data_ptr(), DT_FLOAT if w_router.dtype is torch.float32 else DT_BF16, b.data_ptr(),
+                              b_scale.data_ptr() if fp8 else None, b1.data_ptr(), b1_scale.data_ptr() if fp8 else None, out.data_ptr(),
+                              workspace.data_ptr(), nbytes, T, H, I, E, k, n_shared, mode, quant_mode, _raw_stream(dev.index))
+    if rc != 0:
+        _lib.check(rc)
     return out
 
 
@@ -624,6 +614,9 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
 
     x [T, K], w [N, K], lora_a [L, R, K], lora_b [L, N, R], all bf16 or all fp16; ids int32 [T] (outside [0, L): no adapter), scale fp32
     [L], bias fp32 [N]. x and out may have rows that stand apart (columns next to each other). Returns y [T, N]."""
+    if _elsewhere(x):
+        with torch.cuda.device(x.device):
+            return lora_linear(x, w, lora_a, lora_b, ids, scale, bias, out, workspace)
     dev, dtype = x.device, x.dtype
     T, K, N, L, R = _lora_sizes(x, w, lora_a, lora_b, ids, scale, bias, dev)
     if out is None:
@@ -635,13 +628,18 @@ def lora_linear(x: torch.Tensor, w: torch.Tensor, lora_a: torch.Tensor, lora_b: 
         ldy = N if out.is_contiguous() else out.stride(0)
     lib = _lib.load()
     if workspace is None:
-        workspace = _new_workspace(x, lib.dqmoe_lora_linear_workspace_bytes, T, N, K, L, R)
+        nbytes = lib.dqmoe_lora_linear_workspace_bytes(T, N, K, L, R) or 256  # 0: the call will refuse
+        workspace = x.new_empty(nbytes, dtype=torch.uint8)
     elif workspace.device != dev or not workspace.is_contiguous():
         raise RuntimeError("[ASSERT FAILED] ops.py  Condition: workspace is contiguous and on x's device")
-    nbytes = workspace.numel() * workspace.element_size()
-    _call(dev.index, lib.dqmoe_lora_linear, x.data_ptr(), K if x.is_contiguous() else x.stride(0), w.data_ptr(), lora_a.data_ptr(),
-          lora_b.data_ptr(), ids.data_ptr(), None if scale is None else scale.data_ptr(), None if bias is None else bias.data_ptr(),
-          out.data_ptr(), ldy, workspace.data_ptr(), nbytes, T, N, K, L, R, DT_HALF if dtype is torch.float16 else DT_BF16)
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    rc = lib.dqmoe_lora_linear(x.data_ptr(), K if x.is_contiguous() else x.stride(0), w.data_ptr(), lora_a.data_ptr(), lora_b.data_ptr(),
+                               ids.data_ptr(), None if scale is None else scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                               ldy, workspace.data_ptr(), nbytes, T, N, K, L, R, DT_HALF if dtype is torch.float16 else DT_BF16,
+                               _raw_stream(dev.index))
+    if rc != 0:
+        _lib.check(rc)
     return out
 
 
