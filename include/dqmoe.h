@@ -216,12 +216,16 @@ int dqmoe_moe_block_shared(const void* x_bf16, const float* logits, const void* 
  *   weight * W2 (silu(G x) * (V x)); then n_shared shared experts, which stand behind the E routed ones in b / b1, with weight 1.
  * x [T, H] bf16, w_router [E, H] of router_type DQMOE_DT_BF16 or DQMOE_DT_FLOAT, b [E + n_shared, 2I, H], b1 [E + n_shared, H, I],
  * out [T, H] bf16. quant_mode NONE (bf16 weights) or FP8_TENSOR / _CHANNEL / _BLOCK (e4m3 weights with scales as listed at the top of
- * this file). The activations are not quantised in any mode, sums are fp32, and only the result is rounded to bf16: against
- * dqmoe_moe_block, which quantises both operands, the results differ by that quantisation. T <= 32, E + n_shared <= 1024, k <= 32, H and I
- * multiples of 16, operands aligned to 16 bytes. A token whose weights are not numbers (no logit above -inf) gets NaN, and so does
- * one whose x holds an infinity or a NaN in the FP8 modes; it changes no other token's result. The status codes of
- * dqmoe_device_status are 301 and 302. A call has its workspace for itself until it is over; out and the workspace overlap no operand. No
- * counterpart in the reference.
+ * this file). Sums are fp32, the result is rounded to bf16, and no mode quantises the activations to 8 bits: in the FP8 modes x is two e4m3 with a power of
+ * two per 128 values, exact down to 2^-13 of the largest of them and off by 2^-21 of that one at most below, and the intermediate is held likewise,
+ * within 2^-9 of each value down to there; with bf16 weights the intermediate is two bf16, within 2^-16. dqmoe_moe_block rounds the intermediate to
+ * bf16, and in the FP8 modes both operands to one e4m3: the results differ by that.
+ * T <= 32, E + n_shared <= 1024, k <= 32, H and I multiples of 16, operands aligned to 16 bytes. A token whose weights are not numbers (no logit above
+ * -inf) gets NaN, and in the FP8 modes so does one whose x holds an infinity or a NaN, or whose intermediate leaves fp32's range (with bf16
+ * weights infinities and NaN as fp32 has them); it changes no other token's result. The status codes of dqmoe_device_status are 301 and 302.
+ * A call has its workspace for itself until it is over; out and the workspace overlap no operand.
+ * When: for the same work (router, layer, weighted sum) up to 8 tokens take less time this way in all cases measured (down to half, and 1 % more in
+ * one), 16 tokens within 8 % of dqmoe_moe_block's time, and 32 take dqmoe_moe_block 6 to 15 % less. No counterpart in the reference.
  */
 size_t dqmoe_moe_decode_workspace_bytes(int T, int H, int I, int E, int k, int n_shared, int quant_mode);
 int dqmoe_moe_decode(const void* x_bf16, const void* w_router, int router_type, const void* b, const float* b_scale,
