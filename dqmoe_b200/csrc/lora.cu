@@ -25,8 +25,9 @@
 // project starts while shrink runs: it reads only x, W, ids and B until a tile's K is through. That is sound because shrink lets it start
 // behind its own wait for the kernels before, which wrote those. No counterpart in the reference.
 //
-// us per call: one row, 4096 x 4096, R 16 10.4 (3.2 TB/s; floor 5.2); 64 rows as above 20.0 (3.5 TB/s; floor 10.8); 333 as above 28.5 (floor 6.4);
-// 4096 rows of 6 requests, 4096 x 4096, R 32 113 (1.22 PFLOP/s); 8191 rows of 24, K 7168, N 4096, R 16 348 (1.39 PFLOP/s).
+// us per call over 0.6 GB of inputs: one row, 4096 x 4096, R 16 13.3 (2.5 TB/s; floor 5.2); 64 rows as above 22.9 (3.0 TB/s; floor 10.8); 333 as above 30.4
+// (floor 6.4); 4096 rows of 6 requests, 4096 x 4096, R 32 117 (1.2 PFLOP/s); 8191 rows of 24, K 7168, N 4096, R 16 357 (1.35 PFLOP/s). The figures further up
+// are of calls over one set of inputs, which L2 partly holds: as built 10.7, 20.2 and 28.7.
 #include <mutex>
 
 #include "common.cuh"

@@ -23,14 +23,14 @@
 // Sums are added in a fixed order whoever adds them: results do not depend on which block took which piece.
 //
 // us per call, first with one equal, static share of the units per SM, the sums and the activation on the warps that drain the accumulators and
-// fc2 behind all of fc1, then as it is (and the bandwidth at which that reads the weights of the experts hit):
-//   block FP8, H 1024, I 2048, 8 experts, k 2, 5 tokens                    44.8 / 22.7 (1.7 TB/s)
-//   bf16, H 4096, I 14336, 8 experts, k 2, 1 token                         124 / 122 (5.8)
-//   FP8 by tensor, H 4096, I 14336, 8 experts, k 2, 16 tokens              267 / 232 (6.0)
-//   block FP8, H 7168, I 2048, 32 experts, k 8, 1 shared, 8 tokens         224 / 213 (6.2)
-//   FP8 by channel, H 2048, I 768, 128 experts, k 8, 32 tokens             211 / 126 (4.2)
+// fc2 behind all of fc1, then as it is, both over one set of weights (and what a graph over 0.6 GB of them takes, at which bandwidth):
+//   block FP8, H 1024, I 2048, 8 experts, k 2, 5 tokens                    44.8 / 22.8 (26.0: 1.3 TB/s)
+//   bf16, H 4096, I 14336, 8 experts, k 2, 1 token                         124 / 120 (118: 6.0)
+//   FP8 by tensor, H 4096, I 14336, 8 experts, k 2, 16 tokens              267 / 229 (229: 6.1)
+//   block FP8, H 7168, I 2048, 32 experts, k 8, 1 shared, 8 tokens         224 / 204 (200: 6.3)
+//   FP8 by channel, H 2048, I 768, 128 experts, k 8, 32 tokens             211 / 123 (124: 4.2)
 // What is left above the weights' time is the chain of latencies before the first weight (route 3 us, top-k and plan 2 to 5), between fc1's last sum and
-// fc2's first MMA (8), and behind the last (5): nearly all of the smallest case.
+// fc2's first MMA (8), and behind the last (5): nearly all of the smallest case. At 32 tokens of many experts another 20 to 30 us are not accounted for.
 //
 // No counterpart in the reference, whose runner (csrc/moe_kernels.h:770-892) takes routed rows and five launches.
 #include <cmath>
