@@ -88,7 +88,7 @@ __device__ __forceinline__ void put_z(const ShrinkParams& p, int64_t t, float sc
         // Above 2^15 values would leave the range; below R 2^-14 what R values lose that are not normal numbers any more, 2^-25 each, would
         // be more than the rounding of the row's largest. Such rows have a power of two that brings the largest into [2^14, 2^15). The others do
         // without, so that chunks of one adapter can be summed on top of x W^T. us per call without / with: 4096 rows of 6 requests (4096 x 4096, R 32)
-        // 120 / 157, 512 rows of one (R 16) 32.4 / 35.4, 64 rows of 64 (K 4096, N 6144, R 16; never summed so) 21.1 / 21.9.
+        // 120 / 157, of R 128 129 / 180, 64 rows of 64 (K 4096, N 6144, R 16; never summed so) 21.1 / 21.9.
         const float most = warp_max(lane * 4 < p.R ? fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) : 0.0f);
         float up = 1.0f, down = 1.0f;
         if (most > 0.0f && most <= 3.402823466e38f && (most > 32768.0f || most < float(p.R) * 0x1p-14f)) {
